@@ -5,8 +5,8 @@
  * JNI, N-API). Every buffer is a CUDA device pointer unless a comment says
  * otherwise; every call enqueues on ctx->stream and never synchronizes, never
  * allocates on the hot path and validates all arguments before any launch.
- * Storage is FP32 (int32 for ids/counts/offsets/positions), contiguous,
- * row-major. Each entry point cites the RaggedRoute interface it replaces
+ * Storage is FP32 (int32 for ids/counts/offsets/positions; the expert-block
+ * operators take bfloat16 too), contiguous, row-major. Each entry point cites the RaggedRoute interface it replaces
  * (path:line relative to the RaggedRoute project root).
  *
  * Library-wide limits: 1 <= experts <= RR_MAX_EXPERTS (the reference caps
@@ -416,6 +416,116 @@ rr_status rr_ep_last_step_rows(const rr_ep* ep, int64_t* rows_sent, int64_t* row
 rr_status rr_ep_plan(const int32_t* count_all, int nranks, int rank, int experts,
                      int64_t* send_rows, int64_t* send_offsets, int64_t* recv_rows,
                      int64_t* recv_offsets);
+
+/* ---- expert-block operators (new: no reference counterpart) --------------
+ * What stands around the routing stages in a mixture-of-experts block: the
+ * gated projection of the experts with its backward pass, a grouped product
+ * in 8-bit integers, and the weighted combine with the norms, gate and
+ * residual at the block's end with its backward pass. Storage is FP32 or
+ * bfloat16 (dtype; the other buffers as declared), contiguous, row-major;
+ * rows whose length is a multiple of 16 bytes need 16-byte aligned buffers
+ * where an entry says so. Grouped rows are as for rr_grouped_gemm: segment e
+ * is rows [offsets[e], offsets[e+1]) of route_pairs rows (clipped to them);
+ * rows outside every segment are left as they were. Results repeat bit for
+ * bit: no entry accumulates with atomics. Values of RR_DTYPE_* equal
+ * raggedroute::ScalarType. */
+enum { RR_DTYPE_FP32 = 0, RR_DTYPE_BF16 = 2 };
+enum { RR_ACTIVATION_SILU = 0, RR_ACTIVATION_GELU_TANH = 1, RR_ACTIVATION_RELU = 2 };
+
+/* h[r] = act(x[r] . Wg[e]) * (x[r] . Wu[e]) for r in segment e, in one kernel:
+ * x_permuted [R, K], gate_weights and up_weights [E, K, N], h [R, N], all of
+ * dtype; sums in FP32, one rounding of h. gate_up (FP32 [R, 2N], may be NULL)
+ * receives both products (gate columns, then up), which the backward pass
+ * reads. FP32 operands are multiplied as three bfloat16 parts each (error of
+ * an FP32 product; a row or weight that holds an infinity may give NaN where
+ * FP32 arithmetic gives infinity). ctx->workspace (256-byte aligned) holds
+ * rr_grouped_gated_gemm_workspace_size bytes: 0 for bfloat16 with K and N
+ * multiples of 8 and for few rows; otherwise copies of the operands that the
+ * tensor cores can read (FP32: 6 bytes per element of x and of both weights).
+ * x, the weights, h and gate_up: 16-byte aligned where their rows are a
+ * multiple of 16 bytes. */
+rr_status rr_grouped_gated_gemm(const void* x_permuted, const void* gate_weights,
+                                const void* up_weights, const int32_t* offsets, void* h,
+                                float* gate_up, int route_pairs, int experts, int hidden,
+                                int output, int activation, int dtype, const rr_context* ctx);
+size_t rr_grouped_gated_gemm_workspace_size(int route_pairs, int experts, int hidden, int output,
+                                            int dtype);
+
+/* Gradients of rr_grouped_gated_gemm from dh [R, N] and the saved gate_up:
+ * dg = dh * u * act'(g), du = dh * act(g) (rounded to dtype), dx [R, K] =
+ * dg . Wg^T + du . Wu^T, d_gate_weights[e] = x_e^T dg_e, d_up_weights[e] =
+ * x_e^T du_e ([E, K, N], zero for an expert without rows). dx may be NULL, or
+ * both weight gradients. Rows of dx outside every segment are left as they
+ * were. The slope of RELU at 0 is 0. Alignment as above;
+ * rr_grouped_gated_gemm_backward_workspace_size bytes of workspace. */
+rr_status rr_grouped_gated_gemm_backward(const void* x_permuted, const void* gate_weights,
+                                         const void* up_weights, const int32_t* offsets,
+                                         const float* gate_up, const void* dh, void* dx,
+                                         void* d_gate_weights, void* d_up_weights,
+                                         int route_pairs, int experts, int hidden, int output,
+                                         int activation, int dtype, const rr_context* ctx);
+size_t rr_grouped_gated_gemm_backward_workspace_size(int route_pairs, int experts, int hidden,
+                                                     int output, int dtype);
+
+/* 8-bit integers. Quantised rows and weights are K-major with a row stride of
+ * rr_int8_row_stride(K) bytes (K rounded up to 16; the bytes past K are zero)
+ * and 16-byte aligned. */
+#define RR_MAX_INT8_HIDDEN 131072
+int rr_int8_row_stride(int hidden); /* 0 when K is out of range */
+
+/* Rows x [rows, K] of dtype: top = max |x| of a row, xq = rint(x * (127 / top))
+ * (both roundings FP32, ties to even), x_scale = top / 127. A row below 2^-120
+ * throughout counts as zero (xq = 0, scale 0). With an infinity or NaN in it
+ * the scale is that value and the row's products come out NaN. */
+rr_status rr_quantize_rows_int8(const void* x, int8_t* xq, float* x_scale, int rows, int hidden,
+                                int dtype, const rr_context* ctx);
+/* Expert weights W [E, K, N] of dtype, the same per output channel: wq
+ * [E, N, rr_int8_row_stride(K)], w_scale [E, N]. */
+rr_status rr_quantize_expert_weights_int8(const void* expert_weights, int8_t* wq, float* w_scale,
+                                          int experts, int hidden, int output, int dtype,
+                                          const rr_context* ctx);
+/* y[r, n] = (sum_k xq[r, k] * wq[e, n, k]) * x_scale[r] * w_scale[e, n] for r
+ * in segment e: the sum exact in 32-bit integers, the scaling in FP32, one
+ * rounding to dtype (y_permuted [R, N]). */
+rr_status rr_grouped_gemm_int8(const int8_t* xq, const float* x_scale, const int8_t* wq,
+                               const float* w_scale, const int32_t* offsets, void* y_permuted,
+                               int route_pairs, int experts, int hidden, int output, int dtype,
+                               const rr_context* ctx);
+
+/* rr_unpermute with what follows it in a block, in one kernel:
+ *   c  = sum_k route_weights[t, k] * y_permuted[route_pos[t, k]]
+ *   b  = c / sqrt(mean(c^2) + eps) * post_gamma     (b = c if post_gamma NULL)
+ *   r' = residual_scale * residual + gate * b       (gate NULL: 1)
+ *   normed = r' / sqrt(mean(r'^2) + eps) * pre_gamma   (both NULL: left out)
+ * y_permuted [T * top_k, N], residual, residual_out (= r') and normed [T, N]
+ * of dtype; post_gamma, gate, pre_gamma FP32 [N]; FP32 arithmetic, normed from
+ * the unrounded r'. inv_rms (FP32 [T, 2], may be NULL) receives both inverse
+ * roots for the backward pass (1 for a norm left out). residual_out may be
+ * residual. Routes whose position is outside [0, T * top_k) are skipped. Any
+ * alignment of the element types is accepted; 16-byte aligned rows are faster. */
+#define RR_MAX_NORM_OUTPUT 16384
+#define RR_MAX_NORM_TOP_K 64
+rr_status rr_unpermute_norm(const void* y_permuted, const int32_t* route_pos,
+                            const float* route_weights, const void* residual,
+                            const float* post_gamma, const float* gate, const float* pre_gamma,
+                            void* residual_out, void* normed, float* inv_rms, float eps,
+                            float residual_scale, int tokens, int top_k, int output, int dtype,
+                            const rr_context* ctx);
+/* Gradients of rr_unpermute_norm from d_residual_out and d_normed ([T, N],
+ * either NULL for zero) and the saved inv_rms: d_residual [T, N] (may be
+ * d_residual_out), d_y_permuted [T * top_k, N] (rows no route names are left
+ * as they were; distinct positions), d_route_weights FP32 [T, top_k] (0 for a
+ * skipped route), and FP32 [N] sums for the parameters that are wanted
+ * (d_post_gamma, d_gate, d_pre_gamma; each may be NULL).
+ * rr_unpermute_norm_backward_workspace_size bytes of workspace. */
+rr_status rr_unpermute_norm_backward(
+    const void* y_permuted, const int32_t* route_pos, const float* route_weights,
+    const void* residual, const float* post_gamma, const float* gate, const float* pre_gamma,
+    const float* inv_rms, const void* d_residual_out, const void* d_normed, void* d_residual,
+    void* d_y_permuted, float* d_route_weights, float* d_post_gamma, float* d_gate,
+    float* d_pre_gamma, float residual_scale, int tokens, int top_k, int output, int dtype,
+    const rr_context* ctx);
+size_t rr_unpermute_norm_backward_workspace_size(int tokens, int output);
 
 /* ---- low-level launchers (include/raggedroute/baseline_ops.h:14-42) ------
  * Return a cudaError_t value: cudaErrorInvalidValue (1) on bad arguments,

@@ -56,10 +56,24 @@ from raggedroute_b200.ops import (  # noqa: F401
     kernel_launch_count,
     grouped_gemm_engine,
 )
+from raggedroute_b200.expert_block import (  # noqa: F401
+    grouped_gated_gemm,
+    grouped_gated_gemm_backward,
+    grouped_gated_gemm_workspace_size,
+    grouped_gemm_int8,
+    int8_row_stride,
+    quantize_expert_weights_int8,
+    quantize_rows_int8,
+    unpermute_norm,
+    unpermute_norm_backward,
+    unpermute_norm_backward_workspace_size,
+)
 
 __all__ = [
     "dense_gemm", "topk_gate", "histogram", "exclusive_scan", "histogram_exclusive_scan",
     "token_permute", "grouped_gemm", "unpermute", "chain_from_tokens", "chain_from_logits",
-    "chain_from_route_ids",
+    "chain_from_route_ids", "grouped_gated_gemm", "grouped_gated_gemm_backward",
+    "quantize_rows_int8", "quantize_expert_weights_int8", "grouped_gemm_int8", "unpermute_norm",
+    "unpermute_norm_backward",
     "HostChain", "Context", "RaggedRouteError", "StatusCode", "lib",
 ]

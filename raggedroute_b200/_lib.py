@@ -103,6 +103,17 @@ SIGNATURES = {
     "rr_prepared_expert_weights_size": (ctypes.c_size_t, [_I, _I, _I]),
     "rr_prepare_expert_weights": (RRStatus, [_P, _I, _I, _I, _P, ctypes.c_size_t, _CTX]),
     "rr_grouped_gemm_prepared": (RRStatus, [_P, _P, _P, _P, _I, _I, _I, _I, _CTX]),
+    "rr_grouped_gated_gemm": (RRStatus, [_P] * 6 + [_I] * 6 + [_CTX]),
+    "rr_grouped_gated_gemm_workspace_size": (ctypes.c_size_t, [_I] * 5),
+    "rr_grouped_gated_gemm_backward": (RRStatus, [_P] * 9 + [_I] * 6 + [_CTX]),
+    "rr_grouped_gated_gemm_backward_workspace_size": (ctypes.c_size_t, [_I] * 5),
+    "rr_int8_row_stride": (_I, [_I]),
+    "rr_quantize_rows_int8": (RRStatus, [_P, _P, _P, _I, _I, _I, _CTX]),
+    "rr_quantize_expert_weights_int8": (RRStatus, [_P, _P, _P, _I, _I, _I, _I, _CTX]),
+    "rr_grouped_gemm_int8": (RRStatus, [_P] * 6 + [_I] * 5 + [_CTX]),
+    "rr_unpermute_norm": (RRStatus, [_P] * 10 + [ctypes.c_float] * 2 + [_I] * 4 + [_CTX]),
+    "rr_unpermute_norm_backward": (RRStatus, [_P] * 16 + [ctypes.c_float] + [_I] * 4 + [_CTX]),
+    "rr_unpermute_norm_backward_workspace_size": (ctypes.c_size_t, [_I, _I]),
     "rr_chain_from_route_ids": (RRStatus, [_P] * 11 + [_I] * 5 + [_CTX]),
     "rr_route_chain_workspace_size": (ctypes.c_size_t, [_I, _I, _I]),
     "rr_chain_from_logits": (RRStatus, [_P] * 11 + [_I] * 4 + [_CTX]),

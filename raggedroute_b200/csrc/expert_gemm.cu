@@ -1,0 +1,823 @@
+// Tensor-core engine of the expert block (tcgen05.mma.cta_group::2, sm_100a):
+// four ragged grouped products on one kernel, over segments
+// [offsets[e], offsets[e+1]) of grouped rows.
+//
+//   kGated  h = act(x Wg[e]) * (x Wu[e])             contraction over hidden
+//   kDx     dx = dg Wg[e]^T + du Wu[e]^T             contraction over 2 x output
+//   kDw     dWg[e] = x_e^T dg_e, dWu[e] = x_e^T du_e contraction over the rows
+//   kInt8   y = (xq . wq[e]^T) * xs[row] * ws[e][n]  contraction over hidden
+//
+// A pair of CTAs computes a 256-row tile whose 256 accumulator columns are 256
+// output columns (kDx, kInt8) or 128 columns of each of two products that
+// share their A operand (kGated: gate and up; kDw: the two weight gradients).
+// B is held half by each CTA, so in the second form the even CTA loads Wg (or
+// dg) and the odd CTA Wu (or du), and one MMA of N = 256 advances both
+// products: x is read once for both projections, and gate and up of an output
+// element meet in one thread's registers, where the activation and the
+// product are applied.
+//
+// Operands reach shared memory by TMA in 128-byte-swizzled boxes of 16 KB per
+// operand, part and k-block (64 bfloat16 or 128 int8 deep). Whatever layout
+// the tensors have in memory is used as it is: K-major where the contraction
+// is the contiguous axis (x in kGated, everything in kDx and kInt8), MN-major
+// where it is not (the weights in kGated, both operands of kDw), so no tensor
+// is transposed.
+//
+// FP32 (kTerms = 3): each operand is the exact sum of three bfloat16 parts
+// (8 + 8 + 8 significand bits), and the product sums the six part products of
+// weight 2^-16 and above; what is left out is below 2^-23 of |a||b|. The
+// tensor core truncates when it accumulates, with a bias that grows with the
+// number of steps taken at full magnitude, so every k-block is its own
+// accumulation, small products first (four full-magnitude steps), and the
+// epilogue warps add the blocks in FP32 registers while the next block runs
+// in the other half of TMEM.
+//
+// Roles (384 threads per CTA): warp 0 TMA producer; warp 1 MMA issuer (even
+// CTA); warp 2 relay: passes each landed stage on to the even CTA, and in kDw
+// clears the rows of a segment's last block that belong to other segments;
+// warps 4-11 epilogue. TMEM holds two 256-column accumulators, so a tile's
+// epilogue runs beside the next tile's products. Waits are bounded as in the
+// other pair engine (gemm_pair.cu), with the same exit protocol.
+#include <cuda.h>
+
+#include <mutex>
+
+#include "expert_block.cuh"
+#include "sm100.cuh"
+
+namespace rrb {
+namespace {
+
+using namespace sm100;
+
+enum Mode { kGated, kDx, kDw, kInt8 };
+
+constexpr int kRowsCta = 128;
+constexpr int kTileM = 2 * kRowsCta;
+constexpr int kTileN = 256;
+constexpr int kBoxBytes = 8192;            // 64 lines of 128 bytes
+constexpr int kOperandBytes = 2 * kBoxBytes;
+constexpr int kTmemCols = 512;
+constexpr int kEpiWarp0 = 4;
+constexpr int kEpiWarps = 8;
+constexpr int kThreads = (kEpiWarp0 + kEpiWarps) * 32;
+
+template <int kTerms>
+struct Config {
+  static constexpr int kStageBytes = 2 * kTerms * kOperandBytes;
+  static constexpr int kStages = kTerms == 1 ? 6 : 2;
+};
+
+struct EngineArgs {
+  const int32_t* offsets;
+  void* out0;
+  void* out1;
+  float* gate_up;
+  const float* row_scale;
+  const float* col_scale;
+  unsigned* err;
+  int experts, rows;
+  int hidden;   // contraction of kGated and kInt8; output columns of kDx, rows of kDw's tiles
+  int output;   // output columns of kGated, kDw, kInt8; contraction (twice) of kDx
+  int activation;
+  int vec;          // 16-byte stores of out0 / out1 allowed
+  int vec_gate_up;  // and of gate_up
+};
+
+template <int kTerms>
+struct alignas(1024) EngineSmem {
+  uint8_t stage[Config<kTerms>::kStages][Config<kTerms>::kStageBytes];
+  uint64_t full[Config<kTerms>::kStages];   // this CTA's TMA bytes landed
+  uint64_t empty[Config<kTerms>::kStages];  // the pair's MMAs have read the stage
+  uint64_t ready[Config<kTerms>::kStages];  // even CTA: both CTAs' halves are in place
+  uint64_t tmem_full[2];                    // accumulator finished (both CTAs)
+  uint64_t tmem_empty[2];                   // even CTA: both CTAs have read it
+  uint64_t mma_done;
+  uint32_t tmem_base;
+  int failed;
+  int issued[Config<kTerms>::kStages];
+  int prefix[kMaxExperts + 1];
+  int scratch[33];
+};
+
+// kind::f16 with bfloat16 operands and FP32 accumulation.
+__host__ __device__ constexpr uint32_t idesc_f16(int n, bool a_mn, bool b_mn) {
+  return (1u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(a_mn) << 15) |
+         (static_cast<uint32_t>(b_mn) << 16) | (static_cast<uint32_t>(n >> 3) << 17) |
+         (static_cast<uint32_t>(kTileM >> 4) << 24);
+}
+
+// kind::i8 with signed operands and 32-bit integer accumulation.
+__host__ __device__ constexpr uint32_t idesc_i8(int n) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n >> 3) << 17) |
+         (static_cast<uint32_t>(kTileM >> 4) << 24);
+}
+
+__device__ __forceinline__ void mma_i8_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                            uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+struct Tile {
+  int expert;
+  int m0, m_end;  // rows of the output (kDw: of the weight matrix)
+  int c0, ncols;  // columns of each product
+  int n_mma;      // accumulator columns, a multiple of 32
+  int blocks;     // k-blocks of the contraction
+  int row0, row_end;  // the segment (kDw's contraction)
+};
+
+__device__ __forceinline__ int tiles_of(int2 s, int n_tiles) {
+  return ((s.y - s.x + kTileM - 1) / kTileM) * n_tiles;
+}
+
+// Exclusive prefix of the experts' tile counts (all threads); the total.
+__device__ __forceinline__ int build_prefix(const EngineArgs& p, int n_tiles, int* prefix,
+                                            int* scratch) {
+  const int per = (p.experts + kThreads - 1) / kThreads;
+  const int e0 = min(p.experts, static_cast<int>(threadIdx.x) * per);
+  const int e1 = min(p.experts, e0 + per);
+  int local = 0;
+  for (int e = e0; e < e1; ++e) local += tiles_of(segment(p.offsets, e, p.rows), n_tiles);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int incl = local;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, incl, d);
+    if (lane >= d) incl += v;
+  }
+  if (lane == 31) scratch[warp] = incl;
+  __syncthreads();
+  int run = incl - local;
+  for (int w = 0; w < warp; ++w) run += scratch[w];
+  for (int e = e0; e < e1; ++e) {
+    prefix[e] = run;
+    run += tiles_of(segment(p.offsets, e, p.rows), n_tiles);
+  }
+  if (threadIdx.x == kThreads - 1) prefix[p.experts] = run;
+  __syncthreads();
+  return prefix[p.experts];
+}
+
+template <int kMode>
+__device__ __forceinline__ Tile tile_at(const EngineArgs& p, int t, const int* prefix,
+                                        int n_tiles) {
+  constexpr bool kTwo = kMode == kGated || kMode == kDw;  // two products side by side
+  Tile g;
+  int local;
+  if constexpr (kMode == kDw) {
+    const int per = ((p.hidden + kTileM - 1) / kTileM) * n_tiles;
+    g.expert = t / per;
+    local = t - g.expert * per;
+  } else {
+    int lo = 0, hi = p.experts - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (prefix[mid] <= t) lo = mid; else hi = mid - 1;
+    }
+    g.expert = lo;
+    local = t - prefix[lo];
+  }
+  const int2 s = segment(p.offsets, g.expert, p.rows);
+  g.row0 = s.x;
+  g.row_end = s.y;
+  const int mt = local / n_tiles, nt = local - mt * n_tiles;
+  const int width = kTwo ? kTileN / 2 : kTileN;
+  const int total = kMode == kDx ? p.hidden : p.output;
+  g.c0 = nt * width;
+  g.ncols = min(width, total - g.c0);
+  g.n_mma = kTwo ? 2 * ((g.ncols + 15) & ~15) : (g.ncols + 31) & ~31;
+  if constexpr (kMode == kDw) {
+    g.m0 = mt * kTileM;
+    g.m_end = p.hidden;
+    g.blocks = (s.y - s.x + 63) >> 6;
+  } else {
+    g.m0 = s.x + mt * kTileM;
+    g.m_end = s.y;
+    if constexpr (kMode == kDx) g.blocks = 2 * ((p.output + 63) >> 6);
+    else if constexpr (kMode == kInt8) g.blocks = (p.hidden + 127) >> 7;
+    else g.blocks = (p.hidden + 63) >> 6;
+  }
+  return g;
+}
+
+template <typename T>
+__device__ __forceinline__ void store16(T* dst, const float* v, int valid, bool vec) {
+  if (vec && valid >= 16) {
+    constexpr int kPer = 16 / sizeof(T);
+#pragma unroll
+    for (int i = 0; i < 16 / kPer; ++i) {
+      reinterpret_cast<uint4*>(dst)[i] = pack16<T>(v + kPer * i);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      if (i < valid) dst[i] = from_f32<T>(v[i]);
+    }
+  }
+}
+
+template <int kMode, int kTerms, typename T>
+__global__ void __launch_bounds__(kThreads, 1) expert_gemm_kernel(
+    const __grid_constant__ CUtensorMap map_a0, const __grid_constant__ CUtensorMap map_a1,
+    const __grid_constant__ CUtensorMap map_b0, const __grid_constant__ CUtensorMap map_b1,
+    const EngineArgs p) {
+  constexpr bool kTwo = kMode == kGated || kMode == kDw;
+  constexpr bool kMnA = kMode == kDw;
+  constexpr bool kMnB = kMode == kGated || kMode == kDw;
+  constexpr int kStages = Config<kTerms>::kStages;
+  constexpr uint32_t kStageTx = Config<kTerms>::kStageBytes;
+  constexpr int kOffB = kTerms * kOperandBytes;
+  // Byte step of one K = 16 (bfloat16) or 32 (int8) MMA inside a box, and the
+  // descriptors' offsets: K-major tiles repeat every 8 rows of 128 bytes;
+  // MN-major ones every 8 k-lines of 128 bytes, the next 64 columns one box on.
+  constexpr uint32_t kStepA = kMnA ? 2048 : 32, kStepB = kMnB ? 2048 : 32;
+  constexpr uint32_t kLboA = kMnA ? kBoxBytes : 16, kLboB = kMnB ? kBoxBytes : 16;
+
+  extern __shared__ uint8_t smem_raw[];
+  auto& s = *reinterpret_cast<EngineSmem<kTerms>*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const bool leader = rank == 0;
+  const int unit = static_cast<int>(blockIdx.x >> 1);
+  const int units = static_cast<int>(gridDim.x >> 1);
+  const int n_tiles = ((kMode == kDx ? p.hidden : p.output) + (kTwo ? kTileN / 2 : kTileN) - 1) /
+                      (kTwo ? kTileN / 2 : kTileN);
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&s.full[i], 1);
+      mbar_init(&s.empty[i], 1);
+      mbar_init(&s.ready[i], 2);
+      s.issued[i] = 0;
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s.tmem_full[i], 1);
+      mbar_init(&s.tmem_empty[i], 2 * kEpiWarps);
+    }
+    mbar_init(&s.mma_done, 1);
+    s.failed = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(&s.tmem_base, kTmemCols);
+    tmem_relinquish_pair();
+  }
+  int total;
+  if constexpr (kMode == kDw) {
+    total = p.experts * ((p.hidden + kTileM - 1) / kTileM) * n_tiles;
+  } else {
+    total = build_prefix(p, n_tiles, s.prefix, s.scratch);
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem = s.tmem_base;
+  volatile int* failed = &s.failed;
+  const uint32_t peer_failed = mapa_shared(smem_u32(&s.failed), rank ^ 1u);
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    return mbar_wait_pair(bar, parity, p.err, failed, peer_failed);
+  };
+
+  if (warp == 0) {
+    // ---------------- TMA producer ----------------
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      for (int t = unit; t < total && !*failed; t += units) {
+        const Tile g = tile_at<kMode>(p, t, s.prefix, n_tiles);
+        const int m = g.m0 + static_cast<int>(rank) * kRowsCta;
+        const int half = g.n_mma >> 1;
+        for (int kb = 0; kb < g.blocks; ++kb) {
+          if (!wait(&s.empty[stage], phase ^ 1u)) break;
+          uint8_t* a = s.stage[stage];
+          uint8_t* b = a + kOffB;
+          uint64_t* bar = &s.full[stage];
+          mbar_arrive_expect_tx(bar, kStageTx);
+#pragma unroll
+          for (int q = 0; q < kTerms; ++q, a += kOperandBytes, b += kOperandBytes) {
+            if constexpr (kMode == kGated) {
+              const CUtensorMap* mb = leader ? &map_b0 : &map_b1;
+              tma_load_3d(a, &map_a0, bar, kb * 64, m, q);
+              tma_load_3d(b, mb, bar, g.c0, kb * 64, q * p.experts + g.expert);
+              tma_load_3d(b + kBoxBytes, mb, bar, g.c0 + 64, kb * 64, q * p.experts + g.expert);
+            } else if constexpr (kMode == kDx) {
+              const int per = g.blocks >> 1;
+              const bool first = kb < per;
+              const int k = (first ? kb : kb - per) * 64;
+              tma_load_3d(a, first ? &map_a0 : &map_a1, bar, k, m, q);
+              tma_load_3d(b, first ? &map_b0 : &map_b1, bar, k,
+                          g.c0 + static_cast<int>(rank) * half, q * p.experts + g.expert);
+            } else if constexpr (kMode == kDw) {
+              const CUtensorMap* mb = leader ? &map_b0 : &map_b1;
+              const int r = g.row0 + kb * 64;
+              tma_load_3d(a, &map_a0, bar, m, r, q);
+              tma_load_3d(a + kBoxBytes, &map_a0, bar, m + 64, r, q);
+              tma_load_3d(b, mb, bar, g.c0, r, q);
+              tma_load_3d(b + kBoxBytes, mb, bar, g.c0 + 64, r, q);
+            } else {
+              tma_load_3d(a, &map_a0, bar, kb * 128, m, 0);
+              tma_load_3d(b, &map_b0, bar, kb * 128, g.c0 + static_cast<int>(rank) * half,
+                          g.expert);
+            }
+          }
+          s.issued[stage] += 1;
+          if (++stage == kStages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+      // Wait for the MMAs' last use of every stage: nothing may read or signal
+      // this CTA's shared memory after it exits.
+      for (int i = 0; i < kStages && !*failed; ++i) {
+        if (!wait(&s.empty[stage], phase ^ 1u)) break;
+        if (++stage == kStages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ---------------- MMA issuer (even CTA) ----------------
+    if (leader && lane == 0) {
+      int stage = 0, buf = 0;
+      uint32_t phase = 0, acc_phase = 0;
+      bool ok = true;
+      for (int t = unit; t < total && ok && !*failed; t += units) {
+        const Tile g = tile_at<kMode>(p, t, s.prefix, n_tiles);
+        const uint32_t idesc =
+            kMode == kInt8 ? idesc_i8(g.n_mma) : idesc_f16(g.n_mma, kMnA, kMnB);
+        for (int kb = 0; kb < g.blocks && ok; ++kb) {
+          const bool opens = kTerms == 3 || kb == 0;
+          if (opens && !wait(&s.tmem_empty[buf], acc_phase ^ 1u)) {
+            ok = false;
+            break;
+          }
+          if (!wait(&s.ready[stage], phase)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t d = tmem + static_cast<uint32_t>(buf) * kTileN;
+          const uint32_t base = smem_u32(s.stage[stage]);
+          const uint64_t a0 = smem_desc(base, kLboA, 1024, Swizzle::k128B);
+          const uint64_t b0 = smem_desc(base + kOffB, kLboB, 1024, Swizzle::k128B);
+          if constexpr (kTerms == 1) {
+#pragma unroll
+            for (uint32_t ks = 0; ks < 4; ++ks) {
+              const uint64_t ad = a0 + ks * (kStepA >> 4), bd = b0 + ks * (kStepB >> 4);
+              const uint32_t acc = (kb > 0 || ks > 0) ? 1u : 0u;
+              if constexpr (kMode == kInt8) mma_i8_pair(d, ad, bd, idesc, acc);
+              else mma_bf16_pair(d, ad, bd, idesc, acc);
+            }
+          } else {
+            // Parts (a, b) in rising magnitude: 2^-16 three times, 2^-8 twice, 1.
+            constexpr int kPa[6] = {2, 0, 1, 1, 0, 0};
+            constexpr int kPb[6] = {0, 2, 1, 0, 1, 0};
+#pragma unroll
+            for (int q = 0; q < 6; ++q) {
+#pragma unroll
+              for (uint32_t ks = 0; ks < 4; ++ks) {
+                mma_bf16_pair(d, a0 + kPa[q] * (kOperandBytes >> 4) + ks * (kStepA >> 4),
+                              b0 + kPb[q] * (kOperandBytes >> 4) + ks * (kStepB >> 4), idesc,
+                              (q > 0 || ks > 0) ? 1u : 0u);
+              }
+            }
+          }
+          const uint32_t e = smem_u32(&s.empty[stage]);
+          mma_commit_pair_to(e);
+          mma_commit_pair_to(mapa_shared(e, 1u));
+          if (++stage == kStages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+          if (kTerms == 3 || kb + 1 == g.blocks) {
+            const uint32_t f = smem_u32(&s.tmem_full[buf]);
+            mma_commit_pair_to(f);
+            mma_commit_pair_to(mapa_shared(f, 1u));
+            buf ^= 1;
+            if (buf == 0) acc_phase ^= 1u;
+          }
+        }
+      }
+      mma_commit_pair_to(smem_u32(&s.mma_done));
+      int dummy = 0;
+      mbar_wait(&s.mma_done, 0, p.err, &dummy);
+    }
+  } else if (warp == 2) {
+    // ---------------- relay ----------------
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int t = unit; t < total && ok && !*failed; t += units) {
+      const Tile g = tile_at<kMode>(p, t, s.prefix, n_tiles);
+      for (int kb = 0; kb < g.blocks; ++kb) {
+        if (!wait(&s.full[stage], phase)) {
+          ok = false;
+          break;
+        }
+        if constexpr (kMode == kDw) {
+          // Lines past the segment's end hold other segments' rows (or
+          // anything): both operands become zero there. A line is one row of
+          // a box, so the swizzle inside it does not matter.
+          const int valid = g.row_end - g.row0 - kb * 64;
+          if (valid < 64) {
+            for (int bx = 0; bx < 4 * kTerms; ++bx) {
+              uint8_t* box = s.stage[stage] + bx * kBoxBytes;
+              for (int i = valid * 8 + lane; i < 512; i += 32) {
+                reinterpret_cast<uint4*>(box)[i] = make_uint4(0u, 0u, 0u, 0u);
+              }
+            }
+            fence_proxy_async_smem();
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive_remote(mapa_shared(smem_u32(&s.ready[stage]), 0u));
+        if (++stage == kStages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+    }
+  } else if (warp >= kEpiWarp0) {
+    // ---------------- epilogue ----------------
+    const int quarter = warp & 3;
+    const int hw = (warp - kEpiWarp0) >> 2;
+    const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
+    int buf = 0;
+    uint32_t acc_phase = 0;
+    bool ok = true;
+    for (int t = unit; t < total && ok && !*failed; t += units) {
+      const Tile g = tile_at<kMode>(p, t, s.prefix, n_tiles);
+      const int half = g.n_mma >> 1;
+      const int row = g.m0 + static_cast<int>(rank) * kRowsCta + quarter * 32 + lane;
+      const bool live = row < g.m_end;
+      // Piece q of 16 accumulator columns of this warp: kGated has gate
+      // columns in pieces 0-3 and the up columns they meet in 4-7.
+      auto piece_col = [&](int q) {
+        if constexpr (kMode == kGated) {
+          return (q < 4 ? 0 : half) + hw * 64 + 16 * (q & 3);
+        } else if constexpr (kMode == kDw) {
+          return hw * half + 16 * q;
+        } else {
+          return hw * 128 + 16 * q;
+        }
+      };
+      auto piece_live = [&](int q) {  // warp-uniform
+        if constexpr (kMode == kGated) return hw * 64 + 16 * (q & 3) < half;
+        else if constexpr (kMode == kDw) return 16 * q < half;
+        else return hw * 128 + 16 * q < g.n_mma;
+      };
+      auto put = [&](int q, const float* v, const float* v2) {
+        if constexpr (kMode == kGated) {
+          const int c = hw * 64 + 16 * q;
+          const int valid = min(16, g.ncols - c);
+          if (!live || valid <= 0) return;
+          float h[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) h[i] = activate(p.activation, v[i]) * v2[i];
+          const long long at = static_cast<long long>(row) * p.output + g.c0 + c;
+          store16(static_cast<T*>(p.out0) + at, h, valid, p.vec != 0);
+          if (p.gate_up != nullptr) {
+            float* gu = p.gate_up + 2LL * row * p.output + g.c0 + c;
+            store16(gu, v, valid, p.vec_gate_up != 0);
+            store16(gu + p.output, v2, valid, p.vec_gate_up != 0);
+          }
+        } else if constexpr (kMode == kDw) {
+          const int valid = min(16, g.ncols - 16 * q);
+          if (!live || valid <= 0) return;
+          T* out = static_cast<T*>(hw == 0 ? p.out0 : p.out1) +
+                   (static_cast<long long>(g.expert) * p.hidden + row) * p.output + g.c0 + 16 * q;
+          store16(out, v, valid, p.vec != 0);
+        } else {
+          const int c = hw * 128 + 16 * q;
+          const int valid = min(16, g.ncols - c);
+          if (!live || valid <= 0) return;
+          const int ld = kMode == kDx ? p.hidden : p.output;
+          T* out = static_cast<T*>(p.out0) + static_cast<long long>(row) * ld + g.c0 + c;
+          if constexpr (kMode == kInt8) {
+            const float xs = __ldg(p.row_scale + row);
+            const float* ws =
+                p.col_scale + static_cast<long long>(g.expert) * p.output + g.c0 + c;
+            float y[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              y[i] = static_cast<float>(__float_as_int(v[i])) * xs *
+                     (i < valid ? __ldg(ws + i) : 0.0f);
+            }
+            store16(out, y, valid, p.vec != 0);
+          } else {
+            store16(out, v, valid, p.vec != 0);
+          }
+        }
+      };
+      auto load = [&](int q, float* v) {
+        uint32_t r[16];
+        tmem_ld_32x32b_x16(
+            tmem + static_cast<uint32_t>(buf * kTileN + piece_col(q)) + lane_addr, r);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+      };
+      auto take = [&]() {  // the accumulator is finished
+        if (!wait(&s.tmem_full[buf], acc_phase)) return false;
+        tc_fence_after();
+        return true;
+      };
+      auto release = [&]() {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_remote(mapa_shared(smem_u32(&s.tmem_empty[buf]), 0u));
+        buf ^= 1;
+        if (buf == 0) acc_phase ^= 1u;
+      };
+      if constexpr (kMode == kDw) {
+        if (g.blocks == 0) {  // no rows: a zero gradient
+          const float zero[16] = {};
+          for (int q = 0; q < 8; ++q) put(q, zero, zero);
+          continue;
+        }
+      }
+      if constexpr (kTerms == 1) {
+        if (!take()) break;
+        if constexpr (kMode == kGated) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            if (!piece_live(q)) break;
+            float v[16], v2[16];
+            load(q, v);
+            load(q + 4, v2);
+            put(q, v, v2);
+          }
+        } else {
+#pragma unroll
+          for (int q = 0; q < 8; ++q) {
+            if (!piece_live(q)) break;
+            float v[16];
+            load(q, v);
+            put(q, v, v);
+          }
+        }
+        release();
+      } else {
+        float sum[128];
+#pragma unroll
+        for (int i = 0; i < 128; ++i) sum[i] = 0.0f;
+        for (int kb = 0; kb < g.blocks; ++kb) {
+          if (!take()) {
+            ok = false;
+            break;
+          }
+#pragma unroll
+          for (int q = 0; q < 8; ++q) {
+            if (piece_live(q)) {
+              float v[16];
+              load(q, v);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) sum[16 * q + i] += v[i];
+            }
+          }
+          release();
+        }
+        if (!ok) break;
+#pragma unroll
+        for (int q = 0; q < (kMode == kGated ? 4 : 8); ++q) {
+          put(q, sum + 16 * q, sum + (16 * q + (kMode == kGated ? 64 : 0)));
+        }
+      }
+    }
+  }
+
+  __syncthreads();
+  if (warp == 0 && lane == 0 && *failed) {
+    // Drain TMA loads still in flight into this CTA's shared memory.
+    for (int i = 0; i < kStages; ++i) {
+      if (s.issued[i] > 0) {
+        int dummy = 0;
+        mbar_wait(&s.full[i], static_cast<uint32_t>((s.issued[i] - 1) & 1), p.err, &dummy);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // the pair's MMAs are done; no arrivals into either CTA remain
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc_pair(tmem, kTmemCols);
+}
+
+// ---- host side -----------------------------------------------------------------
+
+// [d2][d1][d0] elements with row stride ld (elements) and plane stride d1 * ld.
+bool encode_map(CUtensorMap* map, const void* base, bool int8, long long d0, long long d1,
+                long long d2, long long ld, int box0, int box1) {
+  EncodeTiledFn encode = tensor_map_encoder();
+  if (encode == nullptr) return false;
+  const cuuint64_t size = int8 ? 1 : 2;
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(d0), static_cast<cuuint64_t>(d1),
+                              static_cast<cuuint64_t>(d2)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(ld) * size,
+                                 static_cast<cuuint64_t>(ld) * size * dims[1]};
+  const cuuint32_t box[3] = {static_cast<cuuint32_t>(box0), static_cast<cuuint32_t>(box1), 1};
+  const cuuint32_t step[3] = {1, 1, 1};
+  return encode(map, int8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+                const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+constexpr int kMaxDevices = 64;
+
+// CTA pairs the device can hold at once, per kernel and device; 0 when the
+// kernel cannot be configured there.
+template <int kMode, int kTerms, typename T>
+int engine_units(std::size_t smem) {
+  static std::mutex mutex;
+  static int known[kMaxDevices] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return 0;
+  std::lock_guard<std::mutex> lock(mutex);
+  if (known[dev] == 0) {
+    auto* kernel = expert_gemm_kernel<kMode, kTerms, T>;
+    int n = 0;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             static_cast<int>(smem)) == cudaSuccess) {
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = 2;
+      attr[0].val.clusterDim.y = 1;
+      attr[0].val.clusterDim.z = 1;
+      cudaLaunchConfig_t cfg{};
+      cfg.gridDim = dim3(2 * sm_count(), 1, 1);
+      cfg.blockDim = dim3(kThreads, 1, 1);
+      cfg.dynamicSmemBytes = smem;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) n = 0;
+    }
+    if (n <= 0) {
+      cudaGetLastError();
+      return 0;
+    }
+    known[dev] = n;
+  }
+  return known[dev];
+}
+
+template <int kMode, int kTerms, typename T>
+cudaError_t launch_engine(const CUtensorMap (&maps)[4], EngineArgs args, long long tiles,
+                          cudaStream_t stream) {
+  constexpr std::size_t smem = sizeof(EngineSmem<kTerms>) + 1024;
+  static_assert(smem <= 227 * 1024, "over the shared memory a CTA may use");
+  int units = engine_units<kMode, kTerms, T>(smem);
+  if (units <= 0) return cudaErrorNotSupported;
+  if (tiles < units) units = static_cast<int>(tiles);
+  if (units <= 0) return cudaSuccess;
+  args.err = device_error_word();
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(2 * units, 1, 1);
+  cfg.blockDim = dim3(kThreads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, expert_gemm_kernel<kMode, kTerms, T>, maps[0],
+                                           maps[1], maps[2], maps[3], args);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return e;
+  }
+  note_launch();
+  return cudaSuccess;
+}
+
+// Output tiles of the row modes, at most: every expert with rows may end in a
+// partial one.
+long long row_tiles(int rows, int experts, int columns, int width) {
+  const long long m = rows / kTileM + (experts < rows ? experts : rows);
+  return m * ceil_div(columns, width);
+}
+
+bool vec_ok(const void* p, int ld, Dtype t) {
+  return p == nullptr || (aligned_to(p, 16) && (ld * dtype_bytes(t)) % 16 == 0);
+}
+
+}  // namespace
+
+cudaError_t launch_gated_gemm(const GatedOperands& in, const int32_t* offsets, void* h,
+                              float* gate_up, int rows, int experts, int hidden, int output,
+                              Activation activation, Dtype dtype, cudaStream_t stream) {
+  CUtensorMap maps[4] = {};
+  const long long planes = static_cast<long long>(in.terms) * experts;
+  if (!encode_map(&maps[0], in.x, false, hidden, rows, in.terms, in.ldk, 64, kRowsCta) ||
+      !encode_map(&maps[2], in.wg, false, output, hidden, planes, in.ldn, 64, 64) ||
+      !encode_map(&maps[3], in.wu, false, output, hidden, planes, in.ldn, 64, 64)) {
+    return cudaErrorInvalidValue;
+  }
+  maps[1] = maps[0];
+  EngineArgs a{};
+  a.offsets = offsets;
+  a.out0 = h;
+  a.gate_up = gate_up;
+  a.experts = experts;
+  a.rows = rows;
+  a.hidden = hidden;
+  a.output = output;
+  a.activation = static_cast<int>(activation);
+  a.vec = vec_ok(h, output, dtype);
+  a.vec_gate_up = vec_ok(gate_up, output, Dtype::kFp32);
+  const long long tiles = row_tiles(rows, experts, output, kTileN / 2);
+  return dtype == Dtype::kBf16 ? launch_engine<kGated, 1, __nv_bfloat16>(maps, a, tiles, stream)
+                               : launch_engine<kGated, 3, float>(maps, a, tiles, stream);
+}
+
+cudaError_t launch_gated_dx(const GatedOperands& in, const __nv_bfloat16* dg,
+                            const __nv_bfloat16* du, const int32_t* offsets, void* dx, int rows,
+                            int experts, int hidden, int output, Dtype dtype,
+                            cudaStream_t stream) {
+  CUtensorMap maps[4] = {};
+  const long long planes = static_cast<long long>(in.terms) * experts;
+  if (!encode_map(&maps[0], dg, false, output, rows, in.terms, in.ldn, 64, kRowsCta) ||
+      !encode_map(&maps[1], du, false, output, rows, in.terms, in.ldn, 64, kRowsCta) ||
+      !encode_map(&maps[2], in.wg, false, output, hidden, planes, in.ldn, 64, kRowsCta) ||
+      !encode_map(&maps[3], in.wu, false, output, hidden, planes, in.ldn, 64, kRowsCta)) {
+    return cudaErrorInvalidValue;
+  }
+  EngineArgs a{};
+  a.offsets = offsets;
+  a.out0 = dx;
+  a.experts = experts;
+  a.rows = rows;
+  a.hidden = hidden;
+  a.output = output;
+  a.vec = vec_ok(dx, hidden, dtype);
+  const long long tiles = row_tiles(rows, experts, hidden, kTileN);
+  return dtype == Dtype::kBf16 ? launch_engine<kDx, 1, __nv_bfloat16>(maps, a, tiles, stream)
+                               : launch_engine<kDx, 3, float>(maps, a, tiles, stream);
+}
+
+cudaError_t launch_gated_dw(const GatedOperands& in, const __nv_bfloat16* dg,
+                            const __nv_bfloat16* du, const int32_t* offsets, void* dwg, void* dwu,
+                            int rows, int experts, int hidden, int output, Dtype dtype,
+                            cudaStream_t stream) {
+  CUtensorMap maps[4] = {};
+  if (!encode_map(&maps[0], in.x, false, hidden, rows, in.terms, in.ldk, 64, 64) ||
+      !encode_map(&maps[2], dg, false, output, rows, in.terms, in.ldn, 64, 64) ||
+      !encode_map(&maps[3], du, false, output, rows, in.terms, in.ldn, 64, 64)) {
+    return cudaErrorInvalidValue;
+  }
+  maps[1] = maps[0];
+  EngineArgs a{};
+  a.offsets = offsets;
+  a.out0 = dwg;
+  a.out1 = dwu;
+  a.experts = experts;
+  a.rows = rows;
+  a.hidden = hidden;
+  a.output = output;
+  a.vec = vec_ok(dwg, output, dtype) && vec_ok(dwu, output, dtype);
+  const long long tiles = static_cast<long long>(experts) * ceil_div(hidden, kTileM) *
+                          ceil_div(output, kTileN / 2);
+  return dtype == Dtype::kBf16 ? launch_engine<kDw, 1, __nv_bfloat16>(maps, a, tiles, stream)
+                               : launch_engine<kDw, 3, float>(maps, a, tiles, stream);
+}
+
+cudaError_t launch_int8_gemm(const int8_t* xq, const float* x_scale, const int8_t* wq,
+                             const float* w_scale, const int32_t* offsets, void* y, int rows,
+                             int experts, int ld, int output, Dtype dtype, cudaStream_t stream) {
+  CUtensorMap maps[4] = {};
+  if (!encode_map(&maps[0], xq, true, ld, rows, 1, ld, 128, kRowsCta) ||
+      !encode_map(&maps[2], wq, true, ld, output, experts, ld, 128, kRowsCta)) {
+    return cudaErrorInvalidValue;
+  }
+  maps[1] = maps[0];
+  maps[3] = maps[2];
+  EngineArgs a{};
+  a.offsets = offsets;
+  a.out0 = y;
+  a.row_scale = x_scale;
+  a.col_scale = w_scale;
+  a.experts = experts;
+  a.rows = rows;
+  a.hidden = ld;
+  a.output = output;
+  a.vec = vec_ok(y, output, dtype);
+  const long long tiles = row_tiles(rows, experts, output, kTileN);
+  return dtype == Dtype::kBf16 ? launch_engine<kInt8, 1, __nv_bfloat16>(maps, a, tiles, stream)
+                               : launch_engine<kInt8, 1, float>(maps, a, tiles, stream);
+}
+
+}  // namespace rrb

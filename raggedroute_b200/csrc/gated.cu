@@ -1,0 +1,365 @@
+// The parts of the gated expert projection around the tensor-core engine
+// (expert_gemm.cu): the form for a few rows, the packing of operands the
+// engine cannot read as they are, and the pointwise half of the gradient.
+#include "expert_block.cuh"
+
+namespace rrb {
+namespace {
+
+// ---- few rows --------------------------------------------------------------------
+//
+// h[r, c] = act(sum_k x[r, k] Wg[e][k, c]) * sum_k x[r, k] Wu[e][k, c] for a
+// handful of rows: bound by reading the weights of the experts that have
+// rows, 2 K N elements each, once. One block takes 32 columns of up to kRows
+// rows of one expert, 16 bytes of each matrix per thread and k-step, with the
+// contraction spread over the block's threads: the partial sums (FP32) meet
+// by shuffles and in shared memory, in a fixed order. No block waits on
+// another, and gate and up of a column meet in the block that owns it.
+
+constexpr int kFewThreads = 256;
+constexpr int kFewWarps = kFewThreads / 32;
+constexpr int kFewCols = 32;
+constexpr int kFewRows = 4;
+
+__device__ __forceinline__ uint4 ld_stream16(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
+
+template <typename T, int kVec>
+__device__ __forceinline__ void load_vec(const T* p, float* f) {
+  if constexpr (kVec == 1) f[0] = to_f32(__ldg(p));
+  else unpack16<T>(ld_stream16(p), f);
+}
+
+template <typename T, int kVec, int kR>
+__device__ __forceinline__ void few_rows(const T* __restrict__ x, const T* __restrict__ wg,
+                                         const T* __restrict__ wu, T* __restrict__ h,
+                                         float* __restrict__ gate_up, int row, int nrows,
+                                         int hidden, int output, int c0, int activation,
+                                         float* red) {
+  constexpr int kLanes = kFewCols / kVec;       // lanes across the columns
+  constexpr int kGroups = kFewThreads / kLanes;  // contraction groups
+  constexpr int kUnroll = 4;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int col = (threadIdx.x % kLanes) * kVec;
+  const int kg = threadIdx.x / kLanes;
+  float g[kR][kVec], u[kR][kVec];
+#pragma unroll
+  for (int i = 0; i < kR; ++i) {
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) g[i][j] = u[i][j] = 0.0f;
+  }
+  if (c0 + col < output) {
+    const T* pg = wg + c0 + col;
+    const T* pu = wu + c0 + col;
+    const T* px[kR];
+#pragma unroll
+    for (int i = 0; i < kR; ++i) {
+      px[i] = x + static_cast<long long>(row + min(i, nrows - 1)) * hidden;
+    }
+    auto step = [&](int k, const float* a, const float* b) {
+#pragma unroll
+      for (int i = 0; i < kR; ++i) {
+        const float v = to_f32(__ldg(px[i] + k));
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) {
+          g[i][j] = fmaf(v, a[j], g[i][j]);
+          u[i][j] = fmaf(v, b[j], u[i][j]);
+        }
+      }
+    };
+    int k = kg;
+    for (; k + (kUnroll - 1) * kGroups < hidden; k += kUnroll * kGroups) {
+      float a[kUnroll][kVec], b[kUnroll][kVec];
+#pragma unroll
+      for (int q = 0; q < kUnroll; ++q) {
+        const long long at = static_cast<long long>(k + q * kGroups) * output;
+        load_vec<T, kVec>(pg + at, a[q]);
+        load_vec<T, kVec>(pu + at, b[q]);
+      }
+#pragma unroll
+      for (int q = 0; q < kUnroll; ++q) step(k + q * kGroups, a[q], b[q]);
+    }
+    for (; k < hidden; k += kGroups) {
+      float a[kVec], b[kVec];
+      const long long at = static_cast<long long>(k) * output;
+      load_vec<T, kVec>(pg + at, a);
+      load_vec<T, kVec>(pu + at, b);
+      step(k, a, b);
+    }
+  }
+  // Sum over the contraction groups: lanes of a warp, then warps.
+#pragma unroll
+  for (int i = 0; i < kR; ++i) {
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) {
+#pragma unroll
+      for (int d = kLanes; d < 32; d <<= 1) {
+        g[i][j] += __shfl_xor_sync(0xffffffffu, g[i][j], d);
+        u[i][j] += __shfl_xor_sync(0xffffffffu, u[i][j], d);
+      }
+      if (lane < kLanes) {
+        red[((warp * kR + i) * 2) * kFewCols + col + j] = g[i][j];
+        red[((warp * kR + i) * 2 + 1) * kFewCols + col + j] = u[i][j];
+      }
+    }
+  }
+  __syncthreads();
+  const int i = threadIdx.x / kFewCols, c = threadIdx.x % kFewCols;
+  if (i < nrows && i < kR && c0 + c < output) {
+    float sg = 0.0f, su = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kFewWarps; ++w) {
+      sg += red[((w * kR + i) * 2) * kFewCols + c];
+      su += red[((w * kR + i) * 2 + 1) * kFewCols + c];
+    }
+    const long long r = row + i;
+    h[r * output + c0 + c] = from_f32<T>(activate(activation, sg) * su);
+    if (gate_up != nullptr) {
+      gate_up[2 * r * output + c0 + c] = sg;
+      gate_up[(2 * r + 1) * output + c0 + c] = su;
+    }
+  }
+}
+
+template <typename T, int kVec>
+__global__ void __launch_bounds__(kFewThreads) gated_few_kernel(
+    const T* __restrict__ x, const T* __restrict__ wg, const T* __restrict__ wu,
+    const int32_t* __restrict__ offsets, T* __restrict__ h, float* __restrict__ gate_up, int rows,
+    int experts, int hidden, int output, int activation) {
+  __shared__ int owner;
+  __shared__ float red[kFewWarps * kFewRows * 2 * kFewCols];
+  if (threadIdx.x == 0) owner = experts;
+  __syncthreads();
+  const int row = blockIdx.y;
+  for (int e = threadIdx.x; e < experts; e += kFewThreads) {
+    const int2 s = segment(offsets, e, rows);
+    if (s.x <= row && row < s.y) atomicMin(&owner, e);
+  }
+  __syncthreads();
+  const int e = owner;
+  if (e == experts) return;  // a row outside every segment
+  const int2 s = segment(offsets, e, rows);
+  if ((row - s.x) % kFewRows != 0) return;  // an earlier block's row
+  const int nrows = min(kFewRows, s.y - row);
+  const int c0 = blockIdx.x * kFewCols;
+  const long long at = static_cast<long long>(e) * hidden * output;
+  if (nrows == 1) {
+    few_rows<T, kVec, 1>(x, wg + at, wu + at, h, gate_up, row, nrows, hidden, output, c0,
+                         activation, red);
+  } else {
+    few_rows<T, kVec, kFewRows>(x, wg + at, wu + at, h, gate_up, row, nrows, hidden, output, c0,
+                                activation, red);
+  }
+}
+
+template <typename T>
+cudaError_t few(const void* x, const void* wg, const void* wu, const int32_t* offsets, void* h,
+                float* gate_up, int rows, int experts, int hidden, int output, int activation,
+                cudaStream_t stream) {
+  constexpr int kVec = 16 / sizeof(T);
+  const dim3 grid(ceil_div(output, kFewCols), rows);
+  const bool vec = output % kVec == 0 && aligned_to(wg, 16) && aligned_to(wu, 16);
+  auto* kernel = vec ? gated_few_kernel<T, kVec> : gated_few_kernel<T, 1>;
+  kernel<<<grid, kFewThreads, 0, stream>>>(
+      static_cast<const T*>(x), static_cast<const T*>(wg), static_cast<const T*>(wu), offsets,
+      static_cast<T*>(h), gate_up, rows, experts, hidden, output, activation);
+  note_launch();
+  return cudaGetLastError();
+}
+
+// ---- operand parts -----------------------------------------------------------------
+
+// v as the exact sum of three bfloat16 values: each takes the top 8
+// significand bits of what is left (truncation, so nothing overflows).
+// Infinity and NaN stay in the first part.
+__device__ __forceinline__ void split3(float v, uint16_t (&part)[3]) {
+  const uint32_t bits = __float_as_uint(v);
+  if ((bits & 0x7F800000u) == 0x7F800000u) {
+    part[0] = static_cast<uint16_t>(bits >> 16) | ((bits & 0x007FFFFFu) != 0 ? 0x40u : 0u);
+    part[1] = part[2] = 0;
+    return;
+  }
+  float rest = v;
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    const uint32_t b = __float_as_uint(rest) & 0xFFFF0000u;
+    part[i] = static_cast<uint16_t>(b >> 16);
+    rest -= __uint_as_float(b);
+  }
+}
+
+// Eight values as one 16-byte store per part; planes `plane` elements apart.
+template <int kTerms>
+__device__ __forceinline__ void store_parts(__nv_bfloat16* dst, long long plane,
+                                            const float (&v)[8]) {
+  if constexpr (kTerms == 1) {
+    *reinterpret_cast<uint4*>(dst) = pack16<__nv_bfloat16>(v);
+  } else {
+    uint32_t w[3][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint16_t lo[3], hi[3];
+      split3(v[2 * i], lo);
+      split3(v[2 * i + 1], hi);
+#pragma unroll
+      for (int q = 0; q < 3; ++q) w[q][i] = lo[q] | (static_cast<uint32_t>(hi[q]) << 16);
+    }
+#pragma unroll
+    for (int q = 0; q < 3; ++q) {
+      *reinterpret_cast<uint4*>(dst + q * plane) = make_uint4(w[q][0], w[q][1], w[q][2], w[q][3]);
+    }
+  }
+}
+
+constexpr int kPackThreads = 256;
+
+// One thread packs eight columns: bound by the bytes (FP32: 4 read, 6 written
+// per element). Runs only for FP32 operands and for row strides that are no
+// multiple of 16 bytes, which TMA cannot read.
+template <typename T, int kTerms, bool kVec>
+__global__ void __launch_bounds__(kPackThreads) pack_terms_kernel(
+    const T* __restrict__ src, __nv_bfloat16* __restrict__ dst, long long rows, int cols,
+    int ld) {
+  const int groups = ld >> 3;
+  const long long total = rows * groups;
+  const long long plane = rows * ld;
+  for (long long i = static_cast<long long>(blockIdx.x) * kPackThreads + threadIdx.x; i < total;
+       i += static_cast<long long>(gridDim.x) * kPackThreads) {
+    const long long r = i / groups;
+    const int c = static_cast<int>(i - r * groups) << 3;
+    const T* p = src + r * cols + c;
+    float v[8];
+    if (kVec && c + 8 <= cols) {
+      constexpr int kPer = 16 / sizeof(T);
+#pragma unroll
+      for (int j = 0; j < 8 / kPer; ++j) {
+        unpack16<T>(__ldg(reinterpret_cast<const uint4*>(p) + j), v + j * kPer);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = c + j < cols ? to_f32(__ldg(p + j)) : 0.0f;
+    }
+    store_parts<kTerms>(dst + r * ld + c, plane, v);
+  }
+}
+
+// ---- pointwise gradient --------------------------------------------------------------
+//
+// From the saved FP32 products g, u and the incoming dh:
+//   dg = dh * u * act'(g), du = dh * act(g).
+// Rounded once to the engine's operand parts (bfloat16: the rounding every
+// tensor-core operand takes; FP32: three exact parts). Bound by its bytes.
+template <typename T, int kTerms, bool kVec>
+__global__ void __launch_bounds__(kPackThreads) gated_pointwise_backward_kernel(
+    const float* __restrict__ gate_up, const T* __restrict__ dh, __nv_bfloat16* __restrict__ dg,
+    __nv_bfloat16* __restrict__ du, int rows, int output, int ld, int activation) {
+  const int groups = ld >> 3;
+  const long long total = static_cast<long long>(rows) * groups;
+  const long long plane = static_cast<long long>(rows) * ld;
+  for (long long i = static_cast<long long>(blockIdx.x) * kPackThreads + threadIdx.x; i < total;
+       i += static_cast<long long>(gridDim.x) * kPackThreads) {
+    const long long r = i / groups;
+    const int c = static_cast<int>(i - r * groups) << 3;
+    const float* pg = gate_up + 2 * r * output + c;
+    const float* pu = pg + output;
+    const T* pd = dh + r * output + c;
+    float g[8], u[8], d[8];
+    if (kVec && c + 8 <= output) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        unpack16<float>(__ldg(reinterpret_cast<const uint4*>(pg) + j), g + 4 * j);
+        unpack16<float>(__ldg(reinterpret_cast<const uint4*>(pu) + j), u + 4 * j);
+      }
+      constexpr int kPer = 16 / sizeof(T);
+#pragma unroll
+      for (int j = 0; j < 8 / kPer; ++j) {
+        unpack16<T>(__ldg(reinterpret_cast<const uint4*>(pd) + j), d + j * kPer);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const bool in = c + j < output;
+        g[j] = in ? __ldg(pg + j) : 0.0f;
+        u[j] = in ? __ldg(pu + j) : 0.0f;
+        d[j] = in ? to_f32(__ldg(pd + j)) : 0.0f;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      float slope;
+      const float a = activate(activation, g[j], &slope);
+      g[j] = d[j] * u[j] * slope;
+      u[j] = d[j] * a;
+    }
+    store_parts<kTerms>(dg + r * ld + c, plane, g);
+    store_parts<kTerms>(du + r * ld + c, plane, u);
+  }
+}
+
+int pack_blocks(long long total) {
+  const long long want = (total + kPackThreads - 1) / kPackThreads;
+  const long long cap = 16LL * sm_count();
+  return static_cast<int>(want < cap ? want : cap);
+}
+
+}  // namespace
+
+cudaError_t launch_gated_few(const void* x, const void* wg, const void* wu,
+                             const int32_t* offsets, void* h, float* gate_up, int rows,
+                             int experts, int hidden, int output, Activation activation,
+                             Dtype dtype, cudaStream_t stream) {
+  const int act = static_cast<int>(activation);
+  return dtype == Dtype::kBf16 ? few<__nv_bfloat16>(x, wg, wu, offsets, h, gate_up, rows, experts,
+                                                    hidden, output, act, stream)
+                               : few<float>(x, wg, wu, offsets, h, gate_up, rows, experts, hidden,
+                                            output, act, stream);
+}
+
+cudaError_t launch_pack_terms(const void* src, __nv_bfloat16* dst, long long rows, int cols,
+                              int ld, Dtype dtype, cudaStream_t stream) {
+  const int blocks = pack_blocks(rows * (ld >> 3));
+  if (blocks == 0) return cudaSuccess;
+  const bool vec = aligned_to(src, 16) && (cols * dtype_bytes(dtype)) % 16 == 0;
+  if (dtype == Dtype::kBf16) {
+    auto* kernel = vec ? pack_terms_kernel<__nv_bfloat16, 1, true>
+                       : pack_terms_kernel<__nv_bfloat16, 1, false>;
+    kernel<<<blocks, kPackThreads, 0, stream>>>(static_cast<const __nv_bfloat16*>(src), dst, rows,
+                                                cols, ld);
+  } else {
+    auto* kernel = vec ? pack_terms_kernel<float, 3, true> : pack_terms_kernel<float, 3, false>;
+    kernel<<<blocks, kPackThreads, 0, stream>>>(static_cast<const float*>(src), dst, rows, cols,
+                                                ld);
+  }
+  note_launch();
+  return cudaGetLastError();
+}
+
+cudaError_t launch_gated_pointwise_backward(const float* gate_up, const void* dh,
+                                            __nv_bfloat16* dg, __nv_bfloat16* du, int rows,
+                                            int output, int ld, Activation activation,
+                                            Dtype dtype, cudaStream_t stream) {
+  const int blocks = pack_blocks(static_cast<long long>(rows) * (ld >> 3));
+  if (blocks == 0) return cudaSuccess;
+  const int act = static_cast<int>(activation);
+  const bool vec = output % 8 == 0 && aligned_to(gate_up, 16) && aligned_to(dh, 16);
+  if (dtype == Dtype::kBf16) {
+    auto* kernel = vec ? gated_pointwise_backward_kernel<__nv_bfloat16, 1, true>
+                       : gated_pointwise_backward_kernel<__nv_bfloat16, 1, false>;
+    kernel<<<blocks, kPackThreads, 0, stream>>>(gate_up, static_cast<const __nv_bfloat16*>(dh), dg,
+                                                du, rows, output, ld, act);
+  } else {
+    auto* kernel = vec ? gated_pointwise_backward_kernel<float, 3, true>
+                       : gated_pointwise_backward_kernel<float, 3, false>;
+    kernel<<<blocks, kPackThreads, 0, stream>>>(gate_up, static_cast<const float*>(dh), dg, du,
+                                                rows, output, ld, act);
+  }
+  note_launch();
+  return cudaGetLastError();
+}
+
+}  // namespace rrb

@@ -1,0 +1,142 @@
+"""The expert-block operators together, as a mixture-of-experts block uses them
+beside the routing stages: router, gate, permute, gated projection, grouped
+GEMM, combine with norms; in FP32 forward and backward, and in 8-bit integers.
+"""
+from __future__ import annotations
+
+import math
+
+import torch
+import pytest
+
+import raggedroute_b200 as rr
+from expert_block_reference import normwise, random, unpermute_norm
+
+pytestmark = pytest.mark.gpu
+
+T, K, E, N = 700, 192, 12, 160
+EPS = 1e-6
+
+
+def route(x, router):
+    """Expert-grouped rows of x: (buffers, offsets, positions, weights)."""
+    dev = x.device
+    logits = torch.empty(T, E, device=dev)
+    ids = torch.empty(T, 2, dtype=torch.int32, device=dev)
+    w = torch.empty(T, 2, device=dev)
+    counts = torch.empty(E, dtype=torch.int32, device=dev)
+    off = torch.empty(E + 1, dtype=torch.int32, device=dev)
+    xp = torch.empty(2 * T, K, device=dev)
+    pos = torch.empty(2 * T, dtype=torch.int32, device=dev)
+    ws = torch.empty(rr.token_permute_workspace_size(T, E, 2, K), dtype=torch.uint8, device=dev)
+    rr.dense_gemm(x, router, logits, T, E, K)
+    rr.topk_gate(logits, ids, w, T, E)
+    rr.histogram_exclusive_scan(ids, counts, off, 2 * T, E)
+    rr.token_permute(x, ids, off, xp, pos, None, T, E, 2, K, ws)
+    return ids, w, off, xp, pos.view(T, 2)
+
+
+def make(device):
+    return dict(x=random((T, K), 1, device), router=random((K, E), 2, device, std=K ** -0.5),
+                wg=random((E, K, N), 3, device, std=K ** -0.5),
+                wu=random((E, K, N), 4, device, std=K ** -0.5),
+                wd=random((E, N, K), 5, device, std=N ** -0.5),
+                post=random((K,), 6, device, std=0.1) + 1, gate=random((K,), 7, device, std=0.5),
+                pre=random((K,), 8, device, std=0.1) + 1)
+
+
+def test_fp32_block_forward_and_backward(cuda):
+    m = make(cuda)
+    ids, w, off, xp, pos = route(m["x"], m["router"])
+    ws = torch.empty(rr.grouped_gated_gemm_workspace_size(2 * T, E, K, N, torch.float32, True),
+                     dtype=torch.uint8, device=cuda)
+    h, gu = torch.empty(2 * T, N, device=cuda), torch.empty(2 * T, 2 * N, device=cuda)
+    yp = torch.empty(2 * T, K, device=cuda)
+    out, normed = torch.empty(T, K, device=cuda), torch.empty(T, K, device=cuda)
+    inv = torch.empty(T, 2, device=cuda)
+    rr.grouped_gated_gemm(xp, m["wg"], m["wu"], off, h, gate_up=gu, workspace=ws)
+    rr.grouped_gemm(h, m["wd"], off, yp, E, N, K, 2 * T)
+    rr.unpermute_norm(yp, pos, w, m["x"], out, normed, post_gamma=m["post"], gate=m["gate"],
+                      pre_gamma=m["pre"], inv_rms=inv, eps=EPS)
+
+    # The same block token by token in float64, with the routing as decided.
+    d = {k: v.double().requires_grad_() for k, v in m.items()}
+    w64 = w.double().requires_grad_()
+    rows = d["x"][torch.arange(T, device=cuda).repeat_interleave(2)]
+    e = ids.view(-1).long()
+    y = torch.zeros(2 * T, K, dtype=torch.float64, device=cuda)
+    for i in range(E):
+        at = (e == i).nonzero()[:, 0]
+        g = rows[at] @ d["wg"][i]
+        y = y.index_put((at,), (g * torch.sigmoid(g) * (rows[at] @ d["wu"][i])) @ d["wd"][i])
+    order = torch.arange(2 * T, device=cuda).view(T, 2)
+    want, want_n = unpermute_norm(y, order, w64, d["x"], d["post"], d["gate"], d["pre"], EPS, 1.0)
+    # Three FP32 products in a row, each within 2^-19 normwise (grouped_gemm
+    # within 1e-5), and a norm of bounded condition.
+    assert normwise(out, want) < 3e-5 and normwise(normed, want_n) < 3e-5
+
+    dro, dn = random((T, K), 9, cuda), random((T, K), 10, cuda)
+    wsn = torch.empty(rr.unpermute_norm_backward_workspace_size(T, K), dtype=torch.uint8,
+                      device=cuda)
+    dres, dyp = torch.empty(T, K, device=cuda), torch.empty(2 * T, K, device=cuda)
+    dw, dgate = torch.empty(T, 2, device=cuda), torch.empty(K, device=cuda)
+    dpost, dpre = torch.empty(K, device=cuda), torch.empty(K, device=cuda)
+    rr.unpermute_norm_backward(yp, pos, w, m["x"], inv, dro, dn, dres, dyp, dw,
+                               post_gamma=m["post"], gate=m["gate"], pre_gamma=m["pre"],
+                               d_post_gamma=dpost, d_gate=dgate, d_pre_gamma=dpre, workspace=wsn)
+    # Through the down projection with the transposed weights, then the gated
+    # projection; a token's rows of dx add up with weights of one.
+    dh = torch.empty(2 * T, N, device=cuda)
+    rr.grouped_gemm(dyp, m["wd"].transpose(1, 2).contiguous(), off, dh, E, K, N, 2 * T)
+    dxp = torch.empty(2 * T, K, device=cuda)
+    dwg, dwu = torch.empty_like(m["wg"]), torch.empty_like(m["wu"])
+    rr.grouped_gated_gemm_backward(xp, m["wg"], m["wu"], off, gu, dh, dxp, dwg, dwu, workspace=ws)
+    dx = torch.empty(T, K, device=cuda)
+    rr.unpermute(dxp, pos.reshape(-1), torch.ones(2 * T, device=cuda), dx, T, 2, K)
+    grads = torch.autograd.grad((want, want_n),
+                                (d["x"], d["wg"], d["wu"], w64, d["post"], d["gate"], d["pre"]),
+                                (dro.double(), dn.double()))
+    got = (dx + dres, dwg, dwu, dw, dpost, dgate, dpre)
+    for a, b in zip(got, grads):
+        assert normwise(a, b) < 1e-4
+
+
+def test_bf16_and_int8_block(cuda):
+    """Rows grouped by the FP32 permute; the same block in bfloat16 with the
+    permute on bfloat16 rows (viewed as half as many floats) and in integers."""
+    m = make(cuda)
+    ids, w, off, xp, pos = route(m["x"], m["router"])
+    bf = torch.bfloat16
+    xb = m["x"].to(bf)
+    xpb = torch.empty(2 * T, K, dtype=bf, device=cuda)
+    ws = torch.empty(rr.token_permute_workspace_size(T, E, 2, K // 2), dtype=torch.uint8,
+                     device=cuda)
+    flat = torch.empty(2 * T, dtype=torch.int32, device=cuda)
+    rr.token_permute(xb.view(torch.float32), ids, off, xpb.view(torch.float32), flat, None, T, E,
+                     2, K // 2, ws)
+    assert torch.equal(xpb, xp.to(bf)) and torch.equal(flat.view(T, 2), pos)
+    wg, wu = m["wg"].to(bf), m["wu"].to(bf)
+    h = torch.empty(2 * T, N, dtype=bf, device=cuda)
+    rr.grouped_gated_gemm(xpb, wg, wu, off, h)
+    wq = torch.empty(E, K, rr.int8_row_stride(N), dtype=torch.int8, device=cuda)
+    wsc = torch.empty(E, K, device=cuda)
+    hq = torch.empty(2 * T, rr.int8_row_stride(N), dtype=torch.int8, device=cuda)
+    hs = torch.empty(2 * T, device=cuda)
+    yp = torch.empty(2 * T, K, dtype=bf, device=cuda)
+    rr.quantize_expert_weights_int8(m["wd"], wq, wsc)
+    rr.quantize_rows_int8(h, hq, hs)
+    rr.grouped_gemm_int8(hq, hs, wq, wsc, off, yp)
+    out, normed = torch.empty_like(xb), torch.empty_like(xb)
+    rr.unpermute_norm(yp, pos, w, xb, out, normed, post_gamma=m["post"], gate=m["gate"],
+                      pre_gamma=m["pre"], eps=EPS)
+    o = off.tolist()
+    y = torch.zeros(2 * T, K, dtype=torch.float64, device=cuda)
+    for i, (a, b) in enumerate(zip(o, o[1:])):
+        g = xpb[a:b].double() @ wg[i].double()
+        y[a:b] = (g * torch.sigmoid(g) * (xpb[a:b].double() @ wu[i].double())) @ m["wd"][i].double()
+    want, want_n = unpermute_norm(y, pos, w.double(), xb.double(), m["post"].double(),
+                                  m["gate"].double(), m["pre"].double(), EPS, 1.0)
+    # An 8-bit step is top / 127 with top below 6 deviations here: at most
+    # 0.5 * 6 / 127 / sqrt(3) of a deviation per operand, two operands.
+    assert normwise(out, want) < math.sqrt(2) * 3 / 127 / math.sqrt(3) + 2.0 ** -7
+    assert normwise(normed, want_n) < math.sqrt(2) * 3 / 127 / math.sqrt(3) + 2.0 ** -7
