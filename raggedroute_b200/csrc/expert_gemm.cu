@@ -32,10 +32,10 @@
 // epilogue warps add the blocks in FP32 registers while the next block runs
 // in the other half of TMEM.
 //
-// Roles (384 threads per CTA): warp 0 TMA producer; warp 1 MMA issuer (even
-// CTA); warp 2 relay: passes each landed stage on to the even CTA, and in kDw
-// clears the rows of a segment's last block that belong to other segments;
-// warps 4-11 epilogue. TMEM holds two 256-column accumulators, so a tile's
+// Roles (384 threads per CTA): warp 0 TMA producer (both CTAs' loads complete
+// on the even CTA's barriers); warp 1 MMA issuer (even CTA); warp 2, in kDw,
+// clears the rows of a segment's last block that belong to other segments and
+// hands that block over; warps 4-11 epilogue. TMEM holds two 256-column accumulators, so a tile's
 // epilogue runs beside the next tile's products. Waits are bounded as in the
 // other pair engine (gemm_pair.cu), with the same exit protocol.
 #include <cuda.h>
@@ -61,6 +61,9 @@ constexpr int kTmemCols = 512;
 constexpr int kEpiWarp0 = 4;
 constexpr int kEpiWarps = 8;
 constexpr int kThreads = (kEpiWarp0 + kEpiWarps) * 32;
+constexpr uint64_t kDrainNs = 2000000;
+constexpr int kPolls = 256;
+constexpr int kStagingBytes = 32 * 64;  // 64 bytes of 32 rows, per epilogue warp
 
 template <int kTerms>
 struct Config {
@@ -87,15 +90,15 @@ struct EngineArgs {
 template <int kTerms>
 struct alignas(1024) EngineSmem {
   uint8_t stage[Config<kTerms>::kStages][Config<kTerms>::kStageBytes];
-  uint64_t full[Config<kTerms>::kStages];   // this CTA's TMA bytes landed
+  uint8_t staging[kEpiWarps][kStagingBytes];  // output rows on their way out
   uint64_t empty[Config<kTerms>::kStages];  // the pair's MMAs have read the stage
   uint64_t ready[Config<kTerms>::kStages];  // even CTA: both CTAs' halves are in place
+  uint64_t tail[Config<kTerms>::kStages];   // kDw: this CTA's half of a short block landed
   uint64_t tmem_full[2];                    // accumulator finished (both CTAs)
   uint64_t tmem_empty[2];                   // even CTA: both CTAs have read it
   uint64_t mma_done;
   uint32_t tmem_base;
   int failed;
-  int issued[Config<kTerms>::kStages];
   int prefix[kMaxExperts + 1];
   int scratch[33];
 };
@@ -206,18 +209,57 @@ __device__ __forceinline__ Tile tile_at(const EngineArgs& p, int t, const int* p
   return g;
 }
 
+// Writes 64 bytes of each of a warp's 32 output rows; lane r holds row r in v.
+// An accumulator row belongs to one thread, so storing from registers would
+// touch 32 lines with 16 bytes each; through shared memory a warp writes whole
+// 64-byte pieces of eight rows at a time (or, where rows are not 16-byte
+// aligned or the piece is cut, consecutive elements). Chunk c of row r sits at
+// c ^ (r / 2 mod 4): no bank conflicts in either direction.
 template <typename T>
-__device__ __forceinline__ void store16(T* dst, const float* v, int valid, bool vec) {
-  if (vec && valid >= 16) {
-    constexpr int kPer = 16 / sizeof(T);
+__device__ __forceinline__ void store_rows(uint8_t* staging, const float* v, T* base, long long ld,
+                                           int rows, int cols, bool vec) {
+  constexpr int kPer = 16 / sizeof(T);
+  constexpr int kCols = 4 * kPer;
+  const int lane = threadIdx.x & 31;
+  __syncwarp();  // the previous piece has been read
 #pragma unroll
-    for (int i = 0; i < 16 / kPer; ++i) {
-      reinterpret_cast<uint4*>(dst)[i] = pack16<T>(v + kPer * i);
+  for (int c = 0; c < 4; ++c) {
+    *reinterpret_cast<uint4*>(staging + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)) =
+        pack16<T>(v + kPer * c);
+  }
+  __syncwarp();
+  if (vec && cols >= kCols) {
+    const int c = lane & 3;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = 8 * i + (lane >> 2);
+      if (r < rows) {
+        *reinterpret_cast<uint4*>(base + r * ld + kPer * c) = *reinterpret_cast<const uint4*>(
+            staging + r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
+      }
     }
   } else {
+    const int col = lane % kCols;
+    const int c = col / kPer;
+    if (col < cols) {
+#pragma unroll 4
+      for (int r = lane / kCols; r < rows; r += 32 / kCols) {
+        base[r * ld + col] = *reinterpret_cast<const T*>(
+            staging + r * 64 + ((c ^ ((r >> 1) & 3)) << 4) + (col % kPer) * sizeof(T));
+      }
+    }
+  }
+}
+
+// 32 columns of a warp's rows: one piece of bfloat16 or two of float.
+template <typename T>
+__device__ __forceinline__ void store_rows32(uint8_t* staging, const float* v, T* base,
+                                             long long ld, int rows, int cols, bool vec) {
+  constexpr int kCols = 64 / sizeof(T);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      if (i < valid) dst[i] = from_f32<T>(v[i]);
+  for (int i = 0; i < 32 / kCols; ++i) {
+    if (cols > i * kCols) {
+      store_rows<T>(staging, v + i * kCols, base + i * kCols, ld, rows, cols - i * kCols, vec);
     }
   }
 }
@@ -253,10 +295,9 @@ __global__ void __launch_bounds__(kThreads, 1) expert_gemm_kernel(
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
-      mbar_init(&s.full[i], 1);
       mbar_init(&s.empty[i], 1);
-      mbar_init(&s.ready[i], 2);
-      s.issued[i] = 0;
+      mbar_init(&s.ready[i], kMode == kDw ? 2 : 1);
+      mbar_init(&s.tail[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s.tmem_full[i], 1);
@@ -284,12 +325,17 @@ __global__ void __launch_bounds__(kThreads, 1) expert_gemm_kernel(
   volatile int* failed = &s.failed;
   const uint32_t peer_failed = mapa_shared(smem_u32(&s.failed), rank ^ 1u);
   auto wait = [&](uint64_t* bar, uint32_t parity) {
+    // Most waits end within microseconds: poll before reading any clock.
+#pragma unroll 1
+    for (int i = 0; i < kPolls; ++i) {
+      if (mbar_try_wait(bar, parity)) return true;
+    }
     return mbar_wait_pair(bar, parity, p.err, failed, peer_failed);
   };
 
   if (warp == 0) {
     // ---------------- TMA producer ----------------
-    if (lane == 0) {
+    {
       int stage = 0;
       uint32_t phase = 0;
       for (int t = unit; t < total && !*failed; t += units) {
@@ -298,38 +344,52 @@ __global__ void __launch_bounds__(kThreads, 1) expert_gemm_kernel(
         const int half = g.n_mma >> 1;
         for (int kb = 0; kb < g.blocks; ++kb) {
           if (!wait(&s.empty[stage], phase ^ 1u)) break;
+          if (elect_one()) {
           uint8_t* a = s.stage[stage];
           uint8_t* b = a + kOffB;
-          uint64_t* bar = &s.full[stage];
-          mbar_arrive_expect_tx(bar, kStageTx);
+          // Both CTAs' bytes complete on the even CTA's barrier. A short last
+          // block of kDw completes on each CTA's own: its relay warp hands it
+          // over once it has cleared the lines past the segment.
+          const bool cut = kMode == kDw && g.row_end - g.row0 - kb * 64 < 64;
+          uint32_t bar;
+          if (cut) {
+            bar = smem_u32(&s.tail[stage]);
+            mbar_arrive_expect_tx(&s.tail[stage], kStageTx);
+          } else {
+            bar = mapa_shared(smem_u32(&s.ready[stage]), 0u);
+            if (leader) mbar_arrive_expect_tx(&s.ready[stage], 2 * kStageTx);
+            else if (kMode == kDw) mbar_arrive_remote(bar);
+          }
 #pragma unroll
           for (int q = 0; q < kTerms; ++q, a += kOperandBytes, b += kOperandBytes) {
             if constexpr (kMode == kGated) {
               const CUtensorMap* mb = leader ? &map_b0 : &map_b1;
-              tma_load_3d(a, &map_a0, bar, kb * 64, m, q);
-              tma_load_3d(b, mb, bar, g.c0, kb * 64, q * p.experts + g.expert);
-              tma_load_3d(b + kBoxBytes, mb, bar, g.c0 + 64, kb * 64, q * p.experts + g.expert);
+              const int z = q * p.experts + g.expert;
+              tma_load_3d_pair(a, &map_a0, bar, kb * 64, m, q);
+              tma_load_3d_pair(b, mb, bar, g.c0, kb * 64, z);
+              tma_load_3d_pair(b + kBoxBytes, mb, bar, g.c0 + 64, kb * 64, z);
             } else if constexpr (kMode == kDx) {
               const int per = g.blocks >> 1;
               const bool first = kb < per;
               const int k = (first ? kb : kb - per) * 64;
-              tma_load_3d(a, first ? &map_a0 : &map_a1, bar, k, m, q);
-              tma_load_3d(b, first ? &map_b0 : &map_b1, bar, k,
-                          g.c0 + static_cast<int>(rank) * half, q * p.experts + g.expert);
+              tma_load_3d_pair(a, first ? &map_a0 : &map_a1, bar, k, m, q);
+              tma_load_3d_pair(b, first ? &map_b0 : &map_b1, bar, k,
+                               g.c0 + static_cast<int>(rank) * half, q * p.experts + g.expert);
             } else if constexpr (kMode == kDw) {
               const CUtensorMap* mb = leader ? &map_b0 : &map_b1;
               const int r = g.row0 + kb * 64;
-              tma_load_3d(a, &map_a0, bar, m, r, q);
-              tma_load_3d(a + kBoxBytes, &map_a0, bar, m + 64, r, q);
-              tma_load_3d(b, mb, bar, g.c0, r, q);
-              tma_load_3d(b + kBoxBytes, mb, bar, g.c0 + 64, r, q);
+              tma_load_3d_pair(a, &map_a0, bar, m, r, q);
+              tma_load_3d_pair(a + kBoxBytes, &map_a0, bar, m + 64, r, q);
+              tma_load_3d_pair(b, mb, bar, g.c0, r, q);
+              tma_load_3d_pair(b + kBoxBytes, mb, bar, g.c0 + 64, r, q);
             } else {
-              tma_load_3d(a, &map_a0, bar, kb * 128, m, 0);
-              tma_load_3d(b, &map_b0, bar, kb * 128, g.c0 + static_cast<int>(rank) * half,
-                          g.expert);
+              tma_load_3d_pair(a, &map_a0, bar, kb * 128, m, 0);
+              tma_load_3d_pair(b, &map_b0, bar, kb * 128, g.c0 + static_cast<int>(rank) * half,
+                               g.expert);
             }
           }
-          s.issued[stage] += 1;
+          }
+          __syncwarp();
           if (++stage == kStages) {
             stage = 0;
             phase ^= 1u;
@@ -348,7 +408,7 @@ __global__ void __launch_bounds__(kThreads, 1) expert_gemm_kernel(
     }
   } else if (warp == 1) {
     // ---------------- MMA issuer (even CTA) ----------------
-    if (leader && lane == 0) {
+    if (leader) {
       int stage = 0, buf = 0;
       uint32_t phase = 0, acc_phase = 0;
       bool ok = true;
@@ -371,6 +431,7 @@ __global__ void __launch_bounds__(kThreads, 1) expert_gemm_kernel(
           const uint32_t base = smem_u32(s.stage[stage]);
           const uint64_t a0 = smem_desc(base, kLboA, 1024, Swizzle::k128B);
           const uint64_t b0 = smem_desc(base + kOffB, kLboB, 1024, Swizzle::k128B);
+          if (elect_one()) {
           if constexpr (kTerms == 1) {
 #pragma unroll
             for (uint32_t ks = 0; ks < 4; ++ks) {
@@ -393,140 +454,128 @@ __global__ void __launch_bounds__(kThreads, 1) expert_gemm_kernel(
               }
             }
           }
-          const uint32_t e = smem_u32(&s.empty[stage]);
-          mma_commit_pair_to(e);
-          mma_commit_pair_to(mapa_shared(e, 1u));
+          mma_commit_pair_both(smem_u32(&s.empty[stage]));
+          if (kTerms == 3 || kb + 1 == g.blocks) {
+            mma_commit_pair_both(smem_u32(&s.tmem_full[buf]));
+          }
+          }
+          __syncwarp();
           if (++stage == kStages) {
             stage = 0;
             phase ^= 1u;
           }
           if (kTerms == 3 || kb + 1 == g.blocks) {
-            const uint32_t f = smem_u32(&s.tmem_full[buf]);
-            mma_commit_pair_to(f);
-            mma_commit_pair_to(mapa_shared(f, 1u));
             buf ^= 1;
             if (buf == 0) acc_phase ^= 1u;
           }
         }
       }
-      mma_commit_pair_to(smem_u32(&s.mma_done));
+      if (elect_one()) mma_commit_pair_to(smem_u32(&s.mma_done));
+      __syncwarp();
       int dummy = 0;
       mbar_wait(&s.mma_done, 0, p.err, &dummy);
     }
   } else if (warp == 2) {
-    // ---------------- relay ----------------
-    int stage = 0;
-    uint32_t phase = 0;
-    bool ok = true;
-    for (int t = unit; t < total && ok && !*failed; t += units) {
-      const Tile g = tile_at<kMode>(p, t, s.prefix, n_tiles);
-      for (int kb = 0; kb < g.blocks; ++kb) {
-        if (!wait(&s.full[stage], phase)) {
-          ok = false;
-          break;
-        }
-        if constexpr (kMode == kDw) {
-          // Lines past the segment's end hold other segments' rows (or
-          // anything): both operands become zero there. A line is one row of
-          // a box, so the swizzle inside it does not matter.
-          const int valid = g.row_end - g.row0 - kb * 64;
-          if (valid < 64) {
-            for (int bx = 0; bx < 4 * kTerms; ++bx) {
-              uint8_t* box = s.stage[stage] + bx * kBoxBytes;
-              for (int i = valid * 8 + lane; i < 512; i += 32) {
-                reinterpret_cast<uint4*>(box)[i] = make_uint4(0u, 0u, 0u, 0u);
-              }
-            }
-            fence_proxy_async_smem();
+    // ---------------- relay (kDw): short last blocks ----------------
+    if constexpr (kMode == kDw) {
+      int at = 0;           // k-blocks so far: stage at % kStages
+      uint32_t phases = 0;  // per stage, of its tail barrier
+      for (int t = unit; t < total && !*failed; t += units) {
+        const Tile g = tile_at<kMode>(p, t, s.prefix, n_tiles);
+        at = (at + g.blocks) % kStages;
+        const int valid = (g.row_end - g.row0) & 63;
+        if (valid == 0) continue;
+        const int stage = (at + kStages - 1) % kStages;  // of the last block
+        if (!wait(&s.tail[stage], (phases >> stage) & 1u)) break;
+        phases ^= 1u << stage;
+        // Lines past the segment's end hold other segments' rows (or
+        // anything): both operands become zero there. A line is one row of a
+        // box, so the swizzle inside it does not matter.
+        for (int bx = 0; bx < 4 * kTerms; ++bx) {
+          uint8_t* box = s.stage[stage] + bx * kBoxBytes;
+          for (int i = valid * 8 + lane; i < 512; i += 32) {
+            reinterpret_cast<uint4*>(box)[i] = make_uint4(0u, 0u, 0u, 0u);
           }
         }
+        fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive_remote(mapa_shared(smem_u32(&s.ready[stage]), 0u));
-        if (++stage == kStages) {
-          stage = 0;
-          phase ^= 1u;
-        }
       }
     }
   } else if (warp >= kEpiWarp0) {
     // ---------------- epilogue ----------------
-    const int quarter = warp & 3;
+    const int quarter = warp & 3;  // the TMEM lanes this warp may read
     const int hw = (warp - kEpiWarp0) >> 2;
     const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
+    uint8_t* staging = s.staging[warp - kEpiWarp0];
     int buf = 0;
     uint32_t acc_phase = 0;
     bool ok = true;
     for (int t = unit; t < total && ok && !*failed; t += units) {
       const Tile g = tile_at<kMode>(p, t, s.prefix, n_tiles);
       const int half = g.n_mma >> 1;
-      const int row = g.m0 + static_cast<int>(rank) * kRowsCta + quarter * 32 + lane;
-      const bool live = row < g.m_end;
-      // Piece q of 16 accumulator columns of this warp: kGated has gate
-      // columns in pieces 0-3 and the up columns they meet in 4-7.
-      auto piece_col = [&](int q) {
-        if constexpr (kMode == kGated) {
-          return (q < 4 ? 0 : half) + hw * 64 + 16 * (q & 3);
-        } else if constexpr (kMode == kDw) {
-          return hw * half + 16 * q;
-        } else {
-          return hw * 128 + 16 * q;
-        }
+      const int row0 = g.m0 + static_cast<int>(rank) * kRowsCta + quarter * 32;  // of the warp
+      const int rows = max(0, min(32, g.m_end - row0));
+      // Group q of 32 accumulator columns of this warp: kGated has gate
+      // columns in groups 0-1 and the up columns they meet in 2-3.
+      auto group_col = [&](int q) {
+        if constexpr (kMode == kGated) return (q < 2 ? 0 : half) + hw * 64 + 32 * (q & 1);
+        else if constexpr (kMode == kDw) return hw * half + 32 * q;
+        else return hw * 128 + 32 * q;
       };
-      auto piece_live = [&](int q) {  // warp-uniform
-        if constexpr (kMode == kGated) return hw * 64 + 16 * (q & 3) < half;
-        else if constexpr (kMode == kDw) return 16 * q < half;
-        else return hw * 128 + 16 * q < g.n_mma;
+      auto group_live = [&](int q) {  // warp-uniform
+        if constexpr (kMode == kGated) return hw * 64 + 32 * (q & 1) < half;
+        else if constexpr (kMode == kDw) return 32 * q < half;
+        else return hw * 128 + 32 * q < g.n_mma;
       };
+      // Stores group q: v, in kGated with its up columns v2.
       auto put = [&](int q, const float* v, const float* v2) {
+        const int c = (kMode == kGated ? hw * 64 : (kMode == kDw ? 0 : hw * 128)) + 32 * q;
+        const int cols = g.ncols - c;
+        if (rows == 0 || cols <= 0) return;  // warp-uniform
         if constexpr (kMode == kGated) {
-          const int c = hw * 64 + 16 * q;
-          const int valid = min(16, g.ncols - c);
-          if (!live || valid <= 0) return;
-          float h[16];
+          float h[32];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) h[i] = activate(p.activation, v[i]) * v2[i];
-          const long long at = static_cast<long long>(row) * p.output + g.c0 + c;
-          store16(static_cast<T*>(p.out0) + at, h, valid, p.vec != 0);
+          for (int i = 0; i < 32; ++i) h[i] = activate(p.activation, v[i]) * v2[i];
+          const long long at = static_cast<long long>(row0) * p.output + g.c0 + c;
+          store_rows32<T>(staging, h, static_cast<T*>(p.out0) + at, p.output, rows, cols,
+                          p.vec != 0);
           if (p.gate_up != nullptr) {
-            float* gu = p.gate_up + 2LL * row * p.output + g.c0 + c;
-            store16(gu, v, valid, p.vec_gate_up != 0);
-            store16(gu + p.output, v2, valid, p.vec_gate_up != 0);
+            float* gu = p.gate_up + 2LL * row0 * p.output + g.c0 + c;
+            store_rows32<float>(staging, v, gu, 2LL * p.output, rows, cols, p.vec_gate_up != 0);
+            store_rows32<float>(staging, v2, gu + p.output, 2LL * p.output, rows, cols,
+                                p.vec_gate_up != 0);
           }
         } else if constexpr (kMode == kDw) {
-          const int valid = min(16, g.ncols - 16 * q);
-          if (!live || valid <= 0) return;
           T* out = static_cast<T*>(hw == 0 ? p.out0 : p.out1) +
-                   (static_cast<long long>(g.expert) * p.hidden + row) * p.output + g.c0 + 16 * q;
-          store16(out, v, valid, p.vec != 0);
+                   (static_cast<long long>(g.expert) * p.hidden + row0) * p.output + g.c0 + c;
+          store_rows32<T>(staging, v, out, p.output, rows, cols, p.vec != 0);
         } else {
-          const int c = hw * 128 + 16 * q;
-          const int valid = min(16, g.ncols - c);
-          if (!live || valid <= 0) return;
           const int ld = kMode == kDx ? p.hidden : p.output;
-          T* out = static_cast<T*>(p.out0) + static_cast<long long>(row) * ld + g.c0 + c;
+          T* out = static_cast<T*>(p.out0) + static_cast<long long>(row0) * ld + g.c0 + c;
           if constexpr (kMode == kInt8) {
-            const float xs = __ldg(p.row_scale + row);
+            const float xs = lane < rows ? __ldg(p.row_scale + row0 + lane) : 0.0f;
             const float* ws =
                 p.col_scale + static_cast<long long>(g.expert) * p.output + g.c0 + c;
-            float y[16];
+            float y[32];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
+            for (int i = 0; i < 32; ++i) {
               y[i] = static_cast<float>(__float_as_int(v[i])) * xs *
-                     (i < valid ? __ldg(ws + i) : 0.0f);
+                     (i < cols ? __ldg(ws + i) : 0.0f);
             }
-            store16(out, y, valid, p.vec != 0);
+            store_rows32<T>(staging, y, out, ld, rows, cols, p.vec != 0);
           } else {
-            store16(out, v, valid, p.vec != 0);
+            store_rows32<T>(staging, v, out, ld, rows, cols, p.vec != 0);
           }
         }
       };
       auto load = [&](int q, float* v) {
-        uint32_t r[16];
-        tmem_ld_32x32b_x16(
-            tmem + static_cast<uint32_t>(buf * kTileN + piece_col(q)) + lane_addr, r);
+        uint32_t r[32];
+        tmem_ld_32x32b_x32(
+            tmem + static_cast<uint32_t>(buf * kTileN + group_col(q)) + lane_addr, r);
         tmem_ld_wait();
 #pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+        for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
       };
       auto take = [&]() {  // the accumulator is finished
         if (!wait(&s.tmem_full[buf], acc_phase)) return false;
@@ -542,28 +591,24 @@ __global__ void __launch_bounds__(kThreads, 1) expert_gemm_kernel(
       };
       if constexpr (kMode == kDw) {
         if (g.blocks == 0) {  // no rows: a zero gradient
-          const float zero[16] = {};
-          for (int q = 0; q < 8; ++q) put(q, zero, zero);
+          const float zero[32] = {};
+#pragma unroll 1
+          for (int q = 0; q < 4; ++q) put(q, zero, zero);
           continue;
         }
       }
       if constexpr (kTerms == 1) {
         if (!take()) break;
-        if constexpr (kMode == kGated) {
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            if (!piece_live(q)) break;
-            float v[16], v2[16];
-            load(q, v);
-            load(q + 4, v2);
+#pragma unroll 1
+        for (int q = 0; q < (kMode == kGated ? 2 : 4); ++q) {
+          if (!group_live(q)) break;
+          float v[32];
+          load(q, v);
+          if constexpr (kMode == kGated) {
+            float v2[32];
+            load(q + 2, v2);
             put(q, v, v2);
-          }
-        } else {
-#pragma unroll
-          for (int q = 0; q < 8; ++q) {
-            if (!piece_live(q)) break;
-            float v[16];
-            load(q, v);
+          } else {
             put(q, v, v);
           }
         }
@@ -579,32 +624,35 @@ __global__ void __launch_bounds__(kThreads, 1) expert_gemm_kernel(
           }
 #pragma unroll
           for (int q = 0; q < 8; ++q) {
-            if (piece_live(q)) {
-              float v[16];
-              load(q, v);
+            if (group_live(q >> 1)) {
+              uint32_t r[16];
+              tmem_ld_32x32b_x16(tmem +
+                                     static_cast<uint32_t>(buf * kTileN + group_col(q >> 1) +
+                                                           16 * (q & 1)) +
+                                     lane_addr,
+                                 r);
+              tmem_ld_wait();
 #pragma unroll
-              for (int i = 0; i < 16; ++i) sum[16 * q + i] += v[i];
+              for (int i = 0; i < 16; ++i) sum[16 * q + i] += __uint_as_float(r[i]);
             }
           }
           release();
         }
         if (!ok) break;
 #pragma unroll
-        for (int q = 0; q < (kMode == kGated ? 4 : 8); ++q) {
-          put(q, sum + 16 * q, sum + (16 * q + (kMode == kGated ? 64 : 0)));
+        for (int q = 0; q < (kMode == kGated ? 2 : 4); ++q) {
+          put(q, sum + 32 * q, sum + (32 * q + (kMode == kGated ? 64 : 0)));
         }
       }
     }
   }
 
   __syncthreads();
-  if (warp == 0 && lane == 0 && *failed) {
-    // Drain TMA loads still in flight into this CTA's shared memory.
-    for (int i = 0; i < kStages; ++i) {
-      if (s.issued[i] > 0) {
-        int dummy = 0;
-        mbar_wait(&s.full[i], static_cast<uint32_t>((s.issued[i] - 1) & 1), p.err, &dummy);
-      }
+  if (threadIdx.x == 0 && *failed) {
+    // After a wait that ran out: give this CTA's loads in flight (microseconds
+    // each) time to land before its shared memory is given up.
+    const uint64_t start = global_timer_ns();
+    while (global_timer_ns() - start < kDrainNs) {
     }
   }
   tc_fence_before();

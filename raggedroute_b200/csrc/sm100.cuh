@@ -167,6 +167,18 @@ __device__ __forceinline__ void cluster_sync() {
                ::: "memory");
 }
 
+// True in one lane of a converged warp. Unlike a test of the lane index it
+// leaves the code around it warp-uniform.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(p));
+  return p != 0;
+}
+
 // ---- explicit shared-memory accesses (32-bit shared addresses) --------------
 
 __device__ __forceinline__ float lds_f32(uint32_t addr) {
@@ -232,6 +244,17 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, u
       "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
       " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+
+// A load of a CTA pair into this CTA's shared memory that completes on the
+// mbarrier at shared::cluster address `bar` (this CTA's or the peer's).
+__device__ __forceinline__ void tma_load_3d_pair(void* dst, const CUtensorMap* map, uint32_t bar,
+                                                 int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z)
       : "memory");
 }
 
@@ -379,6 +402,16 @@ __device__ __forceinline__ void mma_commit_pair_to(uint32_t cluster_addr) {
   asm volatile(
       "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
           cluster_addr)
+      : "memory");
+}
+
+// The same, arriving on the barrier at this shared-memory offset in both CTAs
+// of the pair with one commit.
+__device__ __forceinline__ void mma_commit_pair_both(uint32_t smem_addr) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64"
+      " [%0], %1;" ::"r"(smem_addr),
+      "h"(static_cast<uint16_t>(3))
       : "memory");
 }
 
