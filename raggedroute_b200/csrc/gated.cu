@@ -2,6 +2,7 @@
 // (expert_gemm.cu): the form for a few rows, the packing of operands the
 // engine cannot read as they are, and the pointwise half of the gradient.
 #include "expert_block.cuh"
+#include "sm100.cuh"
 
 namespace rrb {
 namespace {
@@ -10,16 +11,24 @@ namespace {
 //
 // h[r, c] = act(sum_k x[r, k] Wg[e][k, c]) * sum_k x[r, k] Wu[e][k, c] for a
 // handful of rows: bound by reading the weights of the experts that have
-// rows, 2 K N elements each, once. One block takes 32 columns of up to kRows
+// rows, 2 K N elements each, once. A cluster takes 32 columns of up to kFewRows
 // rows of one expert, 16 bytes of each matrix per thread and k-step, with the
-// contraction spread over the block's threads: the partial sums (FP32) meet
-// by shuffles and in shared memory, in a fixed order. No block waits on
-// another, and gate and up of a column meet in the block that owns it.
+// contraction spread over its blocks and their threads; the partial sums
+// (FP32) meet by shuffles, in shared memory and in the first block of the
+// cluster, in a fixed order. The cluster grows (to 8 blocks) until every SM has
+// work to keep its loads in flight: one row of a narrow layer is a few dozen
+// column groups.
 
 constexpr int kFewThreads = 256;
 constexpr int kFewWarps = kFewThreads / 32;
 constexpr int kFewCols = 32;
 constexpr int kFewRows = 4;
+constexpr int kMaxSplit = 8;
+
+struct FewSmem {
+  float warps[kFewWarps][kFewRows][2][kFewCols];      // gate and up sums of each warp
+  float parts[kMaxSplit - 1][kFewRows][2][kFewCols];  // and of the cluster's other blocks
+};
 
 __device__ __forceinline__ uint4 ld_stream16(const void* p) {
   uint4 v;
@@ -29,21 +38,31 @@ __device__ __forceinline__ uint4 ld_stream16(const void* p) {
   return v;
 }
 
+// kVec consecutive elements as loaded, and as floats.
 template <typename T, int kVec>
-__device__ __forceinline__ void load_vec(const T* p, float* f) {
-  if constexpr (kVec == 1) f[0] = to_f32(__ldg(p));
-  else unpack16<T>(ld_stream16(p), f);
-}
+struct Raw {
+  uint4 v;
+  __device__ __forceinline__ void load(const T* p) { v = ld_stream16(p); }
+  __device__ __forceinline__ void get(float* f) const { unpack16<T>(v, f); }
+};
+template <typename T>
+struct Raw<T, 1> {
+  T v;
+  __device__ __forceinline__ void load(const T* p) { v = __ldg(p); }
+  __device__ __forceinline__ void get(float* f) const { f[0] = to_f32(v); }
+};
 
 template <typename T, int kVec, int kR>
 __device__ __forceinline__ void few_rows(const T* __restrict__ x, const T* __restrict__ wg,
                                          const T* __restrict__ wu, T* __restrict__ h,
                                          float* __restrict__ gate_up, int row, int nrows,
                                          int hidden, int output, int c0, int activation,
-                                         float* red) {
+                                         int split, FewSmem& s) {
   constexpr int kLanes = kFewCols / kVec;       // lanes across the columns
-  constexpr int kGroups = kFewThreads / kLanes;  // contraction groups
+  constexpr int kGroups = kFewThreads / kLanes;  // contraction groups of a block
   constexpr int kUnroll = 4;
+  const int part = static_cast<int>(sm100::cluster_ctarank());
+  const int stride = split * kGroups;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int col = (threadIdx.x % kLanes) * kVec;
   const int kg = threadIdx.x / kLanes;
@@ -61,7 +80,10 @@ __device__ __forceinline__ void few_rows(const T* __restrict__ x, const T* __res
     for (int i = 0; i < kR; ++i) {
       px[i] = x + static_cast<long long>(row + min(i, nrows - 1)) * hidden;
     }
-    auto step = [&](int k, const float* a, const float* b) {
+    auto step = [&](int k, const Raw<T, kVec>& wa, const Raw<T, kVec>& wb) {
+      float a[kVec], b[kVec];
+      wa.get(a);
+      wb.get(b);
 #pragma unroll
       for (int i = 0; i < kR; ++i) {
         const float v = to_f32(__ldg(px[i] + k));
@@ -72,23 +94,23 @@ __device__ __forceinline__ void few_rows(const T* __restrict__ x, const T* __res
         }
       }
     };
-    int k = kg;
-    for (; k + (kUnroll - 1) * kGroups < hidden; k += kUnroll * kGroups) {
-      float a[kUnroll][kVec], b[kUnroll][kVec];
+    int k = part * kGroups + kg;
+    for (; k + (kUnroll - 1) * stride < hidden; k += kUnroll * stride) {
+      Raw<T, kVec> a[kUnroll], b[kUnroll];
 #pragma unroll
       for (int q = 0; q < kUnroll; ++q) {
-        const long long at = static_cast<long long>(k + q * kGroups) * output;
-        load_vec<T, kVec>(pg + at, a[q]);
-        load_vec<T, kVec>(pu + at, b[q]);
+        const long long at = static_cast<long long>(k + q * stride) * output;
+        a[q].load(pg + at);
+        b[q].load(pu + at);
       }
 #pragma unroll
-      for (int q = 0; q < kUnroll; ++q) step(k + q * kGroups, a[q], b[q]);
+      for (int q = 0; q < kUnroll; ++q) step(k + q * stride, a[q], b[q]);
     }
-    for (; k < hidden; k += kGroups) {
-      float a[kVec], b[kVec];
+    for (; k < hidden; k += stride) {
+      Raw<T, kVec> a, b;
       const long long at = static_cast<long long>(k) * output;
-      load_vec<T, kVec>(pg + at, a);
-      load_vec<T, kVec>(pu + at, b);
+      a.load(pg + at);
+      b.load(pu + at);
       step(k, a, b);
     }
   }
@@ -103,20 +125,37 @@ __device__ __forceinline__ void few_rows(const T* __restrict__ x, const T* __res
         u[i][j] += __shfl_xor_sync(0xffffffffu, u[i][j], d);
       }
       if (lane < kLanes) {
-        red[((warp * kR + i) * 2) * kFewCols + col + j] = g[i][j];
-        red[((warp * kR + i) * 2 + 1) * kFewCols + col + j] = u[i][j];
+        s.warps[warp][i][0][col + j] = g[i][j];
+        s.warps[warp][i][1][col + j] = u[i][j];
       }
     }
   }
   __syncthreads();
   const int i = threadIdx.x / kFewCols, c = threadIdx.x % kFewCols;
-  if (i < nrows && i < kR && c0 + c < output) {
-    float sg = 0.0f, su = 0.0f;
+  float sg = 0.0f, su = 0.0f;
+  if (i < kR) {
 #pragma unroll
     for (int w = 0; w < kFewWarps; ++w) {
-      sg += red[((w * kR + i) * 2) * kFewCols + c];
-      su += red[((w * kR + i) * 2 + 1) * kFewCols + c];
+      sg += s.warps[w][i][0][c];
+      su += s.warps[w][i][1][c];
     }
+  }
+  if (split > 1) {
+    if (part > 0 && i < kR) {
+      const uint32_t to = sm100::mapa_shared(sm100::smem_u32(&s.parts[part - 1][i][0][c]), 0u);
+      sm100::st_shared_cluster_u32(to, __float_as_uint(sg));
+      sm100::st_shared_cluster_u32(to + kFewCols * 4, __float_as_uint(su));
+    }
+    sm100::cluster_sync();
+    if (part > 0) return;
+    if (i < kR) {
+      for (int q = 0; q < split - 1; ++q) {
+        sg += s.parts[q][i][0][c];
+        su += s.parts[q][i][1][c];
+      }
+    }
+  }
+  if (i < nrows && i < kR && c0 + c < output) {
     const long long r = row + i;
     h[r * output + c0 + c] = from_f32<T>(activate(activation, sg) * su);
     if (gate_up != nullptr) {
@@ -126,13 +165,15 @@ __device__ __forceinline__ void few_rows(const T* __restrict__ x, const T* __res
   }
 }
 
-template <typename T, int kVec>
-__global__ void __launch_bounds__(kFewThreads) gated_few_kernel(
+// kR rows of an expert share a reading of its weights. One row at a time needs
+// half the registers, so twice the loads are in flight.
+template <typename T, int kVec, int kR>
+__global__ void __launch_bounds__(kFewThreads, kR == 1 ? 4 : 2) gated_few_kernel(
     const T* __restrict__ x, const T* __restrict__ wg, const T* __restrict__ wu,
     const int32_t* __restrict__ offsets, T* __restrict__ h, float* __restrict__ gate_up, int rows,
-    int experts, int hidden, int output, int activation) {
+    int experts, int hidden, int output, int activation, int split) {
   __shared__ int owner;
-  __shared__ float red[kFewWarps * kFewRows * 2 * kFewCols];
+  __shared__ FewSmem smem;
   if (threadIdx.x == 0) owner = experts;
   __syncthreads();
   const int row = blockIdx.y;
@@ -142,19 +183,13 @@ __global__ void __launch_bounds__(kFewThreads) gated_few_kernel(
   }
   __syncthreads();
   const int e = owner;
+  // Uniform over a cluster, whose blocks share the row.
   if (e == experts) return;  // a row outside every segment
   const int2 s = segment(offsets, e, rows);
-  if ((row - s.x) % kFewRows != 0) return;  // an earlier block's row
-  const int nrows = min(kFewRows, s.y - row);
-  const int c0 = blockIdx.x * kFewCols;
+  if ((row - s.x) % kR != 0) return;  // an earlier block's row
   const long long at = static_cast<long long>(e) * hidden * output;
-  if (nrows == 1) {
-    few_rows<T, kVec, 1>(x, wg + at, wu + at, h, gate_up, row, nrows, hidden, output, c0,
-                         activation, red);
-  } else {
-    few_rows<T, kVec, kFewRows>(x, wg + at, wu + at, h, gate_up, row, nrows, hidden, output, c0,
-                                activation, red);
-  }
+  few_rows<T, kVec, kR>(x, wg + at, wu + at, h, gate_up, row, min(kR, s.y - row), hidden, output,
+                        blockIdx.x / split * kFewCols, activation, split, smem);
 }
 
 template <typename T>
@@ -162,14 +197,43 @@ cudaError_t few(const void* x, const void* wg, const void* wu, const int32_t* of
                 float* gate_up, int rows, int experts, int hidden, int output, int activation,
                 cudaStream_t stream) {
   constexpr int kVec = 16 / sizeof(T);
-  const dim3 grid(ceil_div(output, kFewCols), rows);
   const bool vec = output % kVec == 0 && aligned_to(wg, 16) && aligned_to(wu, 16);
-  auto* kernel = vec ? gated_few_kernel<T, kVec> : gated_few_kernel<T, 1>;
-  kernel<<<grid, kFewThreads, 0, stream>>>(
-      static_cast<const T*>(x), static_cast<const T*>(wg), static_cast<const T*>(wu), offsets,
-      static_cast<T*>(h), gate_up, rows, experts, hidden, output, activation);
+  const int groups = ceil_div(output, kFewCols);
+  // One token's routes go to different experts, so up to two rows are taken
+  // one at a time; more may share an expert.
+  const bool single = rows <= 2;
+  // Contraction steps of a thread without a split; a split leaves four.
+  const int steps = hidden / (kFewThreads / (kFewCols / (vec ? kVec : 1)));
+  int split = 1;
+  while (split < kMaxSplit &&
+         static_cast<long long>(groups) * rows * split < (single ? 4 : 2) * kNumSms &&
+         steps >= 8 * split) {
+    split *= 2;
+  }
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = split;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(groups * split, rows);
+  cfg.blockDim = dim3(kFewThreads);
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(
+      &cfg,
+      vec ? (single ? gated_few_kernel<T, kVec, 1> : gated_few_kernel<T, kVec, kFewRows>)
+          : (single ? gated_few_kernel<T, 1, 1> : gated_few_kernel<T, 1, kFewRows>),
+      static_cast<const T*>(x),
+      static_cast<const T*>(wg), static_cast<const T*>(wu), offsets, static_cast<T*>(h), gate_up,
+      rows, experts, hidden, output, activation, split);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return e;
+  }
   note_launch();
-  return cudaGetLastError();
+  return cudaSuccess;
 }
 
 // ---- operand parts -----------------------------------------------------------------

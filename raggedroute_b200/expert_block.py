@@ -10,10 +10,12 @@ device of its tensors. No reference counterpart.
 """
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
-from raggedroute_b200._lib import Context, check, lib
-from raggedroute_b200.ops import _ctx, _need, _ptr
+from raggedroute_b200._lib import Context, RRContext, check, lib
+from raggedroute_b200.ops import _need
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 2}
 ACTIVATIONS = {"silu": 0, "gelu_tanh": 1, "relu": 2}
@@ -31,36 +33,53 @@ def _activation(name: str) -> int:
     return ACTIVATIONS[name]
 
 
-def _expect(t: torch.Tensor | None, shape: tuple, dtype: torch.dtype, device: torch.device,
+def _refuse(t: torch.Tensor, shape: tuple, dtype: torch.dtype, device: torch.device,
             name: str) -> None:
-    """`t` (None passes) is a contiguous tensor of this shape, type and device."""
-    if t is None:
-        return
     _need(t, dtype, name)
     if t.shape != shape:
         raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
-    if t.device != device:
-        raise ValueError(f"{name} must be on {device}, got {t.device}")
+    raise ValueError(f"{name} must be on {device}, got {t.device}")
+
+
+def _expect(t: torch.Tensor | None, shape: tuple, dtype: torch.dtype, device: torch.device,
+            name: str) -> int | None:
+    """The address of `t`, a contiguous tensor of this shape, type and device;
+    None passes as a null pointer."""
+    if t is None:
+        return None
+    if t.dtype != dtype or t.shape != shape or t.device != device or not t.is_contiguous():
+        _refuse(t, shape, dtype, device, name)
+    return t.data_ptr() or None
 
 
 def _rank(t: torch.Tensor, dims: int, name: str) -> None:
     if t.dim() != dims:
         raise ValueError(f"{name} must have {dims} dimensions, got {t.dim()}")
-    if t.device.type != "cuda":
+    if not t.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor, got {t.device}")
 
 
-def _call(name: str, device: torch.device, ctx: Context | None,
+def _call(fn, name: str, device: torch.device, ctx: Context | None,
           workspace: torch.Tensor | None, *args) -> None:
-    """Calls lib().rr_<name>(*args, context) with `device` current."""
-    if workspace is not None and workspace.device != device:
-        raise ValueError(f"workspace must be on {device}, got {workspace.device}")
-    fn = getattr(lib(), "rr_" + name)
-    if device.index is None or device.index == torch.cuda.current_device():
-        check(fn(*args, _ctx(ctx, workspace)), name)
-    else:
+    """fn(*args, context) with `device` current, on its current stream unless
+    ctx names one."""
+    if workspace is not None and (workspace.device != device or not workspace.is_contiguous()):
+        raise ValueError(f"workspace must be a contiguous tensor on {device}")
+    if device.index != torch.cuda.current_device():
         with torch.cuda.device(device):
-            check(fn(*args, _ctx(ctx, workspace)), name)
+            return _call(fn, name, device, ctx, workspace, *args)
+    if ctx is not None:
+        c = ctx.as_c()
+        if not c.stream:
+            c.stream = torch.cuda.current_stream().cuda_stream
+    else:
+        c = RRContext(torch._C._cuda_getCurrentRawStream(device.index))
+    if workspace is not None:
+        c.workspace = workspace.data_ptr()
+        c.workspace_bytes = workspace.numel() * workspace.element_size()
+    status = fn(*args, ctypes.byref(c))
+    if status.code != 0:
+        check(status, name)
 
 
 # ---- gated projection ------------------------------------------------------------
@@ -76,17 +95,21 @@ def grouped_gated_gemm_workspace_size(route_pairs: int, experts: int, hidden: in
     return size
 
 
-def _gated_sizes(x: torch.Tensor, gate_weights: torch.Tensor, up_weights: torch.Tensor,
-                 offsets: torch.Tensor) -> tuple[int, int, int, int]:
+def _gated_inputs(x: torch.Tensor, gate_weights: torch.Tensor, up_weights: torch.Tensor,
+                  offsets: torch.Tensor):
+    """((rows, experts, hidden, output), the four addresses)."""
     _rank(x, 2, "x_permuted")
     _rank(gate_weights, 3, "gate_weights")
     rows, hidden = x.shape
-    experts, _, output = gate_weights.shape
-    _expect(x, (rows, hidden), x.dtype, x.device, "x_permuted")
-    _expect(gate_weights, (experts, hidden, output), x.dtype, x.device, "gate_weights")
-    _expect(up_weights, (experts, hidden, output), x.dtype, x.device, "up_weights")
-    _expect(offsets, (experts + 1,), torch.int32, x.device, "offsets")
-    return rows, experts, hidden, output
+    experts, _, output = w_shape = gate_weights.shape
+    if w_shape[1] != hidden:
+        raise ValueError(f"gate_weights must be [E, {hidden}, N], got {tuple(w_shape)}")
+    dtype, device = x.dtype, x.device
+    return (rows, experts, hidden, output), (
+        _expect(x, x.shape, dtype, device, "x_permuted"),
+        _expect(gate_weights, w_shape, dtype, device, "gate_weights"),
+        _expect(up_weights, w_shape, dtype, device, "up_weights"),
+        _expect(offsets, (experts + 1,), torch.int32, device, "offsets"))
 
 
 def grouped_gated_gemm(x_permuted: torch.Tensor, gate_weights: torch.Tensor,
@@ -99,14 +122,14 @@ def grouped_gated_gemm(x_permuted: torch.Tensor, gate_weights: torch.Tensor,
     up_weights [E, K, N], h [R, N]; gate_up (float32 [R, 2N]) receives both
     products for the backward pass. activation: silu, gelu_tanh or relu.
     workspace from grouped_gated_gemm_workspace_size."""
-    dtype = _dtype(x_permuted.dtype, "x_permuted")
-    rows, experts, hidden, output = _gated_sizes(x_permuted, gate_weights, up_weights, offsets)
+    dtype, act = _dtype(x_permuted.dtype, "x_permuted"), _activation(activation)
+    sizes, inputs = _gated_inputs(x_permuted, gate_weights, up_weights, offsets)
+    rows, _, _, output = sizes
     device = x_permuted.device
-    _expect(h, (rows, output), x_permuted.dtype, device, "h")
-    _expect(gate_up, (rows, 2 * output), torch.float32, device, "gate_up")
-    _call("grouped_gated_gemm", device, ctx, workspace, _ptr(x_permuted), _ptr(gate_weights),
-          _ptr(up_weights), _ptr(offsets), _ptr(h), _ptr(gate_up), rows, experts, hidden, output,
-          _activation(activation), dtype)
+    _call(lib().rr_grouped_gated_gemm, "grouped_gated_gemm", device, ctx, workspace, *inputs,
+          _expect(h, (rows, output), x_permuted.dtype, device, "h"),
+          _expect(gate_up, (rows, 2 * output), torch.float32, device, "gate_up"), *sizes, act,
+          dtype)
     return h
 
 
@@ -121,18 +144,17 @@ def grouped_gated_gemm_backward(x_permuted: torch.Tensor, gate_weights: torch.Te
     (rr_grouped_gated_gemm_backward). dx [R, K] may be None, or both weight
     gradients [E, K, N]. workspace from
     grouped_gated_gemm_workspace_size(..., backward=True)."""
-    dtype = _dtype(x_permuted.dtype, "x_permuted")
-    rows, experts, hidden, output = _gated_sizes(x_permuted, gate_weights, up_weights, offsets)
-    t, device = x_permuted.dtype, x_permuted.device
-    _expect(gate_up, (rows, 2 * output), torch.float32, device, "gate_up")
-    _expect(dh, (rows, output), t, device, "dh")
-    _expect(dx, (rows, hidden), t, device, "dx")
-    _expect(d_gate_weights, (experts, hidden, output), t, device, "d_gate_weights")
-    _expect(d_up_weights, (experts, hidden, output), t, device, "d_up_weights")
-    _call("grouped_gated_gemm_backward", device, ctx, workspace, _ptr(x_permuted),
-          _ptr(gate_weights), _ptr(up_weights), _ptr(offsets), _ptr(gate_up), _ptr(dh), _ptr(dx),
-          _ptr(d_gate_weights), _ptr(d_up_weights), rows, experts, hidden, output,
-          _activation(activation), dtype)
+    dtype, act = _dtype(x_permuted.dtype, "x_permuted"), _activation(activation)
+    sizes, inputs = _gated_inputs(x_permuted, gate_weights, up_weights, offsets)
+    rows, experts, hidden, output = sizes
+    t, device, weights = x_permuted.dtype, x_permuted.device, (experts, hidden, output)
+    _call(lib().rr_grouped_gated_gemm_backward, "grouped_gated_gemm_backward", device, ctx,
+          workspace, *inputs,
+          _expect(gate_up, (rows, 2 * output), torch.float32, device, "gate_up"),
+          _expect(dh, (rows, output), t, device, "dh"),
+          _expect(dx, (rows, hidden), t, device, "dx"),
+          _expect(d_gate_weights, weights, t, device, "d_gate_weights"),
+          _expect(d_up_weights, weights, t, device, "d_up_weights"), *sizes, act, dtype)
 
 
 # ---- 8-bit integers ----------------------------------------------------------------
@@ -153,11 +175,11 @@ def quantize_rows_int8(x: torch.Tensor, xq: torch.Tensor, x_scale: torch.Tensor,
     dtype = _dtype(x.dtype, "x")
     _rank(x, 2, "x")
     rows, hidden = x.shape
-    _expect(x, (rows, hidden), x.dtype, x.device, "x")
-    _expect(xq, (rows, int8_row_stride(hidden)), torch.int8, x.device, "xq")
-    _expect(x_scale, (rows,), torch.float32, x.device, "x_scale")
-    _call("quantize_rows_int8", x.device, ctx, None, _ptr(x), _ptr(xq), _ptr(x_scale), rows,
-          hidden, dtype)
+    device = x.device
+    _call(lib().rr_quantize_rows_int8, "quantize_rows_int8", device, ctx, None,
+          _expect(x, x.shape, x.dtype, device, "x"),
+          _expect(xq, (rows, int8_row_stride(hidden)), torch.int8, device, "xq"),
+          _expect(x_scale, (rows,), torch.float32, device, "x_scale"), rows, hidden, dtype)
 
 
 def quantize_expert_weights_int8(expert_weights: torch.Tensor, wq: torch.Tensor,
@@ -169,12 +191,12 @@ def quantize_expert_weights_int8(expert_weights: torch.Tensor, wq: torch.Tensor,
     _rank(expert_weights, 3, "expert_weights")
     experts, hidden, output = expert_weights.shape
     device = expert_weights.device
-    _expect(expert_weights, (experts, hidden, output), expert_weights.dtype, device,
-            "expert_weights")
-    _expect(wq, (experts, output, int8_row_stride(hidden)), torch.int8, device, "wq")
-    _expect(w_scale, (experts, output), torch.float32, device, "w_scale")
-    _call("quantize_expert_weights_int8", device, ctx, None, _ptr(expert_weights), _ptr(wq),
-          _ptr(w_scale), experts, hidden, output, dtype)
+    _call(lib().rr_quantize_expert_weights_int8, "quantize_expert_weights_int8", device, ctx, None,
+          _expect(expert_weights, expert_weights.shape, expert_weights.dtype, device,
+                  "expert_weights"),
+          _expect(wq, (experts, output, int8_row_stride(hidden)), torch.int8, device, "wq"),
+          _expect(w_scale, (experts, output), torch.float32, device, "w_scale"), experts, hidden,
+          output, dtype)
 
 
 def grouped_gemm_int8(xq: torch.Tensor, x_scale: torch.Tensor, wq: torch.Tensor,
@@ -191,33 +213,34 @@ def grouped_gemm_int8(xq: torch.Tensor, x_scale: torch.Tensor, wq: torch.Tensor,
     device = xq.device
     if int8_row_stride(stride) != stride:
         raise ValueError(f"xq rows must be int8_row_stride(K) long, got {stride}")
-    _expect(xq, (rows, stride), torch.int8, device, "xq")
-    _expect(x_scale, (rows,), torch.float32, device, "x_scale")
-    _expect(wq, (experts, output, stride), torch.int8, device, "wq")
-    _expect(w_scale, (experts, output), torch.float32, device, "w_scale")
-    _expect(offsets, (experts + 1,), torch.int32, device, "offsets")
-    _expect(y_permuted, (rows, output), y_permuted.dtype, device, "y_permuted")
-    _call("grouped_gemm_int8", device, ctx, None, _ptr(xq), _ptr(x_scale), _ptr(wq),
-          _ptr(w_scale), _ptr(offsets), _ptr(y_permuted), rows, experts, stride, output, dtype)
+    _call(lib().rr_grouped_gemm_int8, "grouped_gemm_int8", device, ctx, None,
+          _expect(xq, xq.shape, torch.int8, device, "xq"),
+          _expect(x_scale, (rows,), torch.float32, device, "x_scale"),
+          _expect(wq, (experts, output, stride), torch.int8, device, "wq"),
+          _expect(w_scale, (experts, output), torch.float32, device, "w_scale"),
+          _expect(offsets, (experts + 1,), torch.int32, device, "offsets"),
+          _expect(y_permuted, (rows, output), y_permuted.dtype, device, "y_permuted"), rows,
+          experts, stride, output, dtype)
     return y_permuted
 
 
 # ---- combine, norms, gate, residual --------------------------------------------------
 
-def _norm_sizes(y_permuted, route_pos, route_weights, residual, post_gamma, gate,
-                pre_gamma) -> tuple[int, int, int]:
+def _norm_inputs(y_permuted, route_pos, route_weights, residual, post_gamma, gate, pre_gamma):
+    """((tokens, top_k, output), the seven addresses)."""
     _rank(residual, 2, "residual")
     _rank(route_pos, 2, "route_pos")
     tokens, output = residual.shape
     top_k = route_pos.shape[1]
     t, device, f32 = residual.dtype, residual.device, torch.float32
-    _expect(y_permuted, (tokens * top_k, output), t, device, "y_permuted")
-    _expect(route_pos, (tokens, top_k), torch.int32, device, "route_pos")
-    _expect(route_weights, (tokens, top_k), f32, device, "route_weights")
-    _expect(residual, (tokens, output), t, device, "residual")
-    for p, name in ((post_gamma, "post_gamma"), (gate, "gate"), (pre_gamma, "pre_gamma")):
-        _expect(p, (output,), f32, device, name)
-    return tokens, top_k, output
+    return (tokens, top_k, output), (
+        _expect(y_permuted, (tokens * top_k, output), t, device, "y_permuted"),
+        _expect(route_pos, (tokens, top_k), torch.int32, device, "route_pos"),
+        _expect(route_weights, (tokens, top_k), f32, device, "route_weights"),
+        _expect(residual, residual.shape, t, device, "residual"),
+        _expect(post_gamma, (output,), f32, device, "post_gamma"),
+        _expect(gate, (output,), f32, device, "gate"),
+        _expect(pre_gamma, (output,), f32, device, "pre_gamma"))
 
 
 def unpermute_norm(y_permuted: torch.Tensor, route_pos: torch.Tensor,
@@ -239,16 +262,14 @@ def unpermute_norm(y_permuted: torch.Tensor, route_pos: torch.Tensor,
     gate it is not scaled, and normed goes with pre_gamma. inv_rms (float32
     [T, 2]) receives what the backward pass needs."""
     dtype = _dtype(residual.dtype, "residual")
-    tokens, top_k, output = _norm_sizes(y_permuted, route_pos, route_weights, residual,
-                                        post_gamma, gate, pre_gamma)
-    t, device = residual.dtype, residual.device
-    _expect(residual_out, (tokens, output), t, device, "residual_out")
-    _expect(normed, (tokens, output), t, device, "normed")
-    _expect(inv_rms, (tokens, 2), torch.float32, device, "inv_rms")
-    _call("unpermute_norm", device, ctx, None, _ptr(y_permuted), _ptr(route_pos),
-          _ptr(route_weights), _ptr(residual), _ptr(post_gamma), _ptr(gate), _ptr(pre_gamma),
-          _ptr(residual_out), _ptr(normed), _ptr(inv_rms), eps, residual_scale, tokens, top_k,
-          output, dtype)
+    sizes, inputs = _norm_inputs(y_permuted, route_pos, route_weights, residual, post_gamma, gate,
+                                 pre_gamma)
+    t, device, shape = residual.dtype, residual.device, residual.shape
+    _call(lib().rr_unpermute_norm, "unpermute_norm", device, ctx, None, *inputs,
+          _expect(residual_out, shape, t, device, "residual_out"),
+          _expect(normed, shape, t, device, "normed"),
+          _expect(inv_rms, (shape[0], 2), torch.float32, device, "inv_rms"), eps, residual_scale,
+          *sizes, dtype)
     return residual_out
 
 
@@ -276,20 +297,18 @@ def unpermute_norm_backward(y_permuted: torch.Tensor, route_pos: torch.Tensor,
     d_route_weights float32 [T, top_k] and the float32 [N] gradients of the
     parameters that are asked for."""
     dtype = _dtype(residual.dtype, "residual")
-    tokens, top_k, output = _norm_sizes(y_permuted, route_pos, route_weights, residual,
-                                        post_gamma, gate, pre_gamma)
-    t, device, f32 = residual.dtype, residual.device, torch.float32
-    _expect(inv_rms, (tokens, 2), f32, device, "inv_rms")
-    for g, name in ((d_residual_out, "d_residual_out"), (d_normed, "d_normed"),
-                    (d_residual, "d_residual")):
-        _expect(g, (tokens, output), t, device, name)
-    _expect(d_y_permuted, (tokens * top_k, output), t, device, "d_y_permuted")
-    _expect(d_route_weights, (tokens, top_k), f32, device, "d_route_weights")
-    for g, name in ((d_post_gamma, "d_post_gamma"), (d_gate, "d_gate"),
-                    (d_pre_gamma, "d_pre_gamma")):
-        _expect(g, (output,), f32, device, name)
-    _call("unpermute_norm_backward", device, ctx, workspace, _ptr(y_permuted), _ptr(route_pos),
-          _ptr(route_weights), _ptr(residual), _ptr(post_gamma), _ptr(gate), _ptr(pre_gamma),
-          _ptr(inv_rms), _ptr(d_residual_out), _ptr(d_normed), _ptr(d_residual),
-          _ptr(d_y_permuted), _ptr(d_route_weights), _ptr(d_post_gamma), _ptr(d_gate),
-          _ptr(d_pre_gamma), residual_scale, tokens, top_k, output, dtype)
+    sizes, inputs = _norm_inputs(y_permuted, route_pos, route_weights, residual, post_gamma, gate,
+                                 pre_gamma)
+    tokens, top_k, output = sizes
+    t, device, f32, shape = residual.dtype, residual.device, torch.float32, residual.shape
+    _call(lib().rr_unpermute_norm_backward, "unpermute_norm_backward", device, ctx, workspace,
+          *inputs, _expect(inv_rms, (tokens, 2), f32, device, "inv_rms"),
+          _expect(d_residual_out, shape, t, device, "d_residual_out"),
+          _expect(d_normed, shape, t, device, "d_normed"),
+          _expect(d_residual, shape, t, device, "d_residual"),
+          _expect(d_y_permuted, (tokens * top_k, output), t, device, "d_y_permuted"),
+          _expect(d_route_weights, (tokens, top_k), f32, device, "d_route_weights"),
+          _expect(d_post_gamma, (output,), f32, device, "d_post_gamma"),
+          _expect(d_gate, (output,), f32, device, "d_gate"),
+          _expect(d_pre_gamma, (output,), f32, device, "d_pre_gamma"), residual_scale, *sizes,
+          dtype)

@@ -27,6 +27,12 @@ SHAPES = [(1, 1, 1), (1, 2, 4096), (3, 2, 8), (5, 1, 33), (17, 8, 257), (64, 2, 
           (33, 2, 1024), (7, 64, 96), (6, 2, 4100), (4, 2, 8191), (3, 2, 8192), (3, 1, 8200),
           (2, 2, 16384), (2, 2, 16383), (2500, 2, 64), (700, 4, 1000)]
 
+# Enough tokens for the streamed form: each team size, rows that start on odd
+# addresses in both types, many routes, and token counts that end inside a stage.
+SHAPES += [(5001, 2, 96), (4800, 1, 511), (4738, 3, 333), (2400, 2, 1026), (1201, 16, 520),
+           (700, 2, 2340), (601, 2, 4096), (599, 2, 4095), (299, 2, 8192), (300, 1, 8191),
+           (297, 5, 6001)]
+
 
 class Inputs:
     def __init__(self, tokens, top_k, output, dtype, device, seed=0, post=True, gate=True,
