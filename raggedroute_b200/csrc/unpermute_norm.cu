@@ -363,7 +363,7 @@ __global__ void __launch_bounds__(kMaxThreads) unpermute_norm_backward_kernel(
 
 // ---- streamed form ------------------------------------------------------------------
 
-constexpr int kWorkers = 512;                   // worker threads per block
+constexpr int kWorkers = 512;                   // worker threads per block, at most
 constexpr int kStreamThreads = kWorkers + 32;   // and the producer warp
 constexpr int kStreamTopK = 16;
 constexpr int kMaxStages = 4;
@@ -609,7 +609,7 @@ __device__ __forceinline__ void stream_setup(const Stream& st, StreamSmem& s) {
   if (threadIdx.x == 0) {
     for (int i = 0; i < st.stages; ++i) {
       mbar_init(&s.full[i], 1);
-      mbar_init(&s.empty[i], kWorkers / 32);
+      mbar_init(&s.empty[i], st.team * st.teams / 32);
     }
     s.failed = 0;
     fence_mbar_init();
@@ -637,7 +637,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1) unpermute_norm_stream_kerne
   __shared__ StreamSmem s;
   stream_setup(st, s);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (threadIdx.x >= kWorkers) {
+  if (threadIdx.x >= st.team * st.teams) {
     Sources src;
     src.row[0] = in.residual;
     produce<T>(in, src, st, s, smem_u32(ring), err);
@@ -747,12 +747,12 @@ __global__ void __launch_bounds__(kStreamThreads, 1) unpermute_norm_backward_str
   const bool has_dro = g.d_residual_out != nullptr;
   float* pg = reinterpret_cast<float*>(ring + st.stages * st.teams * st.sources * st.stride);
   float* pr = pg + st.padded;
-  for (int c = threadIdx.x; c < st.padded; c += kStreamThreads) {
+  for (int c = threadIdx.x; c < st.padded; c += blockDim.x) {
     column_factors<1>(in, c, pg + c, pr + c);
   }
   stream_setup(st, s);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (threadIdx.x >= kWorkers) {
+  if (threadIdx.x >= st.team * st.teams) {
     Sources src;
     src.row[src.count++] = in.residual;
     if (has_dro) src.row[src.count++] = g.d_residual_out;
@@ -930,6 +930,302 @@ __global__ void __launch_bounds__(kStreamThreads, 1) unpermute_norm_backward_str
   stream_end(s);
 }
 
+// ---- the gradient for one or two routes per token ----------------------------------
+//
+// The same in one pass over the inputs and one reduction. With a = dro + i2 v
+// (v = dn pre) and f = post * gate:
+//   dr = a - i2 m2 rn,  v1 = f dr,  m2 = mean(v rn)
+//   P_k = <v1, y_k> = <f a, y_k> - i2 m2 <f rn, y_k>
+//   mean(v1 cn) = i1 sum_k w_k P_k / N,  Q_k = <cn, y_k> = i1 sum_j w_j <y_j, y_k>
+// so a token's eight sums are known together, before any of its results. Two
+// columns share an instruction (packed FP32 arithmetic, which rounds each half
+// as the plain instruction does).
+
+struct F2 {
+  unsigned long long v;
+};
+__device__ __forceinline__ F2 f2(float lo, float hi) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ F2 f2(float x) { return f2(x, x); }
+__device__ __forceinline__ void split(F2 a, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(a.v));
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ float sum2(F2 a) {
+  float lo, hi;
+  split(a, lo, hi);
+  return lo + hi;
+}
+
+// Eight columns per thread: a token's c, a and rn and the thread's column sums
+// then stay in registers with sixteen warps per SM (sixteen columns spilled,
+// and eight warps leave too little to overlap).
+constexpr int kPairElems = 8;
+constexpr int kPairs = kPairElems / 2;
+
+// This thread's columns of a staged row in pairs, zero past the row's end.
+template <typename T, int kPer>
+__device__ __forceinline__ void staged_row(const char* row, int output, int team, int tid,
+                                           F2 (&v)[kPairs]) {
+  float f[kPairElems];
+#pragma unroll
+  for (int q = 0; q < kPairElems / kPer; ++q) {
+    const int col = (q * team + tid) * kPer;
+    if (col < output) {
+      staged_cols<T, kPer>(row + col * sizeof(T), f + q * kPer);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) f[q * kPer + i] = 0.0f;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kPairs; ++i) v[i] = f2(f[2 * i], f[2 * i + 1]);
+}
+
+template <int kPer>
+__device__ __forceinline__ void shared_row(const float* row, int output, int team, int tid,
+                                           F2 (&v)[kPairs]) {
+  float f[kPairElems];
+#pragma unroll
+  for (int q = 0; q < kPairElems / kPer; ++q) {
+    const int col = (q * team + tid) * kPer;
+    if (col < output) {
+      shared_cols<kPer>(row + col, f + q * kPer);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) f[q * kPer + i] = 0.0f;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kPairs; ++i) v[i] = f2(f[2 * i], f[2 * i + 1]);
+}
+
+template <typename T, int kPer>
+__device__ __forceinline__ void put_row(T* row, int output, int team, int tid,
+                                        const F2 (&v)[kPairs]) {
+  float f[kPairElems];
+#pragma unroll
+  for (int i = 0; i < kPairs; ++i) split(v[i], f[2 * i], f[2 * i + 1]);
+#pragma unroll
+  for (int q = 0; q < kPairElems / kPer; ++q) {
+    const int col = (q * team + tid) * kPer;
+    if (col < output) put_cols<T, kPer>(row + col, f + q * kPer);
+  }
+}
+
+// Eight sums over a warp with nine shuffles: halves of the warp exchange halves
+// of the sums until each lane holds one; lane l ends with the sum l / 4.
+__device__ __forceinline__ float warp_sum8(const float (&v)[8]) {
+  const int lane = threadIdx.x & 31;
+  float a[4], b[2];
+  const bool h4 = lane & 16, h3 = lane & 8, h2 = lane & 4;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float keep = h4 ? v[4 + i] : v[i], give = h4 ? v[i] : v[4 + i];
+    a[i] = keep + __shfl_xor_sync(0xffffffffu, give, 16);
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const float keep = h3 ? a[2 + i] : a[i], give = h3 ? a[i] : a[2 + i];
+    b[i] = keep + __shfl_xor_sync(0xffffffffu, give, 8);
+  }
+  float c = (h2 ? b[1] : b[0]) + __shfl_xor_sync(0xffffffffu, h2 ? b[0] : b[1], 4);
+  c += __shfl_xor_sync(0xffffffffu, c, 2);
+  return c + __shfl_xor_sync(0xffffffffu, c, 1);
+}
+
+template <typename T, int kPer>
+__global__ void __launch_bounds__(kStreamThreads, 1) unpermute_norm_backward_pair_kernel(
+    const UnpermuteNorm in, const Stream st, const UnpermuteNormGrads g, float* partial,
+    unsigned* err) {
+  using namespace sm100;
+  extern __shared__ __align__(16) char ring[];
+  __shared__ StreamSmem s;
+  __shared__ float sums[2][kMaxTeams][8];  // of each warp, by parity of the token
+  const bool post = in.post_gamma != nullptr, pre = in.pre_gamma != nullptr;
+  const bool has_dro = g.d_residual_out != nullptr;
+  float* pg = reinterpret_cast<float*>(ring + st.stages * st.teams * st.sources * st.stride);
+  float* pr = pg + st.padded;
+  for (int c = threadIdx.x; c < st.padded; c += blockDim.x) {
+    column_factors<1>(in, c, pg + c, pr + c);
+  }
+  stream_setup(st, s);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x >= st.team * st.teams) {
+    Sources src;
+    src.row[src.count++] = in.residual;
+    if (has_dro) src.row[src.count++] = g.d_residual_out;
+    if (pre) src.row[src.count++] = g.d_normed;
+    produce<T>(in, src, st, s, smem_u32(ring), err);
+    stream_end(s);
+    return;
+  }
+  const int team = threadIdx.x / st.team, tid = threadIdx.x % st.team;
+  const int team_warps = st.team >> 5, warp0 = team * team_warps;
+  const int n = in.output;
+  const float per_col = 1.0f / static_cast<float>(n);
+  const int at_res = in.top_k, at_dro = in.top_k + 1, at_dn = in.top_k + 1 + (has_dro ? 1 : 0);
+  F2 s_dc[kPairs], s_pre[kPairs];  // sums over tokens of dr cn and dn rn
+#pragma unroll
+  for (int i = 0; i < kPairs; ++i) s_dc[i] = s_pre[i] = f2(0.0f);
+  int stage = 0, parity = 0;
+  uint32_t phase = 0;
+  const long long step = static_cast<long long>(gridDim.x) * st.teams;
+  for (long long first = static_cast<long long>(blockIdx.x) * st.teams; first < in.tokens;
+       first += step) {
+    const bool ok = mbar_wait(&s.full[stage], phase, err, &s.failed);
+    if (!team_all(team, st.team, ok)) break;
+    const long long t = first + team;
+    if (t < in.tokens) {  // uniform over a team
+      const int* start = s.start[stage][team];
+      const bool there0 = start[0] >= 0, there1 = in.top_k > 1 && start[1] >= 0;
+      const float w0 = there0 ? s.weight[stage][team][0] : 0.0f;
+      const float w1 = there1 ? s.weight[stage][team][1] : 0.0f;
+      const float i1 = post ? __ldg(g.inv_rms + 2 * t) : 1.0f;
+      const float i2 = pre ? __ldg(g.inv_rms + 2 * t + 1) : 0.0f;
+      F2 c[kPairs], a[kPairs], rn[kPairs];
+      float v8[8];  // <v, rn>, <f a, y0>, <f a, y1>, <f rn, y0>, <f rn, y1>, <y0, y0>, ...
+      {
+        F2 y0[kPairs], y1[kPairs], x[kPairs], f[kPairs], sum[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum[j] = f2(0.0f);
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) y0[i] = y1[i] = f2(0.0f);
+        if (there0) staged_row<T, kPer>(ring + start[0], n, st.team, tid, y0);
+        if (there1) staged_row<T, kPer>(ring + start[1], n, st.team, tid, y1);
+        shared_row<kPer>(pg, n, st.team, tid, f);
+        staged_row<T, kPer>(ring + start[at_res], n, st.team, tid, x);
+        const F2 w02 = f2(w0), w12 = f2(w1), i12 = f2(i1), i22 = f2(i2);
+        const F2 scale = f2(in.residual_scale);
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) {
+          c[i] = mul2(i12, fma2(w12, y1[i], mul2(w02, y0[i])));
+          rn[i] = mul2(i22, fma2(scale, x[i], mul2(c[i], f[i])));
+        }
+        if (has_dro) {
+          staged_row<T, kPer>(ring + start[at_dro], n, st.team, tid, a);
+        } else {
+#pragma unroll
+          for (int i = 0; i < kPairs; ++i) a[i] = f2(0.0f);
+        }
+        if (pre) {
+          F2 p[kPairs];
+          staged_row<T, kPer>(ring + start[at_dn], n, st.team, tid, x);
+          shared_row<kPer>(pr, n, st.team, tid, p);
+#pragma unroll
+          for (int i = 0; i < kPairs; ++i) {
+            s_pre[i] = fma2(x[i], rn[i], s_pre[i]);
+            const F2 v = mul2(x[i], p[i]);
+            sum[0] = fma2(v, rn[i], sum[0]);
+            a[i] = fma2(i22, v, a[i]);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) {
+          const F2 fa = mul2(f[i], a[i]), fr = mul2(f[i], rn[i]);
+          sum[1] = fma2(fa, y0[i], sum[1]);
+          sum[2] = fma2(fa, y1[i], sum[2]);
+          sum[3] = fma2(fr, y0[i], sum[3]);
+          sum[4] = fma2(fr, y1[i], sum[4]);
+          sum[5] = fma2(y0[i], y0[i], sum[5]);
+          sum[6] = fma2(y0[i], y1[i], sum[6]);
+          sum[7] = fma2(y1[i], y1[i], sum[7]);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v8[j] = sum2(sum[j]);
+      }
+      // The team's sums: lane l of every warp ends with the sum l / 4.
+      float mine = warp_sum8(v8);
+      if (team_warps > 1) {
+        if ((lane & 3) == 0) sums[parity][warp][lane >> 2] = mine;
+        team_sync(team, st.team);
+        mine = 0.0f;
+        for (int w = lane & 3; w < team_warps; w += 4) mine += sums[parity][warp0 + w][lane >> 2];
+        mine += __shfl_xor_sync(0xffffffffu, mine, 1);
+        mine += __shfl_xor_sync(0xffffffffu, mine, 2);
+        parity ^= 1;
+      }
+      auto total = [&](int j) { return __shfl_sync(0xffffffffu, mine, 4 * j); };
+      const float im2 = i2 * (total(0) * per_col);
+      const float p0 = total(1) - im2 * total(3), p1 = total(2) - im2 * total(4);
+      const float g00 = total(5), g01 = total(6), g11 = total(7);
+      const float m1 = post ? i1 * (w0 * p0 + w1 * p1) * per_col : 0.0f;
+      if (tid == 0) {
+        const float q0 = i1 * (w0 * g00 + w1 * g01), q1 = i1 * (w0 * g01 + w1 * g11);
+        float* dw = g.d_route_weights + t * in.top_k;
+        dw[0] = there0 ? i1 * (p0 - m1 * q0) : 0.0f;
+        if (in.top_k > 1) dw[1] = there1 ? i1 * (p1 - m1 * q1) : 0.0f;
+      }
+      {
+        F2 x[kPairs];
+        const F2 nim2 = f2(-im2), scale = f2(in.residual_scale);
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) {
+          a[i] = fma2(nim2, rn[i], a[i]);  // dr
+          s_dc[i] = fma2(a[i], c[i], s_dc[i]);
+          x[i] = mul2(scale, a[i]);
+        }
+        put_row<T, kPer>(static_cast<T*>(g.d_residual) + t * n, n, st.team, tid, x);
+        shared_row<kPer>(pg, n, st.team, tid, x);
+        const F2 i12 = f2(i1), nm1 = f2(-m1);
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) {
+          a[i] = mul2(i12, fma2(nm1, c[i], mul2(x[i], a[i])));  // dc
+        }
+        T* rows = static_cast<T*>(g.d_y_permuted);
+        if (there0) {
+          const F2 w = f2(w0);
+#pragma unroll
+          for (int i = 0; i < kPairs; ++i) x[i] = mul2(w, a[i]);
+          put_row<T, kPer>(rows + static_cast<long long>(s.pos[stage][team][0]) * n, n, st.team,
+                           tid, x);
+        }
+        if (there1) {
+          const F2 w = f2(w1);
+#pragma unroll
+          for (int i = 0; i < kPairs; ++i) x[i] = mul2(w, a[i]);
+          put_row<T, kPer>(rows + static_cast<long long>(s.pos[stage][team][1]) * n, n, st.team,
+                           tid, x);
+        }
+      }
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&s.empty[stage]);
+    if (++stage == st.stages) {
+      stage = 0;
+      phase ^= 1u;
+    }
+  }
+  // This team's shares of the column sums: [block * teams + team][3][output].
+  float* p = partial + 3LL * (static_cast<long long>(blockIdx.x) * st.teams + team) * n;
+#pragma unroll
+  for (int i = 0; i < kPairElems; ++i) {
+    const int col = ((i / kPer) * st.team + tid) * kPer + i % kPer;
+    if (col < n) {
+      float lo, hi;
+      split(s_dc[i / 2], lo, hi);
+      const float d = i % 2 ? hi : lo;
+      split(s_pre[i / 2], lo, hi);
+      p[col] = in.gate != nullptr ? d * __ldg(in.gate + col) : d;
+      p[n + col] = post ? d * __ldg(in.post_gamma + col) : d;
+      p[2 * n + col] = i % 2 ? hi : lo;
+    }
+  }
+  stream_end(s);
+}
+
 constexpr int kSumThreads = 256;
 constexpr int kSumCols = 32;
 
@@ -966,19 +1262,22 @@ int row_threads(int output, int per) {
 // The streamed form's layout, or blocks = 0 where the plain one runs: few
 // tokens (the ring has to fill before it pays: two stages per SM), more routes
 // than a stage keeps track of, or rows of which two stages do not fit.
-Stream stream_plan(int tokens, int top_k, int output, int extra_rows, bool gradient,
+Stream stream_plan(int tokens, int top_k, int output, int extra_rows, bool gradient, int elems,
                    std::size_t size) {
   Stream st;
-  if (top_k > kStreamTopK || output > kWorkers * kElems) return st;
-  st.team = row_threads(output, kElems);
+  if (top_k > kStreamTopK || output > kWorkers * elems) return st;
+  st.team = row_threads(output, elems);
   st.teams = kWorkers / st.team;
   st.sources = top_k + extra_rows;
   if (st.teams * st.sources > 32 * kRounds) return st;
   // A row's granules: up to 15 bytes before and after it.
   st.stride = static_cast<int>((output * size + 15) / 16 * 16 + 16);
   if (gradient) st.padded = (output + 3) / 4 * 4;
-  const std::size_t stage = static_cast<std::size_t>(st.teams) * st.sources * st.stride;
-  st.stages = static_cast<int>((kRingBytes - 8 * st.padded) / stage);
+  for (;; st.teams /= 2) {  // two stages have to fit: halve the teams until they do
+    const std::size_t stage = static_cast<std::size_t>(st.teams) * st.sources * st.stride;
+    st.stages = static_cast<int>((kRingBytes - 8 * st.padded) / stage);
+    if (st.stages >= 2 || st.teams == 1) break;
+  }
   if (st.stages > kMaxStages) st.stages = kMaxStages;
   const int fill = 2 * kNumSms * st.teams;
   if (st.stages >= 2 && tokens >= fill) st.blocks = kNumSms;
@@ -987,6 +1286,12 @@ Stream stream_plan(int tokens, int top_k, int output, int extra_rows, bool gradi
 
 std::size_t ring_bytes(const Stream& st) {
   return static_cast<std::size_t>(st.stages) * st.teams * st.sources * st.stride + 8 * st.padded;
+}
+
+// Columns per thread of the streamed gradient: one or two routes per token have
+// a kernel of their own, up to the width its teams cover.
+int gradient_elems(int top_k, int output) {
+  return top_k <= 2 && output <= kWorkers * kPairElems ? kPairElems : kElems;
 }
 
 // One resident wave of the plain gradient kernel (about 128 registers per
@@ -1079,7 +1384,7 @@ cudaError_t forward_stream(const UnpermuteNorm& in, const Stream& st, void* resi
                            void* normed, float* inv_rms, cudaStream_t stream) {
   constexpr auto kernel = unpermute_norm_stream_kernel<T, kPer>;
   if (!allow_ring<kernel>()) return cudaErrorNotSupported;
-  kernel<<<st.blocks, kStreamThreads, ring_bytes(st), stream>>>(
+  kernel<<<st.blocks, st.team * st.teams + 32, ring_bytes(st), stream>>>(
       in, st, static_cast<T*>(residual_out), static_cast<T*>(normed), inv_rms,
       device_error_word());
   note_launch();
@@ -1089,10 +1394,12 @@ cudaError_t forward_stream(const UnpermuteNorm& in, const Stream& st, void* resi
 template <typename T, int kPer>
 cudaError_t backward_stream(const UnpermuteNorm& in, const Stream& st, const UnpermuteNormGrads& g,
                             float* workspace, cudaStream_t stream) {
-  constexpr auto kernel = unpermute_norm_backward_stream_kernel<T, kPer>;
-  if (!allow_ring<kernel>()) return cudaErrorNotSupported;
-  kernel<<<st.blocks, kStreamThreads, ring_bytes(st), stream>>>(in, st, g, workspace,
-                                                                device_error_word());
+  constexpr auto any = unpermute_norm_backward_stream_kernel<T, kPer>;
+  constexpr auto pair = unpermute_norm_backward_pair_kernel<T, kPer>;
+  const bool two = gradient_elems(in.top_k, in.output) == kPairElems;
+  if (!(two ? allow_ring<pair>() : allow_ring<any>())) return cudaErrorNotSupported;
+  (two ? pair : any)<<<st.blocks, st.team * st.teams + 32, ring_bytes(st), stream>>>(
+      in, st, g, workspace, device_error_word());
   note_launch();
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
@@ -1103,7 +1410,7 @@ cudaError_t backward_stream(const UnpermuteNorm& in, const Stream& st, const Unp
 
 cudaError_t launch_unpermute_norm(const UnpermuteNorm& in, void* residual_out, void* normed,
                                   float* inv_rms, Dtype dtype, cudaStream_t stream) {
-  const Stream st = stream_plan(in.tokens, in.top_k, in.output, 1, false, dtype_bytes(dtype));
+  const Stream st = stream_plan(in.tokens, in.top_k, in.output, 1, false, kElems, dtype_bytes(dtype));
   const int per = stream_columns(in.output, dtype);
   const std::size_t unit = per * dtype_bytes(dtype);
   if (st.blocks > 0 && aligned_to(in.y_permuted, 16) && aligned_to(in.residual, 16) &&
@@ -1131,10 +1438,14 @@ std::size_t unpermute_norm_backward_workspace_bytes(int tokens, int output) {
   // Shares of the column sums: of the plain form's blocks or the streamed
   // form's teams, whichever is more.
   std::size_t parts = static_cast<std::size_t>(backward_blocks(tokens, output));
+  const int elems = gradient_elems(1, output);
   if (output <= kWorkers * kElems) {
-    const std::size_t teams =
-        static_cast<std::size_t>(kNumSms) * (kWorkers / row_threads(output, kElems));
-    if (teams > parts && tokens >= static_cast<long long>(teams)) parts = teams;
+    const std::size_t teams = static_cast<std::size_t>(kNumSms) *
+                              (kWorkers / row_threads(output, kElems));
+    const std::size_t narrow = static_cast<std::size_t>(kNumSms) *
+                               (kWorkers / row_threads(output, elems));
+    const std::size_t most = teams > narrow ? teams : narrow;
+    if (most > parts && tokens >= static_cast<long long>(narrow)) parts = most;
   }
   return 12 * parts * output;
 }
@@ -1142,7 +1453,8 @@ std::size_t unpermute_norm_backward_workspace_bytes(int tokens, int output) {
 cudaError_t launch_unpermute_norm_backward(const UnpermuteNorm& in, const UnpermuteNormGrads& g,
                                            float* workspace, Dtype dtype, cudaStream_t stream) {
   const int extra = 1 + (g.d_residual_out != nullptr) + (in.pre_gamma != nullptr);
-  const Stream st = stream_plan(in.tokens, in.top_k, in.output, extra, true, dtype_bytes(dtype));
+  const Stream st = stream_plan(in.tokens, in.top_k, in.output, extra, true,
+                                gradient_elems(in.top_k, in.output), dtype_bytes(dtype));
   const int per = stream_columns(in.output, dtype);
   const std::size_t unit = per * dtype_bytes(dtype);
   if (st.blocks > 0 && aligned_to(in.y_permuted, 16) && aligned_to(in.residual, 16) &&
