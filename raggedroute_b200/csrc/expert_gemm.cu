@@ -9,12 +9,16 @@
 //
 // A pair of CTAs computes a 256-row tile whose 256 accumulator columns are 256
 // output columns (kDx, kInt8) or 128 columns of each of two products that
-// share their A operand (kGated: gate and up; kDw: the two weight gradients).
-// B is held half by each CTA, so in the second form the even CTA loads Wg (or
-// dg) and the odd CTA Wu (or du), and one MMA of N = 256 advances both
-// products: x is read once for both projections, and gate and up of an output
-// element meet in one thread's registers, where the activation and the
-// product are applied.
+// share their A operand (kGated: gate and up; kDw: the two weight gradients),
+// so one MMA of N = 256 advances both products and x is read once for both.
+// Each CTA holds half of B: in kDw one gradient each, in kGated 64 columns of
+// gate and the same 64 of up, which then lie 64 accumulator columns apart in
+// one thread's row, where the activation and the product are applied.
+//
+// A tile with at most 128 rows left (the end of a segment, or an expert with
+// few rows) is issued with M = 128, 64 rows per CTA, at half the tensor time.
+// Its accumulator is folded: TMEM lanes 0-63 hold the even CTA's half of the
+// columns, lanes 64-127 the odd CTA's, both for the CTA's 64 rows.
 //
 // Operands reach shared memory by TMA in 128-byte-swizzled boxes of 16 KB per
 // operand, part and k-block (64 bfloat16 or 128 int8 deep). Whatever layout
@@ -104,16 +108,16 @@ struct alignas(1024) EngineSmem {
 };
 
 // kind::f16 with bfloat16 operands and FP32 accumulation.
-__host__ __device__ constexpr uint32_t idesc_f16(int n, bool a_mn, bool b_mn) {
+__host__ __device__ constexpr uint32_t idesc_f16(int m, int n, bool a_mn, bool b_mn) {
   return (1u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(a_mn) << 15) |
          (static_cast<uint32_t>(b_mn) << 16) | (static_cast<uint32_t>(n >> 3) << 17) |
-         (static_cast<uint32_t>(kTileM >> 4) << 24);
+         (static_cast<uint32_t>(m >> 4) << 24);
 }
 
 // kind::i8 with signed operands and 32-bit integer accumulation.
-__host__ __device__ constexpr uint32_t idesc_i8(int n) {
+__host__ __device__ constexpr uint32_t idesc_i8(int m, int n) {
   return (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n >> 3) << 17) |
-         (static_cast<uint32_t>(kTileM >> 4) << 24);
+         (static_cast<uint32_t>(m >> 4) << 24);
 }
 
 __device__ __forceinline__ void mma_i8_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
@@ -130,7 +134,9 @@ struct Tile {
   int expert;
   int m0, m_end;  // rows of the output (kDw: of the weight matrix)
   int c0, ncols;  // columns of each product
+  int m_mma;      // rows of the instruction: 256, or 128 when at most 128 are left
   int n_mma;      // accumulator columns, a multiple of 32
+  int own;        // kGated: gate (and up) columns of each CTA
   int blocks;     // k-blocks of the contraction
   int row0, row_end;  // the segment (kDw's contraction)
 };
@@ -194,7 +200,10 @@ __device__ __forceinline__ Tile tile_at(const EngineArgs& p, int t, const int* p
   const int total = kMode == kDx ? p.hidden : p.output;
   g.c0 = nt * width;
   g.ncols = min(width, total - g.c0);
-  g.n_mma = kTwo ? 2 * ((g.ncols + 15) & ~15) : (g.ncols + 31) & ~31;
+  // kGated: a CTA's up columns follow a whole box of 64 gate columns.
+  g.own = min(64, (((g.ncols + 1) >> 1) + 15) & ~15);
+  if constexpr (kMode == kGated) g.n_mma = 2 * (64 + g.own);
+  else g.n_mma = kTwo ? 2 * ((g.ncols + 15) & ~15) : (g.ncols + 31) & ~31;
   if constexpr (kMode == kDw) {
     g.m0 = mt * kTileM;
     g.m_end = p.hidden;
@@ -206,6 +215,7 @@ __device__ __forceinline__ Tile tile_at(const EngineArgs& p, int t, const int* p
     else if constexpr (kMode == kInt8) g.blocks = (p.hidden + 127) >> 7;
     else g.blocks = (p.hidden + 63) >> 6;
   }
+  g.m_mma = g.m_end - g.m0 <= kRowsCta ? kRowsCta : kTileM;
   return g;
 }
 
@@ -340,7 +350,7 @@ __global__ void __launch_bounds__(kThreads, 1) expert_gemm_kernel(
       uint32_t phase = 0;
       for (int t = unit; t < total && !*failed; t += units) {
         const Tile g = tile_at<kMode>(p, t, s.prefix, n_tiles);
-        const int m = g.m0 + static_cast<int>(rank) * kRowsCta;
+        const int m = g.m0 + static_cast<int>(rank) * (g.m_mma >> 1);
         const int half = g.n_mma >> 1;
         for (int kb = 0; kb < g.blocks; ++kb) {
           if (!wait(&s.empty[stage], phase ^ 1u)) break;
@@ -363,11 +373,11 @@ __global__ void __launch_bounds__(kThreads, 1) expert_gemm_kernel(
 #pragma unroll
           for (int q = 0; q < kTerms; ++q, a += kOperandBytes, b += kOperandBytes) {
             if constexpr (kMode == kGated) {
-              const CUtensorMap* mb = leader ? &map_b0 : &map_b1;
+              const int c = g.c0 + static_cast<int>(rank) * g.own;
               const int z = q * p.experts + g.expert;
               tma_load_3d_pair(a, &map_a0, bar, kb * 64, m, q);
-              tma_load_3d_pair(b, mb, bar, g.c0, kb * 64, z);
-              tma_load_3d_pair(b + kBoxBytes, mb, bar, g.c0 + 64, kb * 64, z);
+              tma_load_3d_pair(b, &map_b0, bar, c, kb * 64, z);
+              tma_load_3d_pair(b + kBoxBytes, &map_b1, bar, c, kb * 64, z);
             } else if constexpr (kMode == kDx) {
               const int per = g.blocks >> 1;
               const bool first = kb < per;
@@ -415,7 +425,8 @@ __global__ void __launch_bounds__(kThreads, 1) expert_gemm_kernel(
       for (int t = unit; t < total && ok && !*failed; t += units) {
         const Tile g = tile_at<kMode>(p, t, s.prefix, n_tiles);
         const uint32_t idesc =
-            kMode == kInt8 ? idesc_i8(g.n_mma) : idesc_f16(g.n_mma, kMnA, kMnB);
+            kMode == kInt8 ? idesc_i8(g.m_mma, g.n_mma)
+                           : idesc_f16(g.m_mma, g.n_mma, kMnA, kMnB);
         for (int kb = 0; kb < g.blocks && ok; ++kb) {
           const bool opens = kTerms == 3 || kb == 0;
           if (opens && !wait(&s.tmem_empty[buf], acc_phase ^ 1u)) {
@@ -514,24 +525,44 @@ __global__ void __launch_bounds__(kThreads, 1) expert_gemm_kernel(
     for (int t = unit; t < total && ok && !*failed; t += units) {
       const Tile g = tile_at<kMode>(p, t, s.prefix, n_tiles);
       const int half = g.n_mma >> 1;
-      const int row0 = g.m0 + static_cast<int>(rank) * kRowsCta + quarter * 32;  // of the warp
+      const bool folded = g.m_mma < kTileM;
+      const int side = quarter >> 1;  // folded: the half of the columns in these lanes
+      const int row0 = g.m0 + static_cast<int>(rank) * (g.m_mma >> 1) +
+                       (folded ? quarter & 1 : quarter) * 32;  // of the warp
       const int rows = max(0, min(32, g.m_end - row0));
-      // Group q of 32 accumulator columns of this warp: kGated has gate
-      // columns in groups 0-1 and the up columns they meet in 2-3.
+      // This warp's groups of 32 accumulator columns, q = 0 .. groups - 1: TMEM
+      // column, first output column, and output columns left from there on
+      // (none: the group is skipped; warp-uniform). In kGated a group's up
+      // columns lie 64 TMEM columns after its gate columns.
+      const int groups = (kMode == kGated ? 2 : 4) >> (folded ? 1 : 0);
       auto group_col = [&](int q) {
-        if constexpr (kMode == kGated) return (q < 2 ? 0 : half) + hw * 64 + 32 * (q & 1);
-        else if constexpr (kMode == kDw) return hw * half + 32 * q;
-        else return hw * 128 + 32 * q;
+        if constexpr (kMode == kGated) return folded ? 32 * hw : hw * half + 32 * q;
+        else if constexpr (kMode == kDw) return folded ? hw * 64 + 32 * q : hw * half + 32 * q;
+        else return folded ? hw * 64 + 32 * q : hw * 128 + 32 * q;
       };
-      auto group_live = [&](int q) {  // warp-uniform
-        if constexpr (kMode == kGated) return hw * 64 + 32 * (q & 1) < half;
-        else if constexpr (kMode == kDw) return 32 * q < half;
-        else return hw * 128 + 32 * q < g.n_mma;
+      auto group_out = [&](int q) {
+        if constexpr (kMode == kGated) {
+          return folded ? side * g.own + 32 * hw : hw * g.own + 32 * q;
+        } else if constexpr (kMode == kDw) {
+          return folded ? hw * 64 + 32 * q : 32 * q;
+        } else {
+          return folded ? side * half + hw * 64 + 32 * q : hw * 128 + 32 * q;
+        }
+      };
+      auto group_left = [&](int q) {
+        const int out = group_out(q);
+        if constexpr (kMode == kGated) {
+          return min(g.ncols, ((folded ? side : hw) + 1) * g.own) - out;
+        } else if constexpr (kMode == kDw) {
+          return g.ncols - out;
+        } else {
+          return min(g.ncols, folded ? (side + 1) * half : g.ncols) - out;
+        }
       };
       // Stores group q: v, in kGated with its up columns v2.
       auto put = [&](int q, const float* v, const float* v2) {
-        const int c = (kMode == kGated ? hw * 64 : (kMode == kDw ? 0 : hw * 128)) + 32 * q;
-        const int cols = g.ncols - c;
+        const int c = group_out(q);
+        const int cols = group_left(q);
         if (rows == 0 || cols <= 0) return;  // warp-uniform
         if constexpr (kMode == kGated) {
           float h[32];
@@ -547,7 +578,7 @@ __global__ void __launch_bounds__(kThreads, 1) expert_gemm_kernel(
                                 p.vec_gate_up != 0);
           }
         } else if constexpr (kMode == kDw) {
-          T* out = static_cast<T*>(hw == 0 ? p.out0 : p.out1) +
+          T* out = static_cast<T*>((folded ? side : hw) == 0 ? p.out0 : p.out1) +
                    (static_cast<long long>(g.expert) * p.hidden + row0) * p.output + g.c0 + c;
           store_rows32<T>(staging, v, out, p.output, rows, cols, p.vec != 0);
         } else {
@@ -569,10 +600,9 @@ __global__ void __launch_bounds__(kThreads, 1) expert_gemm_kernel(
           }
         }
       };
-      auto load = [&](int q, float* v) {
+      auto load = [&](int col, float* v) {
         uint32_t r[32];
-        tmem_ld_32x32b_x32(
-            tmem + static_cast<uint32_t>(buf * kTileN + group_col(q)) + lane_addr, r);
+        tmem_ld_32x32b_x32(tmem + static_cast<uint32_t>(buf * kTileN + col) + lane_addr, r);
         tmem_ld_wait();
 #pragma unroll
         for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
@@ -593,20 +623,20 @@ __global__ void __launch_bounds__(kThreads, 1) expert_gemm_kernel(
         if (g.blocks == 0) {  // no rows: a zero gradient
           const float zero[32] = {};
 #pragma unroll 1
-          for (int q = 0; q < 4; ++q) put(q, zero, zero);
+          for (int q = 0; q < groups; ++q) put(q, zero, zero);
           continue;
         }
       }
       if constexpr (kTerms == 1) {
         if (!take()) break;
 #pragma unroll 1
-        for (int q = 0; q < (kMode == kGated ? 2 : 4); ++q) {
-          if (!group_live(q)) break;
+        for (int q = 0; q < groups; ++q) {
+          if (group_left(q) <= 0) break;
           float v[32];
-          load(q, v);
+          load(group_col(q), v);
           if constexpr (kMode == kGated) {
             float v2[32];
-            load(q + 2, v2);
+            load(group_col(q) + 64, v2);
             put(q, v, v2);
           } else {
             put(q, v, v);
@@ -623,17 +653,15 @@ __global__ void __launch_bounds__(kThreads, 1) expert_gemm_kernel(
             break;
           }
 #pragma unroll
-          for (int q = 0; q < 8; ++q) {
-            if (group_live(q >> 1)) {
+          for (int j = 0; j < 8; ++j) {  // 16 columns; kGated: 0-3 gate, 4-7 up
+            const int q = kMode == kGated ? (j >> 1) & 1 : j >> 1;
+            if (q < groups && group_left(q) > 0) {
               uint32_t r[16];
-              tmem_ld_32x32b_x16(tmem +
-                                     static_cast<uint32_t>(buf * kTileN + group_col(q >> 1) +
-                                                           16 * (q & 1)) +
-                                     lane_addr,
-                                 r);
+              const int col = group_col(q) + 16 * (j & 1) + (kMode == kGated ? 64 * (j >> 2) : 0);
+              tmem_ld_32x32b_x16(tmem + static_cast<uint32_t>(buf * kTileN + col) + lane_addr, r);
               tmem_ld_wait();
 #pragma unroll
-              for (int i = 0; i < 16; ++i) sum[16 * q + i] += __uint_as_float(r[i]);
+              for (int i = 0; i < 16; ++i) sum[16 * j + i] += __uint_as_float(r[i]);
             }
           }
           release();
@@ -641,7 +669,7 @@ __global__ void __launch_bounds__(kThreads, 1) expert_gemm_kernel(
         if (!ok) break;
 #pragma unroll
         for (int q = 0; q < (kMode == kGated ? 2 : 4); ++q) {
-          put(q, sum + 32 * q, sum + (32 * q + (kMode == kGated ? 64 : 0)));
+          if (q < groups) put(q, sum + 32 * q, sum + (32 * q + (kMode == kGated ? 64 : 0)));
         }
       }
     }
