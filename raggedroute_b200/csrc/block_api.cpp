@@ -111,11 +111,22 @@ bool gated_few(int rows, int experts, Dtype dtype) {
   return dtype == Dtype::kBf16 ? rows <= 32 : rows <= 2 * experts + 32;
 }
 
+// Parts of dg and du in a bfloat16 backward pass. One rounding to bfloat16 is
+// what any tensor-core operand takes, and over many rows its errors average out
+// against the result's own. With few rows per expert an element of a weight
+// gradient is a sum of few products and carries the rounding whole, and the
+// products are bound by the weights' bytes: there a second part (16 significand
+// bits) doubles tensor work that is hidden behind them.
+int gradient_parts(int rows, int experts, Dtype dtype) {
+  if (dtype == Dtype::kFp32) return 3;
+  return rows <= 64LL * experts ? 2 : 1;
+}
+
 // Where the operands of one call lie in the workspace; an offset of 0 bytes
 // with packed == false means that the caller's buffer is used as it is.
 struct GatedPlan {
   bool pack_x = false, pack_w = false;
-  int terms = 1, ldk = 0, ldn = 0;
+  int terms = 1, parts = 1, ldk = 0, ldn = 0;
   std::size_t x = 0, wg = 0, wu = 0, dg = 0, du = 0, total = 0;
 };
 
@@ -127,17 +138,18 @@ GatedPlan gated_plan(int rows, int experts, int hidden, int output, Dtype dtype,
   if (rows <= 0 || (!backward && gated_few(rows, experts, dtype))) return p;
   p.pack_x = p.terms == 3 || hidden % 8 != 0;
   p.pack_w = p.terms == 3 || output % 8 != 0;
-  auto take = [&p](bool used, std::size_t elements) {
+  p.parts = gradient_parts(rows, experts, dtype);
+  auto take = [&p](bool used, std::size_t elements, int parts) {
     const std::size_t at = p.total;
-    if (used) p.total += up256(2 * elements * p.terms);
+    if (used) p.total += up256(2 * elements * parts);
     return at;
   };
   const std::size_t r = rows, w = static_cast<std::size_t>(experts) * hidden * p.ldn;
-  p.x = take(p.pack_x, r * p.ldk);
-  p.wg = take(p.pack_w, w);
-  p.wu = take(p.pack_w, w);
-  p.dg = take(backward, r * p.ldn);
-  p.du = take(backward, r * p.ldn);
+  p.x = take(p.pack_x, r * p.ldk, p.terms);
+  p.wg = take(p.pack_w, w, p.terms);
+  p.wu = take(p.pack_w, w, p.terms);
+  p.dg = take(backward, r * p.ldn, p.parts);
+  p.du = take(backward, r * p.ldn, p.parts);
   return p;
 }
 
@@ -159,23 +171,20 @@ cudaError_t gated_operands(const GatedPlan& plan, const void* x, const void* wg,
   out->terms = plan.terms;
   out->ldk = plan.ldk;
   out->ldn = plan.ldn;
-  auto place = [&](bool pack, const void* src, std::size_t at, long long r, int cols, int ld,
-                   const __nv_bfloat16** dst) {
-    if (!pack) {
-      *dst = static_cast<const __nv_bfloat16*>(src);
-      return cudaSuccess;
-    }
+  rrb::PackJobs jobs;
+  auto place = [&](bool pack, const void* src, std::size_t at, long long r, int cols, int ld) {
+    if (!pack) return static_cast<const __nv_bfloat16*>(src);
     auto* to = reinterpret_cast<__nv_bfloat16*>(ws + at);
-    *dst = to;
-    return rrb::launch_pack_terms(src, to, r, cols, ld, dtype, stream);
+    jobs.job[jobs.count++] = {src, to, r, cols, ld};
+    return static_cast<const __nv_bfloat16*>(to);
   };
-  cudaError_t e = place(plan.pack_x, x, plan.x, rows, hidden, plan.ldk, &out->x);
+  out->x = place(plan.pack_x, x, plan.x, rows, hidden, plan.ldk);
   const long long wrows = static_cast<long long>(experts) * hidden;
-  if (e == cudaSuccess && need_w) {
-    e = place(plan.pack_w, wg, plan.wg, wrows, output, plan.ldn, &out->wg);
-    if (e == cudaSuccess) e = place(plan.pack_w, wu, plan.wu, wrows, output, plan.ldn, &out->wu);
+  if (need_w) {
+    out->wg = place(plan.pack_w, wg, plan.wg, wrows, output, plan.ldn);
+    out->wu = place(plan.pack_w, wu, plan.wu, wrows, output, plan.ldn);
   }
-  return e;
+  return jobs.count > 0 ? rrb::launch_pack_terms(jobs, dtype, stream) : cudaSuccess;
 }
 
 }  // namespace
@@ -311,7 +320,7 @@ rr_status rr_grouped_gated_gemm_backward(const void* x_permuted, const void* gat
   auto* du = reinterpret_cast<__nv_bfloat16*>(ws + plan.du);
   cudaStream_t stream = stream_of(ctx);
   cudaError_t e = rrb::launch_gated_pointwise_backward(gate_up, dh, dg, du, route_pairs, output,
-                                                       plan.ldn,
+                                                       plan.ldn, plan.parts,
                                                        static_cast<Activation>(activation), t,
                                                        stream);
   rrb::GatedOperands in;
@@ -322,11 +331,11 @@ rr_status rr_grouped_gated_gemm_backward(const void* x_permuted, const void* gat
                        hidden, output, t, need_w, stream, &in);
   }
   if (e == cudaSuccess && need_w) {
-    e = rrb::launch_gated_dx(in, dg, du, offsets, dx, route_pairs, experts, hidden, output, t,
+    e = rrb::launch_gated_dx(in, dg, du, plan.parts, offsets, dx, route_pairs, experts, hidden, output, t,
                              stream);
   }
   if (e == cudaSuccess && need_dw) {
-    e = rrb::launch_gated_dw(in, dg, du, offsets, d_gate_weights, d_up_weights, route_pairs,
+    e = rrb::launch_gated_dw(in, dg, du, plan.parts, offsets, d_gate_weights, d_up_weights, route_pairs,
                              experts, hidden, output, t, stream);
   }
   return launched(e, what);

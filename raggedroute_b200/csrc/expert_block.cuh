@@ -117,15 +117,16 @@ struct GatedOperands {
 cudaError_t launch_gated_gemm(const GatedOperands& in, const int32_t* offsets, void* h,
                               float* gate_up, int rows, int experts, int hidden, int output,
                               Activation activation, Dtype dtype, cudaStream_t stream);
-// dx[r] = dg[r] Wg[e]^T + du[r] Wu[e]^T; dg, du are [terms][rows][ldn].
+// dx[r] = dg[r] Wg[e]^T + du[r] Wu[e]^T; dg, du are [parts][rows][ldn] (parts =
+// terms, or 2 for bfloat16).
 cudaError_t launch_gated_dx(const GatedOperands& in, const __nv_bfloat16* dg,
-                            const __nv_bfloat16* du, const int32_t* offsets, void* dx, int rows,
-                            int experts, int hidden, int output, Dtype dtype,
+                            const __nv_bfloat16* du, int parts, const int32_t* offsets, void* dx,
+                            int rows, int experts, int hidden, int output, Dtype dtype,
                             cudaStream_t stream);
 // dwg[e] = x_e^T dg_e, dwu[e] = x_e^T du_e; zero for an empty segment.
 cudaError_t launch_gated_dw(const GatedOperands& in, const __nv_bfloat16* dg,
-                            const __nv_bfloat16* du, const int32_t* offsets, void* dwg, void* dwu,
-                            int rows, int experts, int hidden, int output, Dtype dtype,
+                            const __nv_bfloat16* du, int parts, const int32_t* offsets, void* dwg,
+                            void* dwu, int rows, int experts, int hidden, int output, Dtype dtype,
                             cudaStream_t stream);
 // y[r, n] = (xq[r] . wq[e][n]) * x_scale[r] * w_scale[e][n]; xq [rows][ld],
 // wq [experts][output][ld], ld a multiple of 16.
@@ -140,14 +141,25 @@ cudaError_t launch_gated_few(const void* x, const void* wg, const void* wu,
                              const int32_t* offsets, void* h, float* gate_up, int rows,
                              int experts, int hidden, int output, Activation activation,
                              Dtype dtype, cudaStream_t stream);
-// src [rows][cols] -> dst [terms][rows][ld] bfloat16 (columns past cols zero).
-cudaError_t launch_pack_terms(const void* src, __nv_bfloat16* dst, long long rows, int cols,
-                              int ld, Dtype dtype, cudaStream_t stream);
+// src [rows][cols] -> dst [terms][rows][ld] bfloat16 (columns past cols zero),
+// for up to three tensors in one launch.
+struct PackJob {
+  const void* src = nullptr;
+  __nv_bfloat16* dst = nullptr;
+  long long rows = 0;
+  int cols = 0;
+  int ld = 0;
+};
+struct PackJobs {
+  PackJob job[3];
+  int count = 0;
+};
+cudaError_t launch_pack_terms(const PackJobs& jobs, Dtype dtype, cudaStream_t stream);
 // dg = dh u act'(g), du = dh act(g) from gate_up [rows][2 output], written as
-// [terms][rows][ld] bfloat16 parts.
+// [parts][rows][ld] bfloat16 parts.
 cudaError_t launch_gated_pointwise_backward(const float* gate_up, const void* dh,
                                             __nv_bfloat16* dg, __nv_bfloat16* du, int rows,
-                                            int output, int ld, Activation activation,
+                                            int output, int ld, int parts, Activation activation,
                                             Dtype dtype, cudaStream_t stream);
 
 // ---- int8.cu -------------------------------------------------------------------

@@ -87,6 +87,7 @@ struct EngineArgs {
   int hidden;   // contraction of kGated and kInt8; output columns of kDx, rows of kDw's tiles
   int output;   // output columns of kGated, kDw, kInt8; contraction (twice) of kDx
   int activation;
+  int parts;        // of dg and du where kTerms == 1: 2 sums the low part first
   int vec;          // 16-byte stores of out0 / out1 allowed
   int vec_gate_up;  // and of gate_up
 };
@@ -207,11 +208,11 @@ __device__ __forceinline__ Tile tile_at(const EngineArgs& p, int t, const int* p
   if constexpr (kMode == kDw) {
     g.m0 = mt * kTileM;
     g.m_end = p.hidden;
-    g.blocks = (s.y - s.x + 63) >> 6;
+    g.blocks = p.parts * ((s.y - s.x + 63) >> 6);
   } else {
     g.m0 = s.x + mt * kTileM;
     g.m_end = s.y;
-    if constexpr (kMode == kDx) g.blocks = 2 * ((p.output + 63) >> 6);
+    if constexpr (kMode == kDx) g.blocks = 2 * p.parts * ((p.output + 63) >> 6);
     else if constexpr (kMode == kInt8) g.blocks = (p.hidden + 127) >> 7;
     else g.blocks = (p.hidden + 63) >> 6;
   }
@@ -352,7 +353,15 @@ __global__ void __launch_bounds__(kThreads, 1) expert_gemm_kernel(
         const Tile g = tile_at<kMode>(p, t, s.prefix, n_tiles);
         const int m = g.m0 + static_cast<int>(rank) * (g.m_mma >> 1);
         const int half = g.n_mma >> 1;
-        for (int kb = 0; kb < g.blocks; ++kb) {
+        // k-blocks of one part: kDx and kDw pass over the contraction once per
+        // part of dg and du (kb runs within it; plane counts down to the top part).
+        const int pass = g.blocks / p.parts;
+        int kb = 0, plane = p.parts - 1;
+        for (int i = 0; i < g.blocks; ++i, ++kb) {
+          if (kb == pass) {
+            kb = 0;
+            --plane;
+          }
           if (!wait(&s.empty[stage], phase ^ 1u)) break;
           if (elect_one()) {
           uint8_t* a = s.stage[stage];
@@ -379,10 +388,10 @@ __global__ void __launch_bounds__(kThreads, 1) expert_gemm_kernel(
               tma_load_3d_pair(b, &map_b0, bar, c, kb * 64, z);
               tma_load_3d_pair(b + kBoxBytes, &map_b1, bar, c, kb * 64, z);
             } else if constexpr (kMode == kDx) {
-              const int per = g.blocks >> 1;
+              const int per = pass >> 1;
               const bool first = kb < per;
               const int k = (first ? kb : kb - per) * 64;
-              tma_load_3d_pair(a, first ? &map_a0 : &map_a1, bar, k, m, q);
+              tma_load_3d_pair(a, first ? &map_a0 : &map_a1, bar, k, m, kTerms == 1 ? plane : q);
               tma_load_3d_pair(b, first ? &map_b0 : &map_b1, bar, k,
                                g.c0 + static_cast<int>(rank) * half, q * p.experts + g.expert);
             } else if constexpr (kMode == kDw) {
@@ -390,8 +399,9 @@ __global__ void __launch_bounds__(kThreads, 1) expert_gemm_kernel(
               const int r = g.row0 + kb * 64;
               tma_load_3d_pair(a, &map_a0, bar, m, r, q);
               tma_load_3d_pair(a + kBoxBytes, &map_a0, bar, m + 64, r, q);
-              tma_load_3d_pair(b, mb, bar, g.c0, r, q);
-              tma_load_3d_pair(b + kBoxBytes, mb, bar, g.c0 + 64, r, q);
+              const int z = kTerms == 1 ? plane : q;
+              tma_load_3d_pair(b, mb, bar, g.c0, r, z);
+              tma_load_3d_pair(b + kBoxBytes, mb, bar, g.c0 + 64, r, z);
             } else {
               tma_load_3d_pair(a, &map_a0, bar, kb * 128, m, 0);
               tma_load_3d_pair(b, &map_b0, bar, kb * 128, g.c0 + static_cast<int>(rank) * half,
@@ -493,24 +503,26 @@ __global__ void __launch_bounds__(kThreads, 1) expert_gemm_kernel(
       uint32_t phases = 0;  // per stage, of its tail barrier
       for (int t = unit; t < total && !*failed; t += units) {
         const Tile g = tile_at<kMode>(p, t, s.prefix, n_tiles);
-        at = (at + g.blocks) % kStages;
         const int valid = (g.row_end - g.row0) & 63;
-        if (valid == 0) continue;
-        const int stage = (at + kStages - 1) % kStages;  // of the last block
-        if (!wait(&s.tail[stage], (phases >> stage) & 1u)) break;
-        phases ^= 1u << stage;
-        // Lines past the segment's end hold other segments' rows (or
-        // anything): both operands become zero there. A line is one row of a
-        // box, so the swizzle inside it does not matter.
-        for (int bx = 0; bx < 4 * kTerms; ++bx) {
-          uint8_t* box = s.stage[stage] + bx * kBoxBytes;
-          for (int i = valid * 8 + lane; i < 512; i += 32) {
-            reinterpret_cast<uint4*>(box)[i] = make_uint4(0u, 0u, 0u, 0u);
+        for (int part = 0; part < p.parts && valid != 0; ++part) {
+          // The last block of each pass over the rows.
+          const int stage = (at + (part + 1) * (g.blocks / p.parts) + kStages - 1) % kStages;
+          if (!wait(&s.tail[stage], (phases >> stage) & 1u)) break;
+          phases ^= 1u << stage;
+          // Lines past the segment's end hold other segments' rows (or
+          // anything): both operands become zero there. A line is one row of a
+          // box, so the swizzle inside it does not matter.
+          for (int bx = 0; bx < 4 * kTerms; ++bx) {
+            uint8_t* box = s.stage[stage] + bx * kBoxBytes;
+            for (int i = valid * 8 + lane; i < 512; i += 32) {
+              reinterpret_cast<uint4*>(box)[i] = make_uint4(0u, 0u, 0u, 0u);
+            }
           }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_remote(mapa_shared(smem_u32(&s.ready[stage]), 0u));
         }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive_remote(mapa_shared(smem_u32(&s.ready[stage]), 0u));
+        at = (at + g.blocks) % kStages;
       }
     }
   } else if (warp >= kEpiWarp0) {
@@ -805,6 +817,7 @@ cudaError_t launch_gated_gemm(const GatedOperands& in, const int32_t* offsets, v
   }
   maps[1] = maps[0];
   EngineArgs a{};
+  a.parts = 1;
   a.offsets = offsets;
   a.out0 = h;
   a.gate_up = gate_up;
@@ -821,24 +834,26 @@ cudaError_t launch_gated_gemm(const GatedOperands& in, const int32_t* offsets, v
 }
 
 cudaError_t launch_gated_dx(const GatedOperands& in, const __nv_bfloat16* dg,
-                            const __nv_bfloat16* du, const int32_t* offsets, void* dx, int rows,
-                            int experts, int hidden, int output, Dtype dtype,
+                            const __nv_bfloat16* du, int parts, const int32_t* offsets, void* dx,
+                            int rows, int experts, int hidden, int output, Dtype dtype,
                             cudaStream_t stream) {
   CUtensorMap maps[4] = {};
   const long long planes = static_cast<long long>(in.terms) * experts;
-  if (!encode_map(&maps[0], dg, false, output, rows, in.terms, in.ldn, 64, kRowsCta) ||
-      !encode_map(&maps[1], du, false, output, rows, in.terms, in.ldn, 64, kRowsCta) ||
+  if (!encode_map(&maps[0], dg, false, output, rows, parts, in.ldn, 64, kRowsCta) ||
+      !encode_map(&maps[1], du, false, output, rows, parts, in.ldn, 64, kRowsCta) ||
       !encode_map(&maps[2], in.wg, false, output, hidden, planes, in.ldn, 64, kRowsCta) ||
       !encode_map(&maps[3], in.wu, false, output, hidden, planes, in.ldn, 64, kRowsCta)) {
     return cudaErrorInvalidValue;
   }
   EngineArgs a{};
+  a.parts = 1;
   a.offsets = offsets;
   a.out0 = dx;
   a.experts = experts;
   a.rows = rows;
   a.hidden = hidden;
   a.output = output;
+  if (in.terms == 1) a.parts = parts;
   a.vec = vec_ok(dx, hidden, dtype);
   const long long tiles = row_tiles(rows, experts, hidden, kTileN);
   return dtype == Dtype::kBf16 ? launch_engine<kDx, 1, __nv_bfloat16>(maps, a, tiles, stream)
@@ -846,17 +861,18 @@ cudaError_t launch_gated_dx(const GatedOperands& in, const __nv_bfloat16* dg,
 }
 
 cudaError_t launch_gated_dw(const GatedOperands& in, const __nv_bfloat16* dg,
-                            const __nv_bfloat16* du, const int32_t* offsets, void* dwg, void* dwu,
-                            int rows, int experts, int hidden, int output, Dtype dtype,
+                            const __nv_bfloat16* du, int parts, const int32_t* offsets, void* dwg,
+                            void* dwu, int rows, int experts, int hidden, int output, Dtype dtype,
                             cudaStream_t stream) {
   CUtensorMap maps[4] = {};
   if (!encode_map(&maps[0], in.x, false, hidden, rows, in.terms, in.ldk, 64, 64) ||
-      !encode_map(&maps[2], dg, false, output, rows, in.terms, in.ldn, 64, 64) ||
-      !encode_map(&maps[3], du, false, output, rows, in.terms, in.ldn, 64, 64)) {
+      !encode_map(&maps[2], dg, false, output, rows, parts, in.ldn, 64, 64) ||
+      !encode_map(&maps[3], du, false, output, rows, parts, in.ldn, 64, 64)) {
     return cudaErrorInvalidValue;
   }
   maps[1] = maps[0];
   EngineArgs a{};
+  a.parts = 1;
   a.offsets = offsets;
   a.out0 = dwg;
   a.out1 = dwu;
@@ -864,6 +880,7 @@ cudaError_t launch_gated_dw(const GatedOperands& in, const __nv_bfloat16* dg,
   a.rows = rows;
   a.hidden = hidden;
   a.output = output;
+  if (in.terms == 1) a.parts = parts;
   a.vec = vec_ok(dwg, output, dtype) && vec_ok(dwu, output, dtype);
   const long long tiles = static_cast<long long>(experts) * ceil_div(hidden, kTileM) *
                           ceil_div(output, kTileN / 2);
@@ -882,6 +899,7 @@ cudaError_t launch_int8_gemm(const int8_t* xq, const float* x_scale, const int8_
   maps[1] = maps[0];
   maps[3] = maps[2];
   EngineArgs a{};
+  a.parts = 1;
   a.offsets = offsets;
   a.out0 = y;
   a.row_scale = x_scale;

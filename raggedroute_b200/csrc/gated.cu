@@ -1,6 +1,8 @@
 // The parts of the gated expert projection around the tensor-core engine
 // (expert_gemm.cu): the form for a few rows, the packing of operands the
 // engine cannot read as they are, and the pointwise half of the gradient.
+#include <climits>
+
 #include "expert_block.cuh"
 #include "sm100.cuh"
 
@@ -11,8 +13,8 @@ namespace {
 //
 // h[r, c] = act(sum_k x[r, k] Wg[e][k, c]) * sum_k x[r, k] Wu[e][k, c] for a
 // handful of rows: bound by reading the weights of the experts that have
-// rows, 2 K N elements each, once. A cluster takes 32 columns of up to kFewRows
-// rows of one expert, 16 bytes of each matrix per thread and k-step, with the
+// rows, 2 K N elements each, once. A cluster takes 128 bytes of columns of up to
+// kFewRows rows of one expert, 16 bytes of each matrix per thread and k-step, with the
 // contraction spread over its blocks and their threads; the partial sums
 // (FP32) meet by shuffles, in shared memory and in the first block of the
 // cluster, in a fixed order. The cluster grows (to 8 blocks) until every SM has
@@ -21,13 +23,15 @@ namespace {
 
 constexpr int kFewThreads = 256;
 constexpr int kFewWarps = kFewThreads / 32;
-constexpr int kFewCols = 32;
+constexpr int kFewMaxCols = 64;
+template <typename T>
+constexpr int kFewCols = 128 / static_cast<int>(sizeof(T));  // a line of the weights
 constexpr int kFewRows = 4;
 constexpr int kMaxSplit = 8;
 
 struct FewSmem {
-  float warps[kFewWarps][kFewRows][2][kFewCols];      // gate and up sums of each warp
-  float parts[kMaxSplit - 1][kFewRows][2][kFewCols];  // and of the cluster's other blocks
+  float warps[kFewWarps][kFewRows][2][kFewMaxCols];      // gate and up sums of each warp
+  float parts[kMaxSplit - 1][kFewRows][2][kFewMaxCols];  // and of the cluster's other blocks
 };
 
 __device__ __forceinline__ uint4 ld_stream16(const void* p) {
@@ -58,12 +62,18 @@ __device__ __forceinline__ void few_rows(const T* __restrict__ x, const T* __res
                                          float* __restrict__ gate_up, int row, int nrows,
                                          int hidden, int output, int c0, int activation,
                                          int split, FewSmem& s) {
-  constexpr int kLanes = kFewCols / kVec;       // lanes across the columns
+  constexpr int kCols = kFewCols<T>;
+  constexpr int kLanes = kCols / kVec;           // threads across the columns
   constexpr int kGroups = kFewThreads / kLanes;  // contraction groups of a block
   constexpr int kUnroll = 4;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  // Partial sums that meet in shared memory: one per warp, or (a scalar row of
+  // 64 bfloat16 takes two warps) one per pair of warps.
+  constexpr int kWide = kLanes > 32 ? kLanes / 32 : 1;
+  constexpr int kSums = kFewWarps / kWide;
+  const int sum_row = warp / kWide;
   const int part = static_cast<int>(sm100::cluster_ctarank());
   const int stride = split * kGroups;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int col = (threadIdx.x % kLanes) * kVec;
   const int kg = threadIdx.x / kLanes;
   float g[kR][kVec], u[kR][kVec];
@@ -120,22 +130,22 @@ __device__ __forceinline__ void few_rows(const T* __restrict__ x, const T* __res
 #pragma unroll
     for (int j = 0; j < kVec; ++j) {
 #pragma unroll
-      for (int d = kLanes; d < 32; d <<= 1) {
+      for (int d = kLanes; d < 32; d <<= 1) {  // (none where a row takes a warp or more)
         g[i][j] += __shfl_xor_sync(0xffffffffu, g[i][j], d);
         u[i][j] += __shfl_xor_sync(0xffffffffu, u[i][j], d);
       }
       if (lane < kLanes) {
-        s.warps[warp][i][0][col + j] = g[i][j];
-        s.warps[warp][i][1][col + j] = u[i][j];
+        s.warps[sum_row][i][0][col + j] = g[i][j];
+        s.warps[sum_row][i][1][col + j] = u[i][j];
       }
     }
   }
   __syncthreads();
-  const int i = threadIdx.x / kFewCols, c = threadIdx.x % kFewCols;
+  const int i = threadIdx.x / kCols, c = threadIdx.x % kCols;
   float sg = 0.0f, su = 0.0f;
   if (i < kR) {
 #pragma unroll
-    for (int w = 0; w < kFewWarps; ++w) {
+    for (int w = 0; w < kSums; ++w) {
       sg += s.warps[w][i][0][c];
       su += s.warps[w][i][1][c];
     }
@@ -144,7 +154,7 @@ __device__ __forceinline__ void few_rows(const T* __restrict__ x, const T* __res
     if (part > 0 && i < kR) {
       const uint32_t to = sm100::mapa_shared(sm100::smem_u32(&s.parts[part - 1][i][0][c]), 0u);
       sm100::st_shared_cluster_u32(to, __float_as_uint(sg));
-      sm100::st_shared_cluster_u32(to + kFewCols * 4, __float_as_uint(su));
+      sm100::st_shared_cluster_u32(to + kFewMaxCols * 4, __float_as_uint(su));
     }
     sm100::cluster_sync();
     if (part > 0) return;
@@ -189,7 +199,7 @@ __global__ void __launch_bounds__(kFewThreads, kR == 1 ? 4 : 2) gated_few_kernel
   if ((row - s.x) % kR != 0) return;  // an earlier block's row
   const long long at = static_cast<long long>(e) * hidden * output;
   few_rows<T, kVec, kR>(x, wg + at, wu + at, h, gate_up, row, min(kR, s.y - row), hidden, output,
-                        blockIdx.x / split * kFewCols, activation, split, smem);
+                        blockIdx.x / split * kFewCols<T>, activation, split, smem);
 }
 
 template <typename T>
@@ -198,12 +208,12 @@ cudaError_t few(const void* x, const void* wg, const void* wu, const int32_t* of
                 cudaStream_t stream) {
   constexpr int kVec = 16 / sizeof(T);
   const bool vec = output % kVec == 0 && aligned_to(wg, 16) && aligned_to(wu, 16);
-  const int groups = ceil_div(output, kFewCols);
+  const int groups = ceil_div(output, kFewCols<T>);
   // One token's routes go to different experts, so up to two rows are taken
   // one at a time; more may share an expert.
   const bool single = rows <= 2;
   // Contraction steps of a thread without a split; a split leaves four.
-  const int steps = hidden / (kFewThreads / (kFewCols / (vec ? kVec : 1)));
+  const int steps = hidden / (kFewThreads / (kFewCols<T> / (vec ? kVec : 1)));
   int split = 1;
   while (split < kMaxSplit &&
          static_cast<long long>(groups) * rows * split < (single ? 4 : 2) * kNumSms &&
@@ -257,12 +267,24 @@ __device__ __forceinline__ void split3(float v, uint16_t (&part)[3]) {
   }
 }
 
-// Eight values as one 16-byte store per part; planes `plane` elements apart.
+// Eight values as one 16-byte store per part; planes `plane` elements apart. One
+// part: rounded to nearest. Two: what the first leaves, rounded again (16
+// significand bits). Three: the exact FP32 value.
 template <int kTerms>
 __device__ __forceinline__ void store_parts(__nv_bfloat16* dst, long long plane,
                                             const float (&v)[8]) {
   if constexpr (kTerms == 1) {
     *reinterpret_cast<uint4*>(dst) = pack16<__nv_bfloat16>(v);
+  } else if constexpr (kTerms == 2) {
+    float hi[8], lo[8];
+    const uint4 top = pack16<__nv_bfloat16>(v);
+    unpack16<__nv_bfloat16>(top, hi);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      lo[i] = isfinite(hi[i]) ? v[i] - hi[i] : 0.0f;
+    }
+    *reinterpret_cast<uint4*>(dst) = top;
+    *reinterpret_cast<uint4*>(dst + plane) = pack16<__nv_bfloat16>(lo);
   } else {
     uint32_t w[3][4];
 #pragma unroll
@@ -283,32 +305,40 @@ __device__ __forceinline__ void store_parts(__nv_bfloat16* dst, long long plane,
 constexpr int kPackThreads = 256;
 
 // One thread packs eight columns: bound by the bytes (FP32: 4 read, 6 written
-// per element). Runs only for FP32 operands and for row strides that are no
-// multiple of 16 bytes, which TMA cannot read.
-template <typename T, int kTerms, bool kVec>
-__global__ void __launch_bounds__(kPackThreads) pack_terms_kernel(
-    const T* __restrict__ src, __nv_bfloat16* __restrict__ dst, long long rows, int cols,
-    int ld) {
-  const int groups = ld >> 3;
-  const long long total = rows * groups;
-  const long long plane = rows * ld;
-  for (long long i = static_cast<long long>(blockIdx.x) * kPackThreads + threadIdx.x; i < total;
-       i += static_cast<long long>(gridDim.x) * kPackThreads) {
-    const long long r = i / groups;
-    const int c = static_cast<int>(i - r * groups) << 3;
-    const T* p = src + r * cols + c;
-    float v[8];
-    if (kVec && c + 8 <= cols) {
-      constexpr int kPer = 16 / sizeof(T);
+// per element; 6.2 TB/s at 64 x 1024 x 1024). Runs only for FP32 operands and
+// for row strides that are no multiple of 16 bytes, which TMA cannot read.
+// The operands of a call are packed by one launch.
+template <typename T, int kTerms>
+__global__ void __launch_bounds__(kPackThreads) pack_terms_kernel(const PackJobs jobs) {
+  long long first = static_cast<long long>(blockIdx.x) * kPackThreads + threadIdx.x;
+  const long long step = static_cast<long long>(gridDim.x) * kPackThreads;
+  for (int q = 0; q < jobs.count; ++q) {
+    const PackJob& job = jobs.job[q];
+    const int groups = job.ld >> 3;
+    const long long total = job.rows * groups;
+    const long long plane = job.rows * job.ld;
+    const bool vec = (job.cols * sizeof(T)) % 16 == 0;  // such rows are 16-byte aligned
+    for (long long i = first; i < total; i += step) {
+      const long long r =
+          total <= INT_MAX ? static_cast<int>(i) / groups : i / groups;  // 32 bits where they do
+      const int c = static_cast<int>(i - r * groups) << 3;
+      const T* p = static_cast<const T*>(job.src) + r * job.cols + c;
+      float v[8];
+      if (vec && c + 8 <= job.cols) {
+        constexpr int kPer = 16 / sizeof(T);
 #pragma unroll
-      for (int j = 0; j < 8 / kPer; ++j) {
-        unpack16<T>(__ldg(reinterpret_cast<const uint4*>(p) + j), v + j * kPer);
+        for (int j = 0; j < 8 / kPer; ++j) {
+          unpack16<T>(__ldg(reinterpret_cast<const uint4*>(p) + j), v + j * kPer);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = c + j < job.cols ? to_f32(__ldg(p + j)) : 0.0f;
       }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = c + j < cols ? to_f32(__ldg(p + j)) : 0.0f;
+      store_parts<kTerms>(job.dst + r * job.ld + c, plane, v);
     }
-    store_parts<kTerms>(dst + r * ld + c, plane, v);
+    // The next job goes on where this one left the grid.
+    first = (first - total) % step;
+    if (first < 0) first += step;
   }
 }
 
@@ -316,8 +346,9 @@ __global__ void __launch_bounds__(kPackThreads) pack_terms_kernel(
 //
 // From the saved FP32 products g, u and the incoming dh:
 //   dg = dh * u * act'(g), du = dh * act(g).
-// Rounded once to the engine's operand parts (bfloat16: the rounding every
-// tensor-core operand takes; FP32: three exact parts). Bound by its bytes.
+// Written as the engine's operand parts: for bfloat16 one rounding, which every
+// tensor-core operand takes, or two parts (see gradient_parts in block_api.cpp);
+// for FP32 three exact parts. Bound by its bytes.
 template <typename T, int kTerms, bool kVec>
 __global__ void __launch_bounds__(kPackThreads) gated_pointwise_backward_kernel(
     const float* __restrict__ gate_up, const T* __restrict__ dh, __nv_bfloat16* __restrict__ dg,
@@ -327,7 +358,7 @@ __global__ void __launch_bounds__(kPackThreads) gated_pointwise_backward_kernel(
   const long long plane = static_cast<long long>(rows) * ld;
   for (long long i = static_cast<long long>(blockIdx.x) * kPackThreads + threadIdx.x; i < total;
        i += static_cast<long long>(gridDim.x) * kPackThreads) {
-    const long long r = i / groups;
+    const long long r = total <= INT_MAX ? static_cast<int>(i) / groups : i / groups;
     const int c = static_cast<int>(i - r * groups) << 3;
     const float* pg = gate_up + 2 * r * output + c;
     const float* pu = pg + output;
@@ -384,20 +415,15 @@ cudaError_t launch_gated_few(const void* x, const void* wg, const void* wu,
                                             output, act, stream);
 }
 
-cudaError_t launch_pack_terms(const void* src, __nv_bfloat16* dst, long long rows, int cols,
-                              int ld, Dtype dtype, cudaStream_t stream) {
-  const int blocks = pack_blocks(rows * (ld >> 3));
+cudaError_t launch_pack_terms(const PackJobs& jobs, Dtype dtype, cudaStream_t stream) {
+  long long total = 0;
+  for (int q = 0; q < jobs.count; ++q) total += jobs.job[q].rows * (jobs.job[q].ld >> 3);
+  const int blocks = pack_blocks(total);
   if (blocks == 0) return cudaSuccess;
-  const bool vec = aligned_to(src, 16) && (cols * dtype_bytes(dtype)) % 16 == 0;
   if (dtype == Dtype::kBf16) {
-    auto* kernel = vec ? pack_terms_kernel<__nv_bfloat16, 1, true>
-                       : pack_terms_kernel<__nv_bfloat16, 1, false>;
-    kernel<<<blocks, kPackThreads, 0, stream>>>(static_cast<const __nv_bfloat16*>(src), dst, rows,
-                                                cols, ld);
+    pack_terms_kernel<__nv_bfloat16, 1><<<blocks, kPackThreads, 0, stream>>>(jobs);
   } else {
-    auto* kernel = vec ? pack_terms_kernel<float, 3, true> : pack_terms_kernel<float, 3, false>;
-    kernel<<<blocks, kPackThreads, 0, stream>>>(static_cast<const float*>(src), dst, rows, cols,
-                                                ld);
+    pack_terms_kernel<float, 3><<<blocks, kPackThreads, 0, stream>>>(jobs);
   }
   note_launch();
   return cudaGetLastError();
@@ -405,15 +431,18 @@ cudaError_t launch_pack_terms(const void* src, __nv_bfloat16* dst, long long row
 
 cudaError_t launch_gated_pointwise_backward(const float* gate_up, const void* dh,
                                             __nv_bfloat16* dg, __nv_bfloat16* du, int rows,
-                                            int output, int ld, Activation activation,
+                                            int output, int ld, int parts, Activation activation,
                                             Dtype dtype, cudaStream_t stream) {
   const int blocks = pack_blocks(static_cast<long long>(rows) * (ld >> 3));
   if (blocks == 0) return cudaSuccess;
   const int act = static_cast<int>(activation);
   const bool vec = output % 8 == 0 && aligned_to(gate_up, 16) && aligned_to(dh, 16);
   if (dtype == Dtype::kBf16) {
-    auto* kernel = vec ? gated_pointwise_backward_kernel<__nv_bfloat16, 1, true>
-                       : gated_pointwise_backward_kernel<__nv_bfloat16, 1, false>;
+    auto* kernel = parts == 2
+                       ? (vec ? gated_pointwise_backward_kernel<__nv_bfloat16, 2, true>
+                              : gated_pointwise_backward_kernel<__nv_bfloat16, 2, false>)
+                       : (vec ? gated_pointwise_backward_kernel<__nv_bfloat16, 1, true>
+                              : gated_pointwise_backward_kernel<__nv_bfloat16, 1, false>);
     kernel<<<blocks, kPackThreads, 0, stream>>>(gate_up, static_cast<const __nv_bfloat16*>(dh), dg,
                                                 du, rows, output, ld, act);
   } else {
