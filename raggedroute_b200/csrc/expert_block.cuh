@@ -62,18 +62,23 @@ __device__ __forceinline__ uint4 pack16(const float* f) {
   }
 }
 
-// Logistic function in full float precision; exp(-g) = inf gives 0.
+// Logistic function; exp(-g) = inf gives 0. For FP32 results in full float
+// precision; a result that is rounded to bfloat16 takes the hardware's exp and
+// division (2^-21 relative).
+template <typename T>
 __device__ __forceinline__ float sigmoid_f32(float g) {
-  return __fdiv_rn(1.0f, 1.0f + expf(-g));
+  if constexpr (sizeof(T) == 2) return __fdividef(1.0f, 1.0f + __expf(-g));
+  else return __fdiv_rn(1.0f, 1.0f + expf(-g));
 }
 
 constexpr float kGeluC = 0.7978845608028654f;  // sqrt(2 / pi)
 constexpr float kGeluA = 0.044715f;
 
-// act(g) and, if derivative != nullptr, act'(g).
+// act(g) and, if derivative != nullptr, act'(g), for a result of type T.
+template <typename T>
 __device__ __forceinline__ float activate(int activation, float g, float* derivative = nullptr) {
   if (activation == static_cast<int>(Activation::kSilu)) {
-    const float s = sigmoid_f32(g);
+    const float s = sigmoid_f32<T>(g);
     if (derivative != nullptr) *derivative = s * (1.0f + g * (1.0f - s));
     return g * s;
   }

@@ -27,7 +27,7 @@
 // where it is not (the weights in kGated, both operands of kDw), so no tensor
 // is transposed.
 //
-// FP32 (kTerms = 3): each operand is the exact sum of three bfloat16 parts
+// FP32 (three parts per operand): each operand is the exact sum of three bfloat16 parts
 // (8 + 8 + 8 significand bits), and the product sums the six part products of
 // weight 2^-16 and above; what is left out is below 2^-23 of |a||b|. The
 // tensor core truncates when it accumulates, with a bias that grows with the
@@ -61,6 +61,7 @@ constexpr int kTileM = 2 * kRowsCta;
 constexpr int kTileN = 256;
 constexpr int kBoxBytes = 8192;            // 64 lines of 128 bytes
 constexpr int kOperandBytes = 2 * kBoxBytes;
+constexpr int kBand = 8;
 constexpr int kTmemCols = 512;
 constexpr int kEpiWarp0 = 4;
 constexpr int kEpiWarps = 8;
@@ -69,10 +70,12 @@ constexpr uint64_t kDrainNs = 2000000;
 constexpr int kPolls = 256;
 constexpr int kStagingBytes = 32 * 64;  // 64 bytes of 32 rows, per epilogue warp
 
-template <int kTerms>
+// A stage holds one k-block: kPa parts of A and kPb parts of B, 16 KB each.
+template <int kPa, int kPb>
 struct Config {
-  static constexpr int kStageBytes = 2 * kTerms * kOperandBytes;
-  static constexpr int kStages = kTerms == 1 ? 6 : 2;
+  static constexpr int kOffB = kPa * kOperandBytes;
+  static constexpr int kStageBytes = kOffB + kPb * kOperandBytes;
+  static constexpr int kStages = 12 * kOperandBytes / kStageBytes;  // 192 KB
 };
 
 struct EngineArgs {
@@ -87,20 +90,19 @@ struct EngineArgs {
   int hidden;   // contraction of kGated and kInt8; output columns of kDx, rows of kDw's tiles
   int output;   // output columns of kGated, kDw, kInt8; contraction (twice) of kDx
   int activation;
-  int parts;        // of dg and du where kTerms == 1: 2 sums the low part first
   int vec;          // 16-byte stores of out0 / out1 allowed
   int vec_gate_up;  // and of gate_up
 };
 
-template <int kTerms>
+template <typename Cfg>
 struct alignas(1024) EngineSmem {
-  uint8_t stage[Config<kTerms>::kStages][Config<kTerms>::kStageBytes];
+  uint8_t stage[Cfg::kStages][Cfg::kStageBytes];
   uint8_t staging[kEpiWarps][kStagingBytes];  // output rows on their way out
-  uint64_t empty[Config<kTerms>::kStages];  // the pair's MMAs have read the stage
-  uint64_t ready[Config<kTerms>::kStages];  // even CTA: both CTAs' halves are in place
-  uint64_t tail[Config<kTerms>::kStages];   // kDw: this CTA's half of a short block landed
-  uint64_t tmem_full[2];                    // accumulator finished (both CTAs)
-  uint64_t tmem_empty[2];                   // even CTA: both CTAs have read it
+  uint64_t empty[Cfg::kStages];  // the pair's MMAs have read the stage
+  uint64_t ready[Cfg::kStages];  // even CTA: both CTAs' halves are in place
+  uint64_t tail[Cfg::kStages];   // kDw: this CTA's half of a short block landed
+  uint64_t tmem_full[2];         // accumulator finished (both CTAs)
+  uint64_t tmem_empty[2];        // even CTA: both CTAs have read it
   uint64_t mma_done;
   uint32_t tmem_base;
   int failed;
@@ -134,11 +136,11 @@ __device__ __forceinline__ void mma_i8_pair(uint32_t d_tmem, uint64_t a_desc, ui
 struct Tile {
   int expert;
   int m0, m_end;  // rows of the output (kDw: of the weight matrix)
-  int c0, ncols;  // columns of each product
   int m_mma;      // rows of the instruction: 256, or 128 when at most 128 are left
+  int c0, ncols;  // columns of each product
   int n_mma;      // accumulator columns, a multiple of 32
   int own;        // kGated: gate (and up) columns of each CTA
-  int blocks;     // k-blocks of the contraction
+  int k_blocks;   // of the contraction
   int row0, row_end;  // the segment (kDw's contraction)
 };
 
@@ -196,7 +198,14 @@ __device__ __forceinline__ Tile tile_at(const EngineArgs& p, int t, const int* p
   const int2 s = segment(p.offsets, g.expert, p.rows);
   g.row0 = s.x;
   g.row_end = s.y;
-  const int mt = local / n_tiles, nt = local - mt * n_tiles;
+  // Bands of kBand row tiles, column by column: the tiles in flight then touch
+  // about as many row blocks as column blocks, so few bytes feed them all.
+  const int m_tiles = kMode == kDw ? (p.hidden + kTileM - 1) / kTileM : tiles_of(s, 1);
+  const int band = local / (kBand * n_tiles);
+  const int in_band = local - band * kBand * n_tiles;
+  const int band_tiles = min(kBand, m_tiles - band * kBand);
+  const int nt = in_band / band_tiles;
+  const int mt = band * kBand + in_band - nt * band_tiles;
   const int width = kTwo ? kTileN / 2 : kTileN;
   const int total = kMode == kDx ? p.hidden : p.output;
   g.c0 = nt * width;
@@ -208,13 +217,13 @@ __device__ __forceinline__ Tile tile_at(const EngineArgs& p, int t, const int* p
   if constexpr (kMode == kDw) {
     g.m0 = mt * kTileM;
     g.m_end = p.hidden;
-    g.blocks = p.parts * ((s.y - s.x + 63) >> 6);
+    g.k_blocks = (s.y - s.x + 63) >> 6;
   } else {
     g.m0 = s.x + mt * kTileM;
     g.m_end = s.y;
-    if constexpr (kMode == kDx) g.blocks = 2 * p.parts * ((p.output + 63) >> 6);
-    else if constexpr (kMode == kInt8) g.blocks = (p.hidden + 127) >> 7;
-    else g.blocks = (p.hidden + 63) >> 6;
+    if constexpr (kMode == kDx) g.k_blocks = 2 * ((p.output + 63) >> 6);
+    else if constexpr (kMode == kInt8) g.k_blocks = (p.hidden + 127) >> 7;
+    else g.k_blocks = (p.hidden + 63) >> 6;
   }
   g.m_mma = g.m_end - g.m0 <= kRowsCta ? kRowsCta : kTileM;
   return g;
@@ -275,34 +284,40 @@ __device__ __forceinline__ void store_rows32(uint8_t* staging, const float* v, T
   }
 }
 
-template <int kMode, int kTerms, typename T>
+template <int kMode, int kPa, int kPb, typename T>
 __global__ void __launch_bounds__(kThreads, 1) expert_gemm_kernel(
     const __grid_constant__ CUtensorMap map_a0, const __grid_constant__ CUtensorMap map_a1,
     const __grid_constant__ CUtensorMap map_b0, const __grid_constant__ CUtensorMap map_b1,
     const EngineArgs p) {
+  using Cfg = Config<kPa, kPb>;
   constexpr bool kTwo = kMode == kGated || kMode == kDw;
   constexpr bool kMnA = kMode == kDw;
   constexpr bool kMnB = kMode == kGated || kMode == kDw;
-  constexpr int kStages = Config<kTerms>::kStages;
-  constexpr uint32_t kStageTx = Config<kTerms>::kStageBytes;
-  constexpr int kOffB = kTerms * kOperandBytes;
+  constexpr bool kFp32 = kPa == 3;  // every k-block its own accumulation
+  constexpr int kStages = Cfg::kStages;
+  constexpr int kOffB = Cfg::kOffB;
   // Byte step of one K = 16 (bfloat16) or 32 (int8) MMA inside a box, and the
   // descriptors' offsets: K-major tiles repeat every 8 rows of 128 bytes;
   // MN-major ones every 8 k-lines of 128 bytes, the next 64 columns one box on.
   constexpr uint32_t kStepA = kMnA ? 2048 : 32, kStepB = kMnB ? 2048 : 32;
   constexpr uint32_t kLboA = kMnA ? kBoxBytes : 16, kLboB = kMnB ? kBoxBytes : 16;
+  // Part products (a, b) in rising magnitude. Three parts: 2^-16 three times,
+  // 2^-8 twice, 1.
+  constexpr int kProducts = kFp32 ? 6 : kPa * kPb;
+  constexpr int kProductA[6] = {kFp32 ? 2 : kPa - 1, 0, 1, 1, 0, 0};
+  constexpr int kProductB[6] = {kFp32 ? 0 : kPb - 1, kFp32 ? 2 : 0, 1, 0, 1, 0};
 
   extern __shared__ uint8_t smem_raw[];
-  auto& s = *reinterpret_cast<EngineSmem<kTerms>*>(
+  auto& s = *reinterpret_cast<EngineSmem<Cfg>*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  const uint32_t rank = cluster_ctarank();
+  const int rank = static_cast<int>(cluster_ctarank());
   const bool leader = rank == 0;
   const int unit = static_cast<int>(blockIdx.x >> 1);
   const int units = static_cast<int>(gridDim.x >> 1);
-  const int n_tiles = ((kMode == kDx ? p.hidden : p.output) + (kTwo ? kTileN / 2 : kTileN) - 1) /
-                      (kTwo ? kTileN / 2 : kTileN);
+  constexpr int kWidth = kTwo ? kTileN / 2 : kTileN;
+  const int n_tiles = ((kMode == kDx ? p.hidden : p.output) + kWidth - 1) / kWidth;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
@@ -334,7 +349,7 @@ __global__ void __launch_bounds__(kThreads, 1) expert_gemm_kernel(
   tc_fence_after();
   const uint32_t tmem = s.tmem_base;
   volatile int* failed = &s.failed;
-  const uint32_t peer_failed = mapa_shared(smem_u32(&s.failed), rank ^ 1u);
+  const uint32_t peer_failed = mapa_shared(smem_u32(&s.failed), rank ^ 1);
   auto wait = [&](uint64_t* bar, uint32_t parity) {
     // Most waits end within microseconds: poll before reading any clock.
 #pragma unroll 1
@@ -343,29 +358,19 @@ __global__ void __launch_bounds__(kThreads, 1) expert_gemm_kernel(
     }
     return mbar_wait_pair(bar, parity, p.err, failed, peer_failed);
   };
+  auto tile = [&](int t) { return tile_at<kMode>(p, t, s.prefix, n_tiles); };
 
   if (warp == 0) {
     // ---------------- TMA producer ----------------
-    {
-      int stage = 0;
-      uint32_t phase = 0;
-      for (int t = unit; t < total && !*failed; t += units) {
-        const Tile g = tile_at<kMode>(p, t, s.prefix, n_tiles);
-        const int m = g.m0 + static_cast<int>(rank) * (g.m_mma >> 1);
-        const int half = g.n_mma >> 1;
-        // k-blocks of one part: kDx and kDw pass over the contraction once per
-        // part of dg and du (kb runs within it; plane counts down to the top part).
-        const int pass = g.blocks / p.parts;
-        int kb = 0, plane = p.parts - 1;
-        for (int i = 0; i < g.blocks; ++i, ++kb) {
-          if (kb == pass) {
-            kb = 0;
-            --plane;
-          }
-          if (!wait(&s.empty[stage], phase ^ 1u)) break;
-          if (elect_one()) {
-          uint8_t* a = s.stage[stage];
-          uint8_t* b = a + kOffB;
+    int stage = 0;
+    uint32_t phase = 0;
+    for (int t = unit; t < total && !*failed; t += units) {
+      const Tile g = tile(t);
+      const int half = g.n_mma >> 1;
+      const int m = g.m0 + rank * (g.m_mma >> 1);
+      for (int kb = 0; kb < g.k_blocks; ++kb) {
+        if (!wait(&s.empty[stage], phase ^ 1u)) break;
+        if (elect_one()) {
           // Both CTAs' bytes complete on the even CTA's barrier. A short last
           // block of kDw completes on each CTA's own: its relay warp hands it
           // over once it has cleared the lines past the segment.
@@ -373,57 +378,58 @@ __global__ void __launch_bounds__(kThreads, 1) expert_gemm_kernel(
           uint32_t bar;
           if (cut) {
             bar = smem_u32(&s.tail[stage]);
-            mbar_arrive_expect_tx(&s.tail[stage], kStageTx);
+            mbar_arrive_expect_tx(&s.tail[stage], Cfg::kStageBytes);
           } else {
             bar = mapa_shared(smem_u32(&s.ready[stage]), 0u);
-            if (leader) mbar_arrive_expect_tx(&s.ready[stage], 2 * kStageTx);
+            if (leader) mbar_arrive_expect_tx(&s.ready[stage], 2 * Cfg::kStageBytes);
             else if (kMode == kDw) mbar_arrive_remote(bar);
           }
+          // The contraction's first element; kDx passes over two pairs of operands.
+          const int pass = g.k_blocks >> 1;
+          const bool second = kMode == kDx && kb >= pass;
+          const int k = kMode == kDw ? g.row0 + kb * 64
+                                     : (second ? kb - pass : kb) * (kMode == kInt8 ? 128 : 64);
+          uint8_t* a = s.stage[stage];
 #pragma unroll
-          for (int q = 0; q < kTerms; ++q, a += kOperandBytes, b += kOperandBytes) {
-            if constexpr (kMode == kGated) {
-              const int c = g.c0 + static_cast<int>(rank) * g.own;
-              const int z = q * p.experts + g.expert;
-              tma_load_3d_pair(a, &map_a0, bar, kb * 64, m, q);
-              tma_load_3d_pair(b, &map_b0, bar, c, kb * 64, z);
-              tma_load_3d_pair(b + kBoxBytes, &map_b1, bar, c, kb * 64, z);
-            } else if constexpr (kMode == kDx) {
-              const int per = pass >> 1;
-              const bool first = kb < per;
-              const int k = (first ? kb : kb - per) * 64;
-              tma_load_3d_pair(a, first ? &map_a0 : &map_a1, bar, k, m, kTerms == 1 ? plane : q);
-              tma_load_3d_pair(b, first ? &map_b0 : &map_b1, bar, k,
-                               g.c0 + static_cast<int>(rank) * half, q * p.experts + g.expert);
-            } else if constexpr (kMode == kDw) {
-              const CUtensorMap* mb = leader ? &map_b0 : &map_b1;
-              const int r = g.row0 + kb * 64;
-              tma_load_3d_pair(a, &map_a0, bar, m, r, q);
-              tma_load_3d_pair(a + kBoxBytes, &map_a0, bar, m + 64, r, q);
-              const int z = kTerms == 1 ? plane : q;
-              tma_load_3d_pair(b, mb, bar, g.c0, r, z);
-              tma_load_3d_pair(b + kBoxBytes, mb, bar, g.c0 + 64, r, z);
+          for (int q = 0; q < kPa; ++q, a += kOperandBytes) {
+            if constexpr (kMode == kDw) {
+              tma_load_3d_pair(a, &map_a0, bar, m, k, q);
+              tma_load_3d_pair(a + kBoxBytes, &map_a0, bar, m + 64, k, q);
             } else {
-              tma_load_3d_pair(a, &map_a0, bar, kb * 128, m, 0);
-              tma_load_3d_pair(b, &map_b0, bar, kb * 128, g.c0 + static_cast<int>(rank) * half,
-                               g.expert);
+              tma_load_3d_pair(a, second ? &map_a1 : &map_a0, bar, k, m, q);
             }
           }
-          }
-          __syncwarp();
-          if (++stage == kStages) {
-            stage = 0;
-            phase ^= 1u;
+          uint8_t* b = a;
+#pragma unroll
+          for (int q = 0; q < kPb; ++q, b += kOperandBytes) {
+            const int z = q * p.experts + g.expert;
+            if constexpr (kMode == kGated) {
+              const int c = g.c0 + rank * g.own;
+              tma_load_3d_pair(b, &map_b0, bar, c, k, z);
+              tma_load_3d_pair(b + kBoxBytes, &map_b1, bar, c, k, z);
+            } else if constexpr (kMode == kDw) {
+              const CUtensorMap* mb = leader ? &map_b0 : &map_b1;
+              tma_load_3d_pair(b, mb, bar, g.c0, k, q);
+              tma_load_3d_pair(b + kBoxBytes, mb, bar, g.c0 + 64, k, q);
+            } else {
+              tma_load_3d_pair(b, second ? &map_b1 : &map_b0, bar, k, g.c0 + rank * half, z);
+            }
           }
         }
-      }
-      // Wait for the MMAs' last use of every stage: nothing may read or signal
-      // this CTA's shared memory after it exits.
-      for (int i = 0; i < kStages && !*failed; ++i) {
-        if (!wait(&s.empty[stage], phase ^ 1u)) break;
+        __syncwarp();
         if (++stage == kStages) {
           stage = 0;
           phase ^= 1u;
         }
+      }
+    }
+    // Wait for the MMAs' last use of every stage: nothing may read or signal
+    // this CTA's shared memory after it exits.
+    for (int i = 0; i < kStages && !*failed; ++i) {
+      if (!wait(&s.empty[stage], phase ^ 1u)) break;
+      if (++stage == kStages) {
+        stage = 0;
+        phase ^= 1u;
       }
     }
   } else if (warp == 1) {
@@ -433,59 +439,43 @@ __global__ void __launch_bounds__(kThreads, 1) expert_gemm_kernel(
       uint32_t phase = 0, acc_phase = 0;
       bool ok = true;
       for (int t = unit; t < total && ok && !*failed; t += units) {
-        const Tile g = tile_at<kMode>(p, t, s.prefix, n_tiles);
-        const uint32_t idesc =
-            kMode == kInt8 ? idesc_i8(g.m_mma, g.n_mma)
-                           : idesc_f16(g.m_mma, g.n_mma, kMnA, kMnB);
-        for (int kb = 0; kb < g.blocks && ok; ++kb) {
-          const bool opens = kTerms == 3 || kb == 0;
-          if (opens && !wait(&s.tmem_empty[buf], acc_phase ^ 1u)) {
-            ok = false;
-            break;
-          }
-          if (!wait(&s.ready[stage], phase)) {
+        const Tile g = tile(t);
+        const uint32_t idesc = kMode == kInt8 ? idesc_i8(g.m_mma, g.n_mma)
+                                              : idesc_f16(g.m_mma, g.n_mma, kMnA, kMnB);
+        for (int kb = 0; kb < g.k_blocks; ++kb) {
+          if (((kFp32 || kb == 0) && !wait(&s.tmem_empty[buf], acc_phase ^ 1u)) ||
+              !wait(&s.ready[stage], phase)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint32_t d = tmem + static_cast<uint32_t>(buf) * kTileN;
-          const uint32_t base = smem_u32(s.stage[stage]);
-          const uint64_t a0 = smem_desc(base, kLboA, 1024, Swizzle::k128B);
-          const uint64_t b0 = smem_desc(base + kOffB, kLboB, 1024, Swizzle::k128B);
+          const bool last = kFp32 || kb + 1 == g.k_blocks;
           if (elect_one()) {
-          if constexpr (kTerms == 1) {
+            const uint32_t d = tmem + static_cast<uint32_t>(buf) * kTileN;
+            const uint32_t base = smem_u32(s.stage[stage]);
+            const uint64_t a0 = smem_desc(base, kLboA, 1024, Swizzle::k128B);
+            const uint64_t b0 = smem_desc(base + kOffB, kLboB, 1024, Swizzle::k128B);
 #pragma unroll
-            for (uint32_t ks = 0; ks < 4; ++ks) {
-              const uint64_t ad = a0 + ks * (kStepA >> 4), bd = b0 + ks * (kStepB >> 4);
-              const uint32_t acc = (kb > 0 || ks > 0) ? 1u : 0u;
-              if constexpr (kMode == kInt8) mma_i8_pair(d, ad, bd, idesc, acc);
-              else mma_bf16_pair(d, ad, bd, idesc, acc);
-            }
-          } else {
-            // Parts (a, b) in rising magnitude: 2^-16 three times, 2^-8 twice, 1.
-            constexpr int kPa[6] = {2, 0, 1, 1, 0, 0};
-            constexpr int kPb[6] = {0, 2, 1, 0, 1, 0};
-#pragma unroll
-            for (int q = 0; q < 6; ++q) {
+            for (int q = 0; q < kProducts; ++q) {
+              const uint64_t aq = a0 + kProductA[q] * (kOperandBytes >> 4);
+              const uint64_t bq = b0 + kProductB[q] * (kOperandBytes >> 4);
 #pragma unroll
               for (uint32_t ks = 0; ks < 4; ++ks) {
-                mma_bf16_pair(d, a0 + kPa[q] * (kOperandBytes >> 4) + ks * (kStepA >> 4),
-                              b0 + kPb[q] * (kOperandBytes >> 4) + ks * (kStepB >> 4), idesc,
-                              (q > 0 || ks > 0) ? 1u : 0u);
+                const uint64_t ad = aq + ks * (kStepA >> 4), bd = bq + ks * (kStepB >> 4);
+                const uint32_t add = ((!kFp32 && kb > 0) || q > 0 || ks > 0) ? 1u : 0u;
+                if constexpr (kMode == kInt8) mma_i8_pair(d, ad, bd, idesc, add);
+                else mma_bf16_pair(d, ad, bd, idesc, add);
               }
             }
-          }
-          mma_commit_pair_both(smem_u32(&s.empty[stage]));
-          if (kTerms == 3 || kb + 1 == g.blocks) {
-            mma_commit_pair_both(smem_u32(&s.tmem_full[buf]));
-          }
+            mma_commit_pair_both(smem_u32(&s.empty[stage]));
+            if (last) mma_commit_pair_both(smem_u32(&s.tmem_full[buf]));
           }
           __syncwarp();
           if (++stage == kStages) {
             stage = 0;
             phase ^= 1u;
           }
-          if (kTerms == 3 || kb + 1 == g.blocks) {
+          if (last) {
             buf ^= 1;
             if (buf == 0) acc_phase ^= 1u;
           }
@@ -502,27 +492,25 @@ __global__ void __launch_bounds__(kThreads, 1) expert_gemm_kernel(
       int at = 0;           // k-blocks so far: stage at % kStages
       uint32_t phases = 0;  // per stage, of its tail barrier
       for (int t = unit; t < total && !*failed; t += units) {
-        const Tile g = tile_at<kMode>(p, t, s.prefix, n_tiles);
+        const Tile g = tile(t);
+        at = (at + g.k_blocks) % kStages;
         const int valid = (g.row_end - g.row0) & 63;
-        for (int part = 0; part < p.parts && valid != 0; ++part) {
-          // The last block of each pass over the rows.
-          const int stage = (at + (part + 1) * (g.blocks / p.parts) + kStages - 1) % kStages;
-          if (!wait(&s.tail[stage], (phases >> stage) & 1u)) break;
-          phases ^= 1u << stage;
-          // Lines past the segment's end hold other segments' rows (or
-          // anything): both operands become zero there. A line is one row of a
-          // box, so the swizzle inside it does not matter.
-          for (int bx = 0; bx < 4 * kTerms; ++bx) {
-            uint8_t* box = s.stage[stage] + bx * kBoxBytes;
-            for (int i = valid * 8 + lane; i < 512; i += 32) {
-              reinterpret_cast<uint4*>(box)[i] = make_uint4(0u, 0u, 0u, 0u);
-            }
+        if (valid == 0) continue;
+        const int stage = (at + kStages - 1) % kStages;  // of the last block
+        if (!wait(&s.tail[stage], (phases >> stage) & 1u)) break;
+        phases ^= 1u << stage;
+        // Lines past the segment's end hold other segments' rows (or
+        // anything): both operands become zero there. A line is one row of a
+        // box, so the swizzle inside it does not matter.
+        for (int bx = 0; bx < 2 * (kPa + kPb); ++bx) {
+          uint8_t* box = s.stage[stage] + bx * kBoxBytes;
+          for (int i = valid * 8 + lane; i < 512; i += 32) {
+            reinterpret_cast<uint4*>(box)[i] = make_uint4(0u, 0u, 0u, 0u);
           }
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_remote(mapa_shared(smem_u32(&s.ready[stage]), 0u));
         }
-        at = (at + g.blocks) % kStages;
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_remote(mapa_shared(smem_u32(&s.ready[stage]), 0u));
       }
     }
   } else if (warp >= kEpiWarp0) {
@@ -535,17 +523,17 @@ __global__ void __launch_bounds__(kThreads, 1) expert_gemm_kernel(
     uint32_t acc_phase = 0;
     bool ok = true;
     for (int t = unit; t < total && ok && !*failed; t += units) {
-      const Tile g = tile_at<kMode>(p, t, s.prefix, n_tiles);
+      const Tile g = tile(t);
       const int half = g.n_mma >> 1;
       const bool folded = g.m_mma < kTileM;
       const int side = quarter >> 1;  // folded: the half of the columns in these lanes
-      const int row0 = g.m0 + static_cast<int>(rank) * (g.m_mma >> 1) +
+      const int row0 = g.m0 + rank * (g.m_mma >> 1) +
                        (folded ? quarter & 1 : quarter) * 32;  // of the warp
       const int rows = max(0, min(32, g.m_end - row0));
-      // This warp's groups of 32 accumulator columns, q = 0 .. groups - 1: TMEM
-      // column, first output column, and output columns left from there on
-      // (none: the group is skipped; warp-uniform). In kGated a group's up
-      // columns lie 64 TMEM columns after its gate columns.
+      // This warp's groups of 32 accumulator columns, q = 0 .. groups - 1:
+      // TMEM column, first output column, and output columns left from there
+      // on (none: the group is skipped; warp-uniform). In kGated a group's
+      // up columns lie 64 TMEM columns after its gate columns.
       const int groups = (kMode == kGated ? 2 : 4) >> (folded ? 1 : 0);
       auto group_col = [&](int q) {
         if constexpr (kMode == kGated) return folded ? 32 * hw : hw * half + 32 * q;
@@ -579,13 +567,14 @@ __global__ void __launch_bounds__(kThreads, 1) expert_gemm_kernel(
         if constexpr (kMode == kGated) {
           float h[32];
 #pragma unroll
-          for (int i = 0; i < 32; ++i) h[i] = activate(p.activation, v[i]) * v2[i];
+          for (int i = 0; i < 32; ++i) h[i] = activate<T>(p.activation, v[i]) * v2[i];
           const long long at = static_cast<long long>(row0) * p.output + g.c0 + c;
           store_rows32<T>(staging, h, static_cast<T*>(p.out0) + at, p.output, rows, cols,
                           p.vec != 0);
           if (p.gate_up != nullptr) {
             float* gu = p.gate_up + 2LL * row0 * p.output + g.c0 + c;
-            store_rows32<float>(staging, v, gu, 2LL * p.output, rows, cols, p.vec_gate_up != 0);
+            store_rows32<float>(staging, v, gu, 2LL * p.output, rows, cols,
+                                p.vec_gate_up != 0);
             store_rows32<float>(staging, v2, gu + p.output, 2LL * p.output, rows, cols,
                                 p.vec_gate_up != 0);
           }
@@ -612,13 +601,6 @@ __global__ void __launch_bounds__(kThreads, 1) expert_gemm_kernel(
           }
         }
       };
-      auto load = [&](int col, float* v) {
-        uint32_t r[32];
-        tmem_ld_32x32b_x32(tmem + static_cast<uint32_t>(buf * kTileN + col) + lane_addr, r);
-        tmem_ld_wait();
-#pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-      };
       auto take = [&]() {  // the accumulator is finished
         if (!wait(&s.tmem_full[buf], acc_phase)) return false;
         tc_fence_after();
@@ -632,15 +614,22 @@ __global__ void __launch_bounds__(kThreads, 1) expert_gemm_kernel(
         if (buf == 0) acc_phase ^= 1u;
       };
       if constexpr (kMode == kDw) {
-        if (g.blocks == 0) {  // no rows: a zero gradient
+        if (g.k_blocks == 0) {  // no rows: a zero gradient
           const float zero[32] = {};
 #pragma unroll 1
           for (int q = 0; q < groups; ++q) put(q, zero, zero);
           continue;
         }
       }
-      if constexpr (kTerms == 1) {
+      if constexpr (!kFp32) {
         if (!take()) break;
+        auto load = [&](int col, float* v) {
+          uint32_t r[32];
+          tmem_ld_32x32b_x32(tmem + static_cast<uint32_t>(buf * kTileN + col) + lane_addr, r);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+        };
 #pragma unroll 1
         for (int q = 0; q < groups; ++q) {
           if (group_left(q) <= 0) break;
@@ -659,21 +648,23 @@ __global__ void __launch_bounds__(kThreads, 1) expert_gemm_kernel(
         float sum[128];
 #pragma unroll
         for (int i = 0; i < 128; ++i) sum[i] = 0.0f;
-        for (int kb = 0; kb < g.blocks; ++kb) {
+        for (int kb = 0; kb < g.k_blocks; ++kb) {
           if (!take()) {
             ok = false;
             break;
           }
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {  // 16 columns; kGated: 0-3 gate, 4-7 up
-            const int q = kMode == kGated ? (j >> 1) & 1 : j >> 1;
+          for (int i = 0; i < 8; ++i) {  // 16 columns; kGated: 0-3 gate, 4-7 up
+            const int q = kMode == kGated ? (i >> 1) & 1 : i >> 1;
             if (q < groups && group_left(q) > 0) {
               uint32_t r[16];
-              const int col = group_col(q) + 16 * (j & 1) + (kMode == kGated ? 64 * (j >> 2) : 0);
-              tmem_ld_32x32b_x16(tmem + static_cast<uint32_t>(buf * kTileN + col) + lane_addr, r);
+              const int col =
+                  group_col(q) + 16 * (i & 1) + (kMode == kGated ? 64 * (i >> 2) : 0);
+              tmem_ld_32x32b_x16(tmem + static_cast<uint32_t>(buf * kTileN + col) + lane_addr,
+                                 r);
               tmem_ld_wait();
 #pragma unroll
-              for (int i = 0; i < 16; ++i) sum[16 * j + i] += __uint_as_float(r[i]);
+              for (int c = 0; c < 16; ++c) sum[16 * i + c] += __uint_as_float(r[c]);
             }
           }
           release();
@@ -726,7 +717,7 @@ constexpr int kMaxDevices = 64;
 
 // CTA pairs the device can hold at once, per kernel and device; 0 when the
 // kernel cannot be configured there.
-template <int kMode, int kTerms, typename T>
+template <int kMode, int kPa, int kPb, typename T>
 int engine_units(std::size_t smem) {
   static std::mutex mutex;
   static int known[kMaxDevices] = {};
@@ -734,7 +725,7 @@ int engine_units(std::size_t smem) {
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return 0;
   std::lock_guard<std::mutex> lock(mutex);
   if (known[dev] == 0) {
-    auto* kernel = expert_gemm_kernel<kMode, kTerms, T>;
+    auto* kernel = expert_gemm_kernel<kMode, kPa, kPb, T>;
     int n = 0;
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              static_cast<int>(smem)) == cudaSuccess) {
@@ -760,12 +751,12 @@ int engine_units(std::size_t smem) {
   return known[dev];
 }
 
-template <int kMode, int kTerms, typename T>
+template <int kMode, int kPa, int kPb, typename T>
 cudaError_t launch_engine(const CUtensorMap (&maps)[4], EngineArgs args, long long tiles,
                           cudaStream_t stream) {
-  constexpr std::size_t smem = sizeof(EngineSmem<kTerms>) + 1024;
+  constexpr std::size_t smem = sizeof(EngineSmem<Config<kPa, kPb>>) + 1024;
   static_assert(smem <= 227 * 1024, "over the shared memory a CTA may use");
-  int units = engine_units<kMode, kTerms, T>(smem);
+  int units = engine_units<kMode, kPa, kPb, T>(smem);
   if (units <= 0) return cudaErrorNotSupported;
   if (tiles < units) units = static_cast<int>(tiles);
   if (units <= 0) return cudaSuccess;
@@ -782,8 +773,9 @@ cudaError_t launch_engine(const CUtensorMap (&maps)[4], EngineArgs args, long lo
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, expert_gemm_kernel<kMode, kTerms, T>, maps[0],
-                                           maps[1], maps[2], maps[3], args);
+  const cudaError_t e = cudaLaunchKernelEx(
+      &cfg, expert_gemm_kernel<kMode, kPa, kPb, T>, maps[0], maps[1], maps[2], maps[3],
+      args);
   if (e != cudaSuccess) {
     cudaGetLastError();
     return e;
@@ -817,7 +809,6 @@ cudaError_t launch_gated_gemm(const GatedOperands& in, const int32_t* offsets, v
   }
   maps[1] = maps[0];
   EngineArgs a{};
-  a.parts = 1;
   a.offsets = offsets;
   a.out0 = h;
   a.gate_up = gate_up;
@@ -829,8 +820,9 @@ cudaError_t launch_gated_gemm(const GatedOperands& in, const int32_t* offsets, v
   a.vec = vec_ok(h, output, dtype);
   a.vec_gate_up = vec_ok(gate_up, output, Dtype::kFp32);
   const long long tiles = row_tiles(rows, experts, output, kTileN / 2);
-  return dtype == Dtype::kBf16 ? launch_engine<kGated, 1, __nv_bfloat16>(maps, a, tiles, stream)
-                               : launch_engine<kGated, 3, float>(maps, a, tiles, stream);
+  return dtype == Dtype::kBf16
+             ? launch_engine<kGated, 1, 1, __nv_bfloat16>(maps, a, tiles, stream)
+             : launch_engine<kGated, 3, 3, float>(maps, a, tiles, stream);
 }
 
 cudaError_t launch_gated_dx(const GatedOperands& in, const __nv_bfloat16* dg,
@@ -846,18 +838,17 @@ cudaError_t launch_gated_dx(const GatedOperands& in, const __nv_bfloat16* dg,
     return cudaErrorInvalidValue;
   }
   EngineArgs a{};
-  a.parts = 1;
   a.offsets = offsets;
   a.out0 = dx;
   a.experts = experts;
   a.rows = rows;
   a.hidden = hidden;
   a.output = output;
-  if (in.terms == 1) a.parts = parts;
   a.vec = vec_ok(dx, hidden, dtype);
   const long long tiles = row_tiles(rows, experts, hidden, kTileN);
-  return dtype == Dtype::kBf16 ? launch_engine<kDx, 1, __nv_bfloat16>(maps, a, tiles, stream)
-                               : launch_engine<kDx, 3, float>(maps, a, tiles, stream);
+  if (dtype == Dtype::kFp32) return launch_engine<kDx, 3, 3, float>(maps, a, tiles, stream);
+  if (parts == 2) return launch_engine<kDx, 2, 1, __nv_bfloat16>(maps, a, tiles, stream);
+  return launch_engine<kDx, 1, 1, __nv_bfloat16>(maps, a, tiles, stream);
 }
 
 cudaError_t launch_gated_dw(const GatedOperands& in, const __nv_bfloat16* dg,
@@ -872,7 +863,6 @@ cudaError_t launch_gated_dw(const GatedOperands& in, const __nv_bfloat16* dg,
   }
   maps[1] = maps[0];
   EngineArgs a{};
-  a.parts = 1;
   a.offsets = offsets;
   a.out0 = dwg;
   a.out1 = dwu;
@@ -880,12 +870,12 @@ cudaError_t launch_gated_dw(const GatedOperands& in, const __nv_bfloat16* dg,
   a.rows = rows;
   a.hidden = hidden;
   a.output = output;
-  if (in.terms == 1) a.parts = parts;
   a.vec = vec_ok(dwg, output, dtype) && vec_ok(dwu, output, dtype);
   const long long tiles = static_cast<long long>(experts) * ceil_div(hidden, kTileM) *
                           ceil_div(output, kTileN / 2);
-  return dtype == Dtype::kBf16 ? launch_engine<kDw, 1, __nv_bfloat16>(maps, a, tiles, stream)
-                               : launch_engine<kDw, 3, float>(maps, a, tiles, stream);
+  if (dtype == Dtype::kFp32) return launch_engine<kDw, 3, 3, float>(maps, a, tiles, stream);
+  if (parts == 2) return launch_engine<kDw, 1, 2, __nv_bfloat16>(maps, a, tiles, stream);
+  return launch_engine<kDw, 1, 1, __nv_bfloat16>(maps, a, tiles, stream);
 }
 
 cudaError_t launch_int8_gemm(const int8_t* xq, const float* x_scale, const int8_t* wq,
@@ -899,7 +889,6 @@ cudaError_t launch_int8_gemm(const int8_t* xq, const float* x_scale, const int8_
   maps[1] = maps[0];
   maps[3] = maps[2];
   EngineArgs a{};
-  a.parts = 1;
   a.offsets = offsets;
   a.out0 = y;
   a.row_scale = x_scale;
@@ -910,8 +899,8 @@ cudaError_t launch_int8_gemm(const int8_t* xq, const float* x_scale, const int8_
   a.output = output;
   a.vec = vec_ok(y, output, dtype);
   const long long tiles = row_tiles(rows, experts, output, kTileN);
-  return dtype == Dtype::kBf16 ? launch_engine<kInt8, 1, __nv_bfloat16>(maps, a, tiles, stream)
-                               : launch_engine<kInt8, 1, float>(maps, a, tiles, stream);
+  return dtype == Dtype::kBf16 ? launch_engine<kInt8, 1, 1, __nv_bfloat16>(maps, a, tiles, stream)
+                               : launch_engine<kInt8, 1, 1, float>(maps, a, tiles, stream);
 }
 
 }  // namespace rrb

@@ -167,7 +167,7 @@ __device__ __forceinline__ void few_rows(const T* __restrict__ x, const T* __res
   }
   if (i < nrows && i < kR && c0 + c < output) {
     const long long r = row + i;
-    h[r * output + c0 + c] = from_f32<T>(activate(activation, sg) * su);
+    h[r * output + c0 + c] = from_f32<T>(activate<T>(activation, sg) * su);
     if (gate_up != nullptr) {
       gate_up[2 * r * output + c0 + c] = sg;
       gate_up[(2 * r + 1) * output + c0 + c] = su;
@@ -387,7 +387,7 @@ __global__ void __launch_bounds__(kPackThreads) gated_pointwise_backward_kernel(
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       float slope;
-      const float a = activate(activation, g[j], &slope);
+      const float a = activate<T>(activation, g[j], &slope);
       g[j] = d[j] * u[j] * slope;
       u[j] = d[j] * a;
     }

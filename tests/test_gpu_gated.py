@@ -44,6 +44,16 @@ SHAPES = [
 ]
 
 
+# Long contractions and many tiles: two row blocks share a tile. Segments that
+# end in each quarter of such a tile; N and K that end inside one.
+LARGE = [
+    ([700, 0, 1100, 257, 513, 130, 385, 1], 3, 2050, 3400),  # forward (contraction K)
+    ([513, 900, 0, 1281, 100], 0, 3330, 1030),               # input gradient (2 N)
+    ([2600, 4100], 5, 1100, 7700),                           # weight gradients (rows)
+]
+SHAPES += LARGE
+
+
 def make(counts, behind, k, n, dtype, device, seed=0):
     rows = int(np.sum(counts)) + behind
     e = len(counts)

@@ -120,6 +120,7 @@ def operands(rows, experts, hidden, output, device, seed=0):
     ([300, 500], 9, 1030, 515),
     ([20] * 70, 0, 64, 40),
     ([90], 0, 20000, 24),
+    ([700, 0, 1100, 257, 513, 130, 385, 1], 3, 4100, 6700),  # two row blocks share a tile
 ], ids=str)
 def test_product(cuda, counts, behind, hidden, output, dtype):
     rows = int(np.sum(counts)) + behind
