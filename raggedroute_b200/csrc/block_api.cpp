@@ -103,12 +103,16 @@ bool rows_aligned(const void* p, long long cols, std::size_t size) {
 // ---- gated projection ----------------------------------------------------------
 
 // Few rows run without the tensor cores, straight from the caller's weights.
-// BF16: above 32 rows the engine's tiles read the weights as fast and reuse
-// them for all rows of an expert. FP32: the engine first writes the weights
-// as three bfloat16 parts (16 bytes moved per element against 4), which pays
-// once most experts have several rows.
+// BF16: where hardly any two rows share an expert both forms read the weights
+// once, and the plain one spreads them over all SMs (128 experts, K=4096,
+// N=1408: 2 rows 11 against 22 us, 64 rows 202 against 216; 64 experts,
+// K=N=1024: 32 rows 21 against 27); sharing experts, the engine's tiles reuse
+// them (64 rows 46 against 37). FP32: the engine first writes the weights of
+// every expert as three bfloat16 parts, 16 bytes moved per element, which pays
+// from about 16 rows per expert (8 experts, K=N=1024: 128 rows 46 against 73 us,
+// 256 rows 80 against 74).
 bool gated_few(int rows, int experts, Dtype dtype) {
-  return dtype == Dtype::kBf16 ? rows <= 32 : rows <= 2 * experts + 32;
+  return rows <= 4 || (dtype == Dtype::kBf16 ? 2LL * rows <= experts : rows <= 16LL * experts);
 }
 
 // Parts of dg and du in a bfloat16 backward pass. One rounding to bfloat16 is
@@ -119,7 +123,7 @@ bool gated_few(int rows, int experts, Dtype dtype) {
 // bits) doubles tensor work that is hidden behind them.
 int gradient_parts(int rows, int experts, Dtype dtype) {
   if (dtype == Dtype::kFp32) return 3;
-  return rows <= 64LL * experts ? 2 : 1;
+  return rows <= 32LL * experts ? 2 : 1;
 }
 
 // Where the operands of one call lie in the workspace; an offset of 0 bytes
@@ -439,8 +443,11 @@ rr_status rr_grouped_gemm_int8(const int8_t* xq, const float* x_scale, const int
   s = check_device(ctx);
   if (s.code != RR_SUCCESS) return s;
   // Few rows: the weights are read once either way, and the plain kernel
-  // spreads a single row over the whole GPU.
-  const bool few = route_pairs <= 32;
+  // spreads a single row over the whole GPU and starts faster (128 experts,
+  // K=4096, N=1408: 2 rows 3.2 against 13 us, 128 rows 88 against 95, 256 rows
+  // 138 against 130; 8 experts, K=N=1024: 32 rows 6.2 against 7.6, 64 rows 9.6
+  // against 7.6).
+  const bool few = route_pairs <= 32 || route_pairs <= experts;
   const cudaError_t e =
       few ? rrb::launch_int8_few(xq, x_scale, wq, w_scale, offsets, y_permuted, route_pairs,
                                  experts, ld, output, t, stream_of(ctx))

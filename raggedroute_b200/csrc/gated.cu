@@ -209,9 +209,9 @@ cudaError_t few(const void* x, const void* wg, const void* wu, const int32_t* of
   constexpr int kVec = 16 / sizeof(T);
   const bool vec = output % kVec == 0 && aligned_to(wg, 16) && aligned_to(wu, 16);
   const int groups = ceil_div(output, kFewCols<T>);
-  // One token's routes go to different experts, so up to two rows are taken
-  // one at a time; more may share an expert.
-  const bool single = rows <= 2;
+  // With rows scarce among the experts hardly any two share one, and rows are
+  // taken one at a time; more may share an expert.
+  const bool single = rows <= 2 || 2 * rows <= experts;
   // Contraction steps of a thread without a split; a split leaves four.
   const int steps = hidden / (kFewThreads / (kFewCols<T> / (vec ? kVec : 1)));
   int split = 1;

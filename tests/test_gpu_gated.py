@@ -345,7 +345,7 @@ def test_buffers_at_odd_addresses(cuda, dtype):
         assert bool((flat[:65] == 9.0).all()) and bool((flat[65 + t.numel():] == 9.0).all())
 
 
-@pytest.mark.parametrize("rows", [1, 2, 31, 32, 33, 34])
+@pytest.mark.parametrize("rows", [1, 2, 3, 4, 5, 6, 31, 32, 33, 34])
 def test_one_form_meets_the_other(cuda, rows):
     """The few-row and the tensor-core forms agree around their boundary."""
     x, wg, wu, off, _ = make([rows], 0, 512, 256, BF16, cuda, seed=80)
