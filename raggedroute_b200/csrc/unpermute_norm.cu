@@ -18,11 +18,11 @@
 // Two forms of each kernel. A token passes several dependent steps (positions,
 // rows, one or two reductions, stores), and with loads issued by the threads
 // that wait for them too few bytes are in flight. From a few tokens per SM up,
-// one persistent block per SM therefore streams the rows of the next tokens
-// into shared memory with bulk copies (a producer warp, a ring of stages)
-// while teams of 32 to 512 threads work on the current ones; rows of any
-// alignment are copied as the 16-byte granules they touch. Fewer tokens, and
-// rows too wide for the ring, take one plain block per token.
+// teams of 32 to 512 threads of one persistent block per SM therefore take a
+// token each, and each team streams the rows of its next tokens into a ring in
+// shared memory with bulk copies; rows of any alignment are copied as the
+// 16-byte granules they touch. Fewer tokens, and rows too wide for the ring,
+// take one plain block per token.
 #include <mutex>
 
 #include "expert_block.cuh"
@@ -363,36 +363,33 @@ __global__ void __launch_bounds__(kMaxThreads) unpermute_norm_backward_kernel(
 
 // ---- streamed form ------------------------------------------------------------------
 
-constexpr int kWorkers = 512;                   // worker threads per block, at most
-constexpr int kStreamThreads = kWorkers + 32;   // and the producer warp
+constexpr int kStreamThreads = 512;  // per block, at most
 constexpr int kStreamTopK = 16;
 constexpr int kMaxStages = 4;
-constexpr int kRounds = 3;                      // rows of a stage per producer lane
-constexpr int kMaxTeams = kWorkers / 32;
-constexpr std::size_t kRingBytes = 200 * 1024;
+constexpr int kMaxTeams = kStreamThreads / 32;
+constexpr std::size_t kRingBytes = 204 * 1024;
 
-// A stage holds the rows of one token per team: the route rows, the residual,
+// A team's ring has one token's rows per stage: the route rows, the residual,
 // and for the gradient d_residual_out and d_normed.
 struct Stream {
   int team = 0;      // threads per token
-  int teams = 0;     // tokens per stage
+  int teams = 0;     // of a block
   int sources = 0;   // rows per token
   int stride = 0;    // bytes of a row's place
-  int padded = 0;    // gradient: columns of the factors behind the ring
+  int padded = 0;    // gradient: columns of a factor kept behind the rings
+  int factors = 0;   // gradient: factors kept there: post * gate, and pre if it fits
   int stages = 0;
   int blocks = 0;
 };
 
 struct StreamSmem {
-  uint64_t full[kMaxStages];
-  uint64_t empty[kMaxStages];
+  uint64_t full[kMaxTeams][kMaxStages];
   int failed;
-  // What the producer knows of each token: where in its place a row starts
-  // (-1: a skipped route), and the route weights.
-  int start[kMaxStages][kMaxTeams][kStreamTopK + 3];
-  float weight[kMaxStages][kMaxTeams][kStreamTopK];
-  int pos[kMaxStages][kMaxTeams][kStreamTopK];
-  float parts[2][kMaxTeams][kStreamTopK + 1];  // of each warp, two reductions
+  // Of each token in a ring: where its rows start (-1: a skipped route), and
+  // the routes' weights and positions.
+  int start[kMaxTeams][kMaxStages][kStreamTopK + 3];
+  float weight[kMaxTeams][kMaxStages][kStreamTopK];
+  int pos[kMaxTeams][kMaxStages][kStreamTopK];
 };
 
 // The threads of one team (a barrier of its own each; one warp needs none).
@@ -401,102 +398,82 @@ __device__ __forceinline__ void team_sync(int team, int threads) {
   else asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "r"(threads) : "memory");
 }
 
-// Whether `ok` holds in every thread of the team.
-__device__ __forceinline__ bool team_all(int team, int threads, bool ok) {
-  if (threads == 32) return __all_sync(0xffffffffu, ok);
-  int r;
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\t"
-      "setp.ne.b32 p, %3, 0;\n\t"
-      "bar.red.and.pred q, %1, %2, p;\n\t"
-      "selp.b32 %0, 1, 0, q;\n\t}"
-      : "=r"(r)
-      : "r"(team + 1), "r"(threads), "r"(static_cast<int>(ok))
-      : "memory");
-  return r != 0;
-}
-
 struct Sources {
   const void* row[3] = {};  // residual, d_residual_out, d_normed; null ones left out
-  int count = 0;
 };
 
-// Streams the rows of this block's tokens. Lanes share the rows of a stage, up
-// to kRounds each; a route's position and weight are fetched one stage ahead.
-template <typename T>
-__device__ __forceinline__ void produce(const UnpermuteNorm& in, const Sources& src,
-                                        const Stream& st, StreamSmem& s, uint32_t ring,
-                                        unsigned* err) {
-  using namespace sm100;
-  const int lane = threadIdx.x & 31;
-  const long long routes = static_cast<long long>(in.tokens) * in.top_k;
-  const long long bytes = static_cast<long long>(in.output) * sizeof(T);
-  const int items = st.teams * st.sources;
-  const long long step = static_cast<long long>(gridDim.x) * st.teams;
-  int team[kRounds], r[kRounds], pos[kRounds];
-  float weight[kRounds];
-#pragma unroll
-  for (int j = 0; j < kRounds; ++j) {
-    team[j] = (lane + 32 * j) / st.sources;
-    r[j] = lane + 32 * j - team[j] * st.sources;
+// Fills a team's ring; called by its first warp, a lane per row (sources <= 32).
+// kAligned: rows are whole 16-byte granules.
+template <typename T, bool kAligned>
+struct Filler {
+  const UnpermuteNorm& in;
+  const Stream& st;
+  StreamSmem& s;
+  uint32_t ring;     // this team's
+  int team;
+  const char* base;  // of this lane's rows
+  long long rows;    // how many there are
+  int pos;           // of the next token's row, fetched ahead
+  float weight;
+
+  __device__ __forceinline__ Filler(const UnpermuteNorm& in, const Stream& st, StreamSmem& s,
+                                    const Sources& src, uint32_t ring, int team)
+      : in(in), st(st), s(s), ring(ring), team(team) {
+    const int lane = threadIdx.x & 31;
+    const bool route = lane < in.top_k;
+    base = route ? static_cast<const char*>(in.y_permuted)
+                 : (lane < st.sources ? static_cast<const char*>(src.row[lane - in.top_k])
+                                      : nullptr);
+    rows = route ? static_cast<long long>(in.tokens) * in.top_k
+                 : (lane < st.sources ? in.tokens : 0);
   }
-  auto fetch = [&](long long first) {
-#pragma unroll
-    for (int j = 0; j < kRounds; ++j) {
-      const long long t = first + team[j];
-      pos[j] = -1;
-      weight[j] = 0.0f;
-      if (lane + 32 * j < items && r[j] < in.top_k && t < in.tokens) {
-        pos[j] = __ldg(in.route_pos + t * in.top_k + r[j]);
-        weight[j] = __ldg(in.route_weights + t * in.top_k + r[j]);
-      }
+  __device__ __forceinline__ void fetch(long long t) {
+    const int lane = threadIdx.x & 31;
+    pos = -1;
+    weight = 0.0f;
+    if (lane < in.top_k && t < in.tokens) {
+      pos = __ldg(in.route_pos + t * in.top_k + lane);
+      weight = __ldg(in.route_weights + t * in.top_k + lane);
     }
-  };
-  int stage = 0;
-  uint32_t phase = 0;
-  long long first = static_cast<long long>(blockIdx.x) * st.teams;
-  fetch(first);
-  for (; first < in.tokens; first += step) {
-    if (!mbar_wait(&s.empty[stage], phase ^ 1u, err, &s.failed)) return;
-    const char* from[kRounds];
-    uint32_t size[kRounds], place[kRounds], total = 0;
-#pragma unroll
-    for (int j = 0; j < kRounds; ++j) {
-      size[j] = 0;
-      const int i = lane + 32 * j;
-      const long long t = first + team[j];
-      if (i >= items || t >= in.tokens) continue;
-      long long row = t, rows = in.tokens;
-      const char* base;
-      if (r[j] < in.top_k) {
-        row = pos[j];
-        rows = routes;
-        base = static_cast<const char*>(in.y_permuted);
-        s.weight[stage][team[j]][r[j]] = weight[j];
-        s.pos[stage][team[j]][r[j]] = pos[j];
-        if (row < 0 || row >= routes) {
-          s.start[stage][team[j]][r[j]] = -1;
-          continue;
-        }
-      } else {
-        base = static_cast<const char*>(src.row[r[j] - in.top_k]);
-      }
-      // The granules of the row. The buffers start on a 16-byte boundary, so
-      // only the last row's last granule can reach past one; its elements are
-      // copied one by one.
-      const long long at = row * bytes;
-      const long long a0 = at & ~15LL;
-      long long a1 = (at + bytes + 15) & ~15LL;
-      const bool past = a1 > rows * bytes;
+  }
+  // Starts token t's rows (position and weight fetched) into `stage`, and fetches
+  // those of token `next`.
+  __device__ __forceinline__ void fill(long long t, int stage, long long next) {
+    using namespace sm100;
+    if (t >= in.tokens) return;
+    const int lane = threadIdx.x & 31;
+    const long long bytes = static_cast<long long>(in.output) * sizeof(T);
+    const bool route = lane < in.top_k;
+    const long long row = route ? pos : t;
+    const bool there = row >= 0 && row < rows;
+    const int place = (stage * st.sources + lane) * st.stride;
+    const long long at = row * bytes;
+    // The granules of the row. The buffers start on a 16-byte boundary, so only
+    // the last row's last granule can reach past one; its elements are copied
+    // one by one.
+    long long a0 = at, a1 = at + bytes;
+    bool past = false;
+    if constexpr (!kAligned) {
+      a0 = at & ~15LL;
+      a1 = (a1 + 15) & ~15LL;
+      past = a1 > rows * bytes;
       if (past) a1 -= 16;
-      place[j] = (stage * items + i) * st.stride;
-      s.start[stage][team[j]][r[j]] = static_cast<int>(place[j] + (at - a0));
-      from[j] = base + a0;
-      size[j] = a1 > a0 ? static_cast<uint32_t>(a1 - a0) : 0u;
-      total += size[j];
-      if (past) {
+    }
+    const uint32_t size = there && a1 > a0 ? static_cast<uint32_t>(a1 - a0) : 0u;
+    if (lane < st.sources) {
+      s.start[team][stage][lane] = there ? static_cast<int>(place + (at - a0)) : -1;
+    }
+    if (route) {
+      s.weight[team][stage][lane] = weight;
+      s.pos[team][stage][lane] = pos;
+    }
+    uint32_t total;
+    if constexpr (kAligned) {
+      total = __popc(__ballot_sync(0xffffffffu, there)) * static_cast<uint32_t>(bytes);
+    } else {
+      if (there && past) {
         for (long long b = a1 > at ? a1 : at; b < at + bytes; b += sizeof(T)) {
-          const uint32_t to = ring + place[j] + static_cast<uint32_t>(b - a0);
+          const uint32_t to = ring + place + static_cast<uint32_t>(b - a0);
           if constexpr (sizeof(T) == 2) {
             asm volatile("st.shared.u16 [%0], %1;" ::"r"(to),
                          "h"(__ldg(reinterpret_cast<const unsigned short*>(base + b)))
@@ -508,22 +485,16 @@ __device__ __forceinline__ void produce(const UnpermuteNorm& in, const Sources& 
           }
         }
       }
+      total = __reduce_add_sync(0xffffffffu, size);
     }
-    total = __reduce_add_sync(0xffffffffu, total);
+    uint64_t* full = &s.full[team][stage];
     __syncwarp();  // the lanes' notes come before the arrival
-    if (lane == 0) mbar_arrive_expect_tx(&s.full[stage], total);
+    if (lane == 0) mbar_arrive_expect_tx(full, total);
     __syncwarp();
-#pragma unroll
-    for (int j = 0; j < kRounds; ++j) {
-      if (size[j] > 0) bulk_load(ring + place[j], from[j], size[j], &s.full[stage]);
-    }
-    fetch(first + step);
-    if (++stage == st.stages) {
-      stage = 0;
-      phase ^= 1u;
-    }
+    if (size > 0) bulk_load(ring + place, base + a0, size, full);
+    fetch(next);
   }
-}
+};
 
 // kPer columns of a staged row.
 template <typename T, int kPer>
@@ -604,15 +575,18 @@ __device__ __forceinline__ void staged_combine(const UnpermuteNorm& in, const St
   }
 }
 
-__device__ __forceinline__ void stream_setup(const Stream& st, StreamSmem& s) {
+__device__ __forceinline__ void stream_setup(const Stream& st, int top_k, StreamSmem& s) {
   using namespace sm100;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < st.stages; ++i) {
-      mbar_init(&s.full[i], 1);
-      mbar_init(&s.empty[i], st.team * st.teams / 32);
+    for (int i = 0; i < st.teams; ++i) {
+      for (int j = 0; j < st.stages; ++j) mbar_init(&s.full[i][j], 1);
     }
     s.failed = 0;
     fence_mbar_init();
+  }
+  // What a token finds after a wait that ran out: nothing, at a valid place.
+  for (int i = threadIdx.x; i < kMaxTeams * kMaxStages * (kStreamTopK + 3); i += blockDim.x) {
+    (&s.start[0][0][0])[i] = i % (kStreamTopK + 3) < top_k ? -1 : 0;
   }
   __syncthreads();
 }
@@ -628,318 +602,156 @@ __device__ __forceinline__ void stream_end(StreamSmem& s) {
   }
 }
 
+// The tokens of a team. step() waits for the next token's rows; refill(), called
+// after a barrier of the team inside that token, starts the rows that go where
+// the token before it was. A wait that runs out raises the error word and lets
+// the loop run on (further waits return at once): the team's barriers stay
+// matched, and what is computed is reported as wrong.
+template <typename T, bool kAligned>
+struct TokenLoop {
+  Filler<T, kAligned> filler;
+  unsigned* err;
+  long long t, stride;
+  int stage;
+  uint32_t phase;
+  bool filling, first_token;
+
+  __device__ __forceinline__ TokenLoop(const UnpermuteNorm& in, const Stream& st, StreamSmem& s,
+                                       const Sources& src, uint32_t ring, int team, unsigned* err)
+      : filler(in, st, s, src, ring, team), err(err) {
+    t = static_cast<long long>(blockIdx.x) * st.teams + team;
+    stride = static_cast<long long>(gridDim.x) * st.teams;
+    stage = -1;
+    phase = 0;
+    first_token = true;
+    filling = threadIdx.x % st.team < 32;
+    if (filling) {
+      filler.fetch(t);
+      for (int i = 0; i < st.stages; ++i) filler.fill(t + i * stride, i, t + (i + 1) * stride);
+    }
+    t -= stride;
+  }
+  __device__ __forceinline__ bool step() {
+    t += stride;
+    if (t >= filler.in.tokens) return false;  // uniform over a team
+    if (++stage == filler.st.stages) {
+      stage = 0;
+      phase ^= 1u;
+    }
+    sm100::mbar_wait(&filler.s.full[filler.team][stage], phase, err, &filler.s.failed);
+    return true;
+  }
+  __device__ __forceinline__ void refill() {
+    if (filling && !first_token) {
+      const int stages = filler.st.stages;
+      filler.fill(t + (stages - 1) * stride, stage == 0 ? stages - 1 : stage - 1,
+                  t + stages * stride);
+    }
+    first_token = false;
+  }
+};
+
 template <typename T, int kPer>
 __global__ void __launch_bounds__(kStreamThreads, 1) unpermute_norm_stream_kernel(
     const UnpermuteNorm in, const Stream st, T* residual_out, T* normed, float* inv_rms,
     unsigned* err) {
   using namespace sm100;
-  extern __shared__ __align__(16) char ring[];
+  extern __shared__ __align__(16) char rings[];
   __shared__ StreamSmem s;
-  stream_setup(st, s);
+  __shared__ float parts[2][kMaxTeams];  // sums of each warp
+  stream_setup(st, in.top_k, s);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (threadIdx.x >= st.team * st.teams) {
-    Sources src;
-    src.row[0] = in.residual;
-    produce<T>(in, src, st, s, smem_u32(ring), err);
-    stream_end(s);
-    return;
-  }
   const int team = threadIdx.x / st.team, tid = threadIdx.x % st.team;
   const int team_warps = st.team >> 5, warp0 = team * team_warps;
+  const char* ring = rings + team * st.stages * st.sources * st.stride;
   const float per_col = 1.0f / static_cast<float>(in.output);
   float pg[kElems], pr[kElems];  // post * gate and pre of this thread's columns
 #pragma unroll
   for (int q = 0; q < kElems / kPer; ++q) {
     column_factors<kPer>(in, (q * st.team + tid) * kPer, pg + q * kPer, pr + q * kPer);
   }
-  int stage = 0;
-  uint32_t phase = 0;
-  const long long step = static_cast<long long>(gridDim.x) * st.teams;
-  for (long long first = static_cast<long long>(blockIdx.x) * st.teams; first < in.tokens;
-       first += step) {
-    const bool ok = mbar_wait(&s.full[stage], phase, err, &s.failed);
-    if (!team_all(team, st.team, ok)) break;
-    const long long t = first + team;
-    if (t < in.tokens) {  // uniform over a team
-      const int* start = s.start[stage][team];
-      float c[kElems];
-      staged_combine<T, kPer>(in, st, ring, start, s.weight[stage][team], tid, c);
-      auto team_sum = [&](float v, int which) {
-        v = warp_sum(v);
-        if (team_warps == 1) return v;
-        if (lane == 0) s.parts[which][warp][0] = v;
-        team_sync(team, st.team);
-        float sum = 0.0f;
-        for (int w = 0; w < team_warps; ++w) sum += s.parts[which][warp0 + w][0];
-        return sum;
-      };
-      float i1 = 1.0f;
-      if (in.post_gamma != nullptr) {
-        float sq = 0.0f;
-#pragma unroll
-        for (int i = 0; i < kElems; ++i) sq = fmaf(c[i], c[i], sq);
-        i1 = rsqrtf(team_sum(sq, 0) * per_col + in.eps);
-      }
-      const char* res_row = ring + start[in.top_k];
+  auto team_sum = [&](float v, int which) {
+    v = warp_sum(v);
+    if (team_warps == 1) {
+      __syncwarp();
+      return v;
+    }
+    if (lane == 0) parts[which][warp] = v;
+    team_sync(team, st.team);
+    float sum = 0.0f;
+    for (int w = 0; w < team_warps; ++w) sum += parts[which][warp0 + w];
+    return sum;
+  };
+  Sources src;
+  src.row[0] = in.residual;
+  TokenLoop<T, kPer * sizeof(T) == 16> loop(in, st, s, src, smem_u32(ring), team, err);
+  while (loop.step()) {
+    const long long t = loop.t;
+    const int* start = s.start[team][loop.stage];
+    float c[kElems];
+    staged_combine<T, kPer>(in, st, ring, start, s.weight[team][loop.stage], tid, c);
+    float i1 = 1.0f;
+    if (in.post_gamma != nullptr) {
       float sq = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kElems; ++i) sq = fmaf(c[i], c[i], sq);
+      i1 = rsqrtf(team_sum(sq, 0) * per_col + in.eps);
+    } else {
+      team_sync(team, st.team);
+    }
+    loop.refill();
+    const char* res_row = ring + start[in.top_k];
+    float sq = 0.0f;
+#pragma unroll
+    for (int q = 0; q < kElems / kPer; ++q) {
+      const int col = (q * st.team + tid) * kPer;
+      if (col < in.output) {
+        float* r = c + q * kPer;
+        float res[kPer];
+        staged_cols<T, kPer>(res_row + col * sizeof(T), res);
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+          r[i] = fmaf(in.residual_scale, res[i], r[i] * i1 * pg[q * kPer + i]);
+          sq = fmaf(r[i], r[i], sq);
+        }
+        put_cols<T, kPer>(residual_out + t * in.output + col, r);
+      }
+    }
+    float i2 = 1.0f;
+    if (in.pre_gamma != nullptr) {
+      i2 = rsqrtf(team_sum(sq, 1) * per_col + in.eps);
 #pragma unroll
       for (int q = 0; q < kElems / kPer; ++q) {
         const int col = (q * st.team + tid) * kPer;
         if (col < in.output) {
           float* r = c + q * kPer;
-          float res[kPer];
-          staged_cols<T, kPer>(res_row + col * sizeof(T), res);
 #pragma unroll
-          for (int i = 0; i < kPer; ++i) {
-            r[i] = fmaf(in.residual_scale, res[i], r[i] * i1 * pg[q * kPer + i]);
-            sq = fmaf(r[i], r[i], sq);
-          }
-          put_cols<T, kPer>(residual_out + t * in.output + col, r);
+          for (int i = 0; i < kPer; ++i) r[i] *= i2 * pr[q * kPer + i];
+          put_cols<T, kPer>(normed + t * in.output + col, r);
         }
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&s.empty[stage]);
-      float i2 = 1.0f;
-      if (in.pre_gamma != nullptr) {
-        i2 = rsqrtf(team_sum(sq, 1) * per_col + in.eps);
-#pragma unroll
-        for (int q = 0; q < kElems / kPer; ++q) {
-          const int col = (q * st.team + tid) * kPer;
-          if (col < in.output) {
-            float* r = c + q * kPer;
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) r[i] *= i2 * pr[q * kPer + i];
-            put_cols<T, kPer>(normed + t * in.output + col, r);
-          }
-        }
-      }
-      if (inv_rms != nullptr && tid == 0) {
-        inv_rms[2 * t] = i1;
-        inv_rms[2 * t + 1] = i2;
-      }
-    } else {
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&s.empty[stage]);
     }
-    if (++stage == st.stages) {
-      stage = 0;
-      phase ^= 1u;
+    if (inv_rms != nullptr && tid == 0) {
+      inv_rms[2 * t] = i1;
+      inv_rms[2 * t + 1] = i2;
     }
   }
   stream_end(s);
 }
 
-// The gradient, with two reductions per token: the first of <v, rn> and of
-// Q_k = <cn, y_k>, the second of <v1, cn> and of P_k = <v1, y_k>, where
-// v1 = db post; then dw_k = <dc, y_k> = i1 (P_k - mean(v1 cn) Q_k) needs no
-// third (without the norm of c: dc = v1, dw_k = P_k). The gradients of post and
-// gate are one column sum, of dr cn, times the other factor. post * gate and
-// pre lie in shared memory behind the ring: read from the caller's buffers for
-// every token they would be as many bytes as its rows.
-template <typename T, int kPer>
-__global__ void __launch_bounds__(kStreamThreads, 1) unpermute_norm_backward_stream_kernel(
-    const UnpermuteNorm in, const Stream st, const UnpermuteNormGrads g, float* partial,
-    unsigned* err) {
-  using namespace sm100;
-  extern __shared__ __align__(16) char ring[];
-  __shared__ StreamSmem s;
-  const bool post = in.post_gamma != nullptr, pre = in.pre_gamma != nullptr;
-  const bool has_dro = g.d_residual_out != nullptr;
-  float* pg = reinterpret_cast<float*>(ring + st.stages * st.teams * st.sources * st.stride);
-  float* pr = pg + st.padded;
-  for (int c = threadIdx.x; c < st.padded; c += blockDim.x) {
-    column_factors<1>(in, c, pg + c, pr + c);
-  }
-  stream_setup(st, s);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (threadIdx.x >= st.team * st.teams) {
-    Sources src;
-    src.row[src.count++] = in.residual;
-    if (has_dro) src.row[src.count++] = g.d_residual_out;
-    if (pre) src.row[src.count++] = g.d_normed;
-    produce<T>(in, src, st, s, smem_u32(ring), err);
-    stream_end(s);
-    return;
-  }
-  const int team = threadIdx.x / st.team, tid = threadIdx.x % st.team;
-  const int team_warps = st.team >> 5, warp0 = team * team_warps;
-  const float per_col = 1.0f / static_cast<float>(in.output);
-  const int at_res = in.top_k, at_dro = in.top_k + 1, at_dn = in.top_k + 1 + (has_dro ? 1 : 0);
-  float s_dc[kElems], s_pre[kElems];  // sums over tokens of dr cn and dn rn
-#pragma unroll
-  for (int i = 0; i < kElems; ++i) s_dc[i] = s_pre[i] = 0.0f;
-  int stage = 0;
-  uint32_t phase = 0;
-  const long long step = static_cast<long long>(gridDim.x) * st.teams;
-  for (long long first = static_cast<long long>(blockIdx.x) * st.teams; first < in.tokens;
-       first += step) {
-    const bool ok = mbar_wait(&s.full[stage], phase, err, &s.failed);
-    if (!team_all(team, st.team, ok)) break;
-    const long long t = first + team;
-    if (t < in.tokens) {  // uniform over a team
-      const int* start = s.start[stage][team];
-      const float* weight = s.weight[stage][team];
-      // Sums of the team's warps are kept as parts[which][warp][j].
-      auto part = [&](float v, int which, int j) {
-        v = warp_sum(v);
-        if (lane == 0) s.parts[which][warp][j] = v;
-      };
-      auto total = [&](int which, int j) {
-        float sum = 0.0f;
-        for (int w = 0; w < team_warps; ++w) sum += s.parts[which][warp0 + w][j];
-        return sum;
-      };
-      // <x, y_k> of this thread's columns.
-      auto route_dot = [&](const float (&x)[kElems], int k) {
-        float d = 0.0f;
-        if (start[k] >= 0) {
-#pragma unroll
-          for (int q = 0; q < kElems / kPer; ++q) {
-            const int col = (q * st.team + tid) * kPer;
-            if (col < in.output) {
-              float v[kPer];
-              staged_cols<T, kPer>(ring + start[k] + col * sizeof(T), v);
-#pragma unroll
-              for (int i = 0; i < kPer; ++i) d = fmaf(x[q * kPer + i], v[i], d);
-            }
-          }
-        }
-        return d;
-      };
-      const float i1 = post ? __ldg(g.inv_rms + 2 * t) : 1.0f;
-      const float i2 = pre ? __ldg(g.inv_rms + 2 * t + 1) : 0.0f;
-      float c[kElems];  // cn
-      staged_combine<T, kPer>(in, st, ring, start, weight, tid, c);
-#pragma unroll
-      for (int i = 0; i < kElems; ++i) c[i] *= i1;
-      // rn of kPer columns, from the staged residual and cn.
-      auto normalised = [&](int q, int col, const float* f, float* rn) {
-        staged_cols<T, kPer>(ring + start[at_res] + col * sizeof(T), rn);
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-          rn[i] = fmaf(in.residual_scale, rn[i], c[q * kPer + i] * f[i]) * i2;
-        }
-      };
-      float dot = 0.0f;
-      if (pre) {
-#pragma unroll
-        for (int q = 0; q < kElems / kPer; ++q) {
-          const int col = (q * st.team + tid) * kPer;
-          if (col < in.output) {
-            float f[kPer], rn[kPer], v[kPer];
-            shared_cols<kPer>(pg + col, f);
-            normalised(q, col, f, rn);
-            staged_cols<T, kPer>(ring + start[at_dn] + col * sizeof(T), v);
-            shared_cols<kPer>(pr + col, f);
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) {
-              s_pre[q * kPer + i] = fmaf(v[i], rn[i], s_pre[q * kPer + i]);
-              dot = fmaf(v[i] * f[i], rn[i], dot);
-            }
-          }
-        }
-      }
-      part(dot, 0, 0);
-      if (post) {
-        for (int k = 0; k < in.top_k; ++k) part(route_dot(c, k), 0, k + 1);
-      }
-      team_sync(team, st.team);
-      const float m2 = total(0, 0) * per_col;
-      float dr[kElems];  // v1
-      dot = 0.0f;
-#pragma unroll
-      for (int q = 0; q < kElems / kPer; ++q) {
-        const int col = (q * st.team + tid) * kPer;
-        float* d = dr + q * kPer;
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) d[i] = 0.0f;
-        if (col < in.output) {
-          float f[kPer], out[kPer];
-          if (has_dro) staged_cols<T, kPer>(ring + start[at_dro] + col * sizeof(T), d);
-          shared_cols<kPer>(pg + col, f);
-          if (pre) {
-            float rn[kPer], v[kPer], a[kPer];
-            normalised(q, col, f, rn);
-            staged_cols<T, kPer>(ring + start[at_dn] + col * sizeof(T), v);
-            shared_cols<kPer>(pr + col, a);
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) d[i] += i2 * (v[i] * a[i] - rn[i] * m2);
-          }
-#pragma unroll
-          for (int i = 0; i < kPer; ++i) out[i] = in.residual_scale * d[i];
-          put_cols<T, kPer>(static_cast<T*>(g.d_residual) + t * in.output + col, out);
-#pragma unroll
-          for (int i = 0; i < kPer; ++i) {
-            s_dc[q * kPer + i] = fmaf(d[i], c[q * kPer + i], s_dc[q * kPer + i]);
-            d[i] *= f[i];
-            dot = fmaf(d[i], c[q * kPer + i], dot);
-          }
-        }
-      }
-      part(dot, 1, 0);
-      for (int k = 0; k < in.top_k; ++k) part(route_dot(dr, k), 1, k + 1);
-      team_sync(team, st.team);
-      const float m1 = post ? total(1, 0) * per_col : 0.0f;
-#pragma unroll
-      for (int i = 0; i < kElems; ++i) dr[i] = i1 * (dr[i] - c[i] * m1);
-      for (int k = 0; k < in.top_k; ++k) {
-        const bool there = start[k] >= 0;
-        if (tid == k) {
-          const float p = total(1, k + 1);
-          g.d_route_weights[t * in.top_k + k] =
-              !there ? 0.0f : (post ? i1 * (p - m1 * total(0, k + 1)) : p);
-        }
-        if (!there) continue;
-        const float w = weight[k];
-        T* row = static_cast<T*>(g.d_y_permuted) +
-                 static_cast<long long>(s.pos[stage][team][k]) * in.output;
-#pragma unroll
-        for (int q = 0; q < kElems / kPer; ++q) {
-          const int col = (q * st.team + tid) * kPer;
-          if (col < in.output) {
-            float out[kPer];
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) out[i] = w * dr[q * kPer + i];
-            put_cols<T, kPer>(row + col, out);
-          }
-        }
-      }
-    }
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&s.empty[stage]);
-    if (++stage == st.stages) {
-      stage = 0;
-      phase ^= 1u;
-    }
-  }
-  // This team's shares of the column sums: [block * teams + team][3][output].
-  float* p = partial + 3LL * (static_cast<long long>(blockIdx.x) * st.teams + team) * in.output;
-#pragma unroll
-  for (int q = 0; q < kElems / kPer; ++q) {
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int col = (q * st.team + tid) * kPer + i;
-      if (col < in.output) {
-        const float d = s_dc[q * kPer + i];
-        p[col] = in.gate != nullptr ? d * __ldg(in.gate + col) : d;
-        p[in.output + col] = post ? d * __ldg(in.post_gamma + col) : d;
-        p[2 * in.output + col] = s_pre[q * kPer + i];
-      }
-    }
-  }
-  stream_end(s);
-}
-
-// ---- the gradient for one or two routes per token ----------------------------------
-//
-// The same in one pass over the inputs and one reduction. With a = dro + i2 v
-// (v = dn pre) and f = post * gate:
+// The gradient, in one pass over a token's inputs and one reduction. With
+// a = dro + i2 v (v = dn pre) and f = post * gate:
 //   dr = a - i2 m2 rn,  v1 = f dr,  m2 = mean(v rn)
 //   P_k = <v1, y_k> = <f a, y_k> - i2 m2 <f rn, y_k>
-//   mean(v1 cn) = i1 sum_k w_k P_k / N,  Q_k = <cn, y_k> = i1 sum_j w_j <y_j, y_k>
-// so a token's eight sums are known together, before any of its results. Two
-// columns share an instruction (packed FP32 arithmetic, which rounds each half
-// as the plain instruction does).
+//   m1 = mean(v1 cn) = i1 sum_k w_k P_k / N
+//   dw_k = <dc, y_k> = i1 (P_k - m1 <cn, y_k>)
+// (without the norm of c: i1 = 1, m1 = 0), so a token's 1 + 3 top_k sums are
+// known together, before any of its results. The gradients of post and gate
+// are one column sum, of dr cn, times the other factor. post * gate and pre
+// lie in shared memory behind the ring: read from the caller's buffers for
+// every token they would be as many bytes as its rows. Two columns share an
+// instruction (packed FP32 arithmetic, which rounds each half as the plain
+// instruction does).
 
 struct F2 {
   unsigned long long v;
@@ -969,19 +781,13 @@ __device__ __forceinline__ float sum2(F2 a) {
   return lo + hi;
 }
 
-// Eight columns per thread: a token's c, a and rn and the thread's column sums
-// then stay in registers with sixteen warps per SM (sixteen columns spilled,
-// and eight warps leave too little to overlap).
-constexpr int kPairElems = 8;
-constexpr int kPairs = kPairElems / 2;
-
 // This thread's columns of a staged row in pairs, zero past the row's end.
-template <typename T, int kPer>
+template <typename T, int kPer, int kPairs>
 __device__ __forceinline__ void staged_row(const char* row, int output, int team, int tid,
                                            F2 (&v)[kPairs]) {
-  float f[kPairElems];
+  float f[2 * kPairs];
 #pragma unroll
-  for (int q = 0; q < kPairElems / kPer; ++q) {
+  for (int q = 0; q < 2 * kPairs / kPer; ++q) {
     const int col = (q * team + tid) * kPer;
     if (col < output) {
       staged_cols<T, kPer>(row + col * sizeof(T), f + q * kPer);
@@ -994,12 +800,12 @@ __device__ __forceinline__ void staged_row(const char* row, int output, int team
   for (int i = 0; i < kPairs; ++i) v[i] = f2(f[2 * i], f[2 * i + 1]);
 }
 
-template <int kPer>
+template <int kPer, int kPairs>
 __device__ __forceinline__ void shared_row(const float* row, int output, int team, int tid,
                                            F2 (&v)[kPairs]) {
-  float f[kPairElems];
+  float f[2 * kPairs];
 #pragma unroll
-  for (int q = 0; q < kPairElems / kPer; ++q) {
+  for (int q = 0; q < 2 * kPairs / kPer; ++q) {
     const int col = (q * team + tid) * kPer;
     if (col < output) {
       shared_cols<kPer>(row + col, f + q * kPer);
@@ -1012,14 +818,14 @@ __device__ __forceinline__ void shared_row(const float* row, int output, int tea
   for (int i = 0; i < kPairs; ++i) v[i] = f2(f[2 * i], f[2 * i + 1]);
 }
 
-template <typename T, int kPer>
+template <typename T, int kPer, int kPairs>
 __device__ __forceinline__ void put_row(T* row, int output, int team, int tid,
                                         const F2 (&v)[kPairs]) {
-  float f[kPairElems];
+  float f[2 * kPairs];
 #pragma unroll
   for (int i = 0; i < kPairs; ++i) split(v[i], f[2 * i], f[2 * i + 1]);
 #pragma unroll
-  for (int q = 0; q < kPairElems / kPer; ++q) {
+  for (int q = 0; q < 2 * kPairs / kPer; ++q) {
     const int col = (q * team + tid) * kPer;
     if (col < output) put_cols<T, kPer>(row + col, f + q * kPer);
   }
@@ -1046,200 +852,253 @@ __device__ __forceinline__ float warp_sum8(const float (&v)[8]) {
   return c + __shfl_xor_sync(0xffffffffu, c, 1);
 }
 
-template <typename T, int kPer>
-__global__ void __launch_bounds__(kStreamThreads, 1) unpermute_norm_backward_pair_kernel(
+template <typename T, int kPer, int kCols, bool kTwo>
+__global__ void __launch_bounds__(kStreamThreads, 1) unpermute_norm_backward_stream_kernel(
     const UnpermuteNorm in, const Stream st, const UnpermuteNormGrads g, float* partial,
     unsigned* err) {
   using namespace sm100;
-  extern __shared__ __align__(16) char ring[];
+  constexpr int kPairs = kCols / 2;
+  constexpr int kSets = kTwo ? 1 : kStreamTopK / 2;
+  extern __shared__ __align__(16) char rings[];
   __shared__ StreamSmem s;
-  __shared__ float sums[2][kMaxTeams][8];  // of each warp, by parity of the token
+  // Of each warp, by parity of the token: for two routes at a time
+  // <f a, y>, <f rn, y>, <cn, y> of the first, the same of the second, and
+  // (with the first two) <v, rn>.
+  __shared__ float sums[2][kMaxTeams][kSets][8];
   const bool post = in.post_gamma != nullptr, pre = in.pre_gamma != nullptr;
   const bool has_dro = g.d_residual_out != nullptr;
-  float* pg = reinterpret_cast<float*>(ring + st.stages * st.teams * st.sources * st.stride);
-  float* pr = pg + st.padded;
+  const int n = in.output;
+  const int ring_size = st.stages * st.sources * st.stride;
+  float* pg = reinterpret_cast<float*>(rings + st.teams * ring_size);
+  float* shared_pre = pg + st.padded;
   for (int c = threadIdx.x; c < st.padded; c += blockDim.x) {
-    column_factors<1>(in, c, pg + c, pr + c);
+    float f, p;
+    column_factors<1>(in, c, &f, &p);
+    pg[c] = f;
+    if (st.factors > 1) shared_pre[c] = p;
   }
-  stream_setup(st, s);
+  const float* pr = st.factors > 1 ? shared_pre : in.pre_gamma;
+  stream_setup(st, in.top_k, s);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (threadIdx.x >= st.team * st.teams) {
-    Sources src;
-    src.row[src.count++] = in.residual;
-    if (has_dro) src.row[src.count++] = g.d_residual_out;
-    if (pre) src.row[src.count++] = g.d_normed;
-    produce<T>(in, src, st, s, smem_u32(ring), err);
-    stream_end(s);
-    return;
-  }
   const int team = threadIdx.x / st.team, tid = threadIdx.x % st.team;
   const int team_warps = st.team >> 5, warp0 = team * team_warps;
-  const int n = in.output;
+  const char* ring = rings + team * ring_size;
   const float per_col = 1.0f / static_cast<float>(n);
   const int at_res = in.top_k, at_dro = in.top_k + 1, at_dn = in.top_k + 1 + (has_dro ? 1 : 0);
   F2 s_dc[kPairs], s_pre[kPairs];  // sums over tokens of dr cn and dn rn
 #pragma unroll
   for (int i = 0; i < kPairs; ++i) s_dc[i] = s_pre[i] = f2(0.0f);
-  int stage = 0, parity = 0;
-  uint32_t phase = 0;
-  const long long step = static_cast<long long>(gridDim.x) * st.teams;
-  for (long long first = static_cast<long long>(blockIdx.x) * st.teams; first < in.tokens;
-       first += step) {
-    const bool ok = mbar_wait(&s.full[stage], phase, err, &s.failed);
-    if (!team_all(team, st.team, ok)) break;
-    const long long t = first + team;
-    if (t < in.tokens) {  // uniform over a team
-      const int* start = s.start[stage][team];
-      const bool there0 = start[0] >= 0, there1 = in.top_k > 1 && start[1] >= 0;
-      const float w0 = there0 ? s.weight[stage][team][0] : 0.0f;
-      const float w1 = there1 ? s.weight[stage][team][1] : 0.0f;
-      const float i1 = post ? __ldg(g.inv_rms + 2 * t) : 1.0f;
-      const float i2 = pre ? __ldg(g.inv_rms + 2 * t + 1) : 0.0f;
-      F2 c[kPairs], a[kPairs], rn[kPairs];
-      float v8[8];  // <v, rn>, <f a, y0>, <f a, y1>, <f rn, y0>, <f rn, y1>, <y0, y0>, ...
-      {
-        F2 y0[kPairs], y1[kPairs], x[kPairs], f[kPairs], sum[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) sum[j] = f2(0.0f);
+  Sources src;
+  src.row[0] = in.residual;
+  src.row[1] = has_dro ? g.d_residual_out : g.d_normed;
+  src.row[2] = g.d_normed;
+  int parity = 0;
+  TokenLoop<T, kPer * sizeof(T) == 16> loop(in, st, s, src, smem_u32(ring), team, err);
+  while (loop.step()) {
+    const long long t = loop.t;
+    const int* start = s.start[team][loop.stage];
+    const float* weight = s.weight[team][loop.stage];
+    const float i1 = post ? __ldg(g.inv_rms + 2 * t) : 1.0f;
+    const float i2 = pre ? __ldg(g.inv_rms + 2 * t + 1) : 0.0f;
+    const F2 i12 = f2(i1), i22 = f2(i2), scale = f2(in.residual_scale);
+    F2 c[kPairs], a[kPairs], rn[kPairs];
+    F2 y0[kTwo ? kPairs : 1], y1[kTwo ? kPairs : 1];  // the routes' rows, if there are two at most
+    F2 f[kPairs];                                     // post * gate
+    F2 dot = f2(0.0f);                                // <v, rn>
+    auto route_row = [&](int k, F2 (&y)[kPairs]) {
+      staged_row<T, kPer>(ring + start[k], n, st.team, tid, y);
+    };
+    {
+      F2 x[kPairs];
+      if constexpr (kTwo) {
+        const bool there0 = start[0] >= 0, there1 = in.top_k > 1 && start[1] >= 0;
 #pragma unroll
         for (int i = 0; i < kPairs; ++i) y0[i] = y1[i] = f2(0.0f);
-        if (there0) staged_row<T, kPer>(ring + start[0], n, st.team, tid, y0);
-        if (there1) staged_row<T, kPer>(ring + start[1], n, st.team, tid, y1);
-        shared_row<kPer>(pg, n, st.team, tid, f);
-        staged_row<T, kPer>(ring + start[at_res], n, st.team, tid, x);
-        const F2 w02 = f2(w0), w12 = f2(w1), i12 = f2(i1), i22 = f2(i2);
-        const F2 scale = f2(in.residual_scale);
+        if (there0) route_row(0, y0);
+        if (there1) route_row(1, y1);
+        const F2 w0 = f2(there0 ? weight[0] : 0.0f), w1 = f2(there1 ? weight[1] : 0.0f);
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) c[i] = fma2(w1, y1[i], mul2(w0, y0[i]));
+      } else {
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) c[i] = f2(0.0f);
+        for (int k = 0; k < in.top_k; ++k) {
+          if (start[k] < 0) continue;
+          route_row(k, x);
+          const F2 w = f2(weight[k]);
+#pragma unroll
+          for (int i = 0; i < kPairs; ++i) c[i] = fma2(w, x[i], c[i]);
+        }
+      }
+      shared_row<kPer>(pg, n, st.team, tid, f);
+      staged_row<T, kPer>(ring + start[at_res], n, st.team, tid, x);
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) {
+        c[i] = mul2(i12, c[i]);
+        rn[i] = mul2(i22, fma2(scale, x[i], mul2(c[i], f[i])));
+      }
+      if (has_dro) {
+        staged_row<T, kPer>(ring + start[at_dro], n, st.team, tid, a);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) a[i] = f2(0.0f);
+      }
+      if (pre) {
+        F2 p[kPairs];
+        staged_row<T, kPer>(ring + start[at_dn], n, st.team, tid, x);
+        shared_row<kPer>(pr, n, st.team, tid, p);
 #pragma unroll
         for (int i = 0; i < kPairs; ++i) {
-          c[i] = mul2(i12, fma2(w12, y1[i], mul2(w02, y0[i])));
-          rn[i] = mul2(i22, fma2(scale, x[i], mul2(c[i], f[i])));
+          s_pre[i] = fma2(x[i], rn[i], s_pre[i]);
+          const F2 v = mul2(x[i], p[i]);
+          dot = fma2(v, rn[i], dot);
+          a[i] = fma2(i22, v, a[i]);
         }
-        if (has_dro) {
-          staged_row<T, kPer>(ring + start[at_dro], n, st.team, tid, a);
-        } else {
+      }
+    }
+    // The sums of two routes at a time, reduced over the warp.
+    float mine = 0.0f;
+    auto reduce_pair = [&](int k) {
+      float v8[8];
 #pragma unroll
-          for (int i = 0; i < kPairs; ++i) a[i] = f2(0.0f);
-        }
-        if (pre) {
-          F2 p[kPairs];
-          staged_row<T, kPer>(ring + start[at_dn], n, st.team, tid, x);
-          shared_row<kPer>(pr, n, st.team, tid, p);
+      for (int h = 0; h < 2; ++h) {
+        F2 fa = f2(0.0f), fr = f2(0.0f), cy = f2(0.0f);
+        if (kTwo || (k + h < in.top_k && start[k + h] >= 0)) {
+          F2 y[kPairs];
+          if constexpr (kTwo) {
+#pragma unroll
+            for (int i = 0; i < kPairs; ++i) y[i] = h == 0 ? y0[i] : y1[i];
+          } else {
+            route_row(k + h, y);
+          }
 #pragma unroll
           for (int i = 0; i < kPairs; ++i) {
-            s_pre[i] = fma2(x[i], rn[i], s_pre[i]);
-            const F2 v = mul2(x[i], p[i]);
-            sum[0] = fma2(v, rn[i], sum[0]);
-            a[i] = fma2(i22, v, a[i]);
+            cy = fma2(c[i], y[i], cy);
+            y[i] = mul2(f[i], y[i]);
+            fa = fma2(a[i], y[i], fa);
+            fr = fma2(rn[i], y[i], fr);
           }
         }
-#pragma unroll
-        for (int i = 0; i < kPairs; ++i) {
-          const F2 fa = mul2(f[i], a[i]), fr = mul2(f[i], rn[i]);
-          sum[1] = fma2(fa, y0[i], sum[1]);
-          sum[2] = fma2(fa, y1[i], sum[2]);
-          sum[3] = fma2(fr, y0[i], sum[3]);
-          sum[4] = fma2(fr, y1[i], sum[4]);
-          sum[5] = fma2(y0[i], y0[i], sum[5]);
-          sum[6] = fma2(y0[i], y1[i], sum[6]);
-          sum[7] = fma2(y1[i], y1[i], sum[7]);
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v8[j] = sum2(sum[j]);
+        v8[3 * h] = sum2(fa);
+        v8[3 * h + 1] = sum2(fr);
+        v8[3 * h + 2] = sum2(cy);
       }
-      // The team's sums: lane l of every warp ends with the sum l / 4.
-      float mine = warp_sum8(v8);
-      if (team_warps > 1) {
-        if ((lane & 3) == 0) sums[parity][warp][lane >> 2] = mine;
-        team_sync(team, st.team);
-        mine = 0.0f;
-        for (int w = lane & 3; w < team_warps; w += 4) mine += sums[parity][warp0 + w][lane >> 2];
-        mine += __shfl_xor_sync(0xffffffffu, mine, 1);
-        mine += __shfl_xor_sync(0xffffffffu, mine, 2);
-        parity ^= 1;
+      v8[6] = k == 0 ? sum2(dot) : 0.0f;
+      v8[7] = 0.0f;
+      mine = warp_sum8(v8);
+      if ((team_warps > 1 || !kTwo) && (lane & 3) == 0) {
+        sums[parity][warp][k >> 1][lane >> 2] = mine;
       }
-      auto total = [&](int j) { return __shfl_sync(0xffffffffu, mine, 4 * j); };
-      const float im2 = i2 * (total(0) * per_col);
-      const float p0 = total(1) - im2 * total(3), p1 = total(2) - im2 * total(4);
-      const float g00 = total(5), g01 = total(6), g11 = total(7);
-      const float m1 = post ? i1 * (w0 * p0 + w1 * p1) * per_col : 0.0f;
-      if (tid == 0) {
-        const float q0 = i1 * (w0 * g00 + w1 * g01), q1 = i1 * (w0 * g01 + w1 * g11);
-        float* dw = g.d_route_weights + t * in.top_k;
-        dw[0] = there0 ? i1 * (p0 - m1 * q0) : 0.0f;
-        if (in.top_k > 1) dw[1] = there1 ? i1 * (p1 - m1 * q1) : 0.0f;
+    };
+    if constexpr (kTwo) {
+      reduce_pair(0);
+    } else {
+      for (int k = 0; k < in.top_k; k += 2) reduce_pair(k);
+    }
+    // Over the team: lane l ends with sum l / 4 of routes k and k + 1.
+    team_sync(team, st.team);
+    loop.refill();
+    auto team_sums = [&](int k) {
+      if (kTwo && team_warps == 1) return mine;
+      float v = 0.0f;
+      for (int w = lane & 3; w < team_warps; w += 4) {
+        v += sums[parity][warp0 + w][k >> 1][lane >> 2];
       }
-      {
-        F2 x[kPairs];
-        const F2 nim2 = f2(-im2), scale = f2(in.residual_scale);
+      v += __shfl_xor_sync(0xffffffffu, v, 1);
+      return v + __shfl_xor_sync(0xffffffffu, v, 2);
+    };
+    auto sum_of = [&](float v, int j) { return __shfl_sync(0xffffffffu, v, 4 * j); };
+    const float sums01 = team_sums(0);
+    const float im2 = i2 * (sum_of(sums01, 6) * per_col);
+    auto p_of = [&](float v, int h) { return sum_of(v, 3 * h) - im2 * sum_of(v, 3 * h + 1); };
+    float m1 = 0.0f;
+    for (int k = 0; k < (kTwo ? 1 : in.top_k); k += 2) {
+      const float v = k == 0 ? sums01 : team_sums(k);
+      const float p0 = p_of(v, 0), p1 = p_of(v, 1);
+      if (start[k] >= 0) m1 = fmaf(weight[k], p0, m1);
+      if (k + 1 < in.top_k && start[k + 1] >= 0) m1 = fmaf(weight[k + 1], p1, m1);
+    }
+    m1 = post ? i1 * m1 * per_col : 0.0f;
+    for (int k = 0; k < (kTwo ? 1 : in.top_k); k += 2) {
+      const float v = k == 0 ? sums01 : team_sums(k);
 #pragma unroll
-        for (int i = 0; i < kPairs; ++i) {
-          a[i] = fma2(nim2, rn[i], a[i]);  // dr
-          s_dc[i] = fma2(a[i], c[i], s_dc[i]);
-          x[i] = mul2(scale, a[i]);
-        }
-        put_row<T, kPer>(static_cast<T*>(g.d_residual) + t * n, n, st.team, tid, x);
-        shared_row<kPer>(pg, n, st.team, tid, x);
-        const F2 i12 = f2(i1), nm1 = f2(-m1);
-#pragma unroll
-        for (int i = 0; i < kPairs; ++i) {
-          a[i] = mul2(i12, fma2(nm1, c[i], mul2(x[i], a[i])));  // dc
-        }
-        T* rows = static_cast<T*>(g.d_y_permuted);
-        if (there0) {
-          const F2 w = f2(w0);
-#pragma unroll
-          for (int i = 0; i < kPairs; ++i) x[i] = mul2(w, a[i]);
-          put_row<T, kPer>(rows + static_cast<long long>(s.pos[stage][team][0]) * n, n, st.team,
-                           tid, x);
-        }
-        if (there1) {
-          const F2 w = f2(w1);
-#pragma unroll
-          for (int i = 0; i < kPairs; ++i) x[i] = mul2(w, a[i]);
-          put_row<T, kPer>(rows + static_cast<long long>(s.pos[stage][team][1]) * n, n, st.team,
-                           tid, x);
+      for (int h = 0; h < 2; ++h) {
+        const float d = i1 * (p_of(v, h) - m1 * sum_of(v, 3 * h + 2));
+        if (tid == 0 && k + h < in.top_k) {
+          g.d_route_weights[t * in.top_k + k + h] = start[k + h] >= 0 ? d : 0.0f;
         }
       }
     }
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&s.empty[stage]);
-    if (++stage == st.stages) {
-      stage = 0;
-      phase ^= 1u;
+    parity ^= 1;
+    F2 x[kPairs];
+    const F2 nim2 = f2(-im2), nm1 = f2(-m1);
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) {
+      a[i] = fma2(nim2, rn[i], a[i]);  // dr
+      s_dc[i] = fma2(a[i], c[i], s_dc[i]);
+      x[i] = mul2(scale, a[i]);
+    }
+    put_row<T, kPer>(static_cast<T*>(g.d_residual) + t * n, n, st.team, tid, x);
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) {
+      a[i] = mul2(i12, fma2(nm1, c[i], mul2(f[i], a[i])));  // dc
+    }
+    for (int k = 0; k < in.top_k; ++k) {
+      if (start[k] < 0) continue;
+      const F2 w = f2(weight[k]);
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) x[i] = mul2(w, a[i]);
+      put_row<T, kPer>(static_cast<T*>(g.d_y_permuted) +
+                           static_cast<long long>(s.pos[team][loop.stage][k]) * n,
+                       n, st.team, tid, x);
     }
   }
-  // This team's shares of the column sums: [block * teams + team][3][output].
-  float* p = partial + 3LL * (static_cast<long long>(blockIdx.x) * st.teams + team) * n;
+  // The block's shares of the column sums, [block][3][output]: its teams' add up
+  // in the rings, of which every load has been used by now.
+  __syncthreads();
+  float* shared = reinterpret_cast<float*>(rings);
 #pragma unroll
-  for (int i = 0; i < kPairElems; ++i) {
+  for (int i = 0; i < kCols; ++i) {
     const int col = ((i / kPer) * st.team + tid) * kPer + i % kPer;
     if (col < n) {
       float lo, hi;
       split(s_dc[i / 2], lo, hi);
-      const float d = i % 2 ? hi : lo;
+      shared[(2 * team) * n + col] = i % 2 ? hi : lo;
       split(s_pre[i / 2], lo, hi);
-      p[col] = in.gate != nullptr ? d * __ldg(in.gate + col) : d;
-      p[n + col] = post ? d * __ldg(in.post_gamma + col) : d;
-      p[2 * n + col] = i % 2 ? hi : lo;
+      shared[(2 * team + 1) * n + col] = i % 2 ? hi : lo;
     }
+  }
+  __syncthreads();
+  float* p = partial + 3LL * blockIdx.x * n;
+  for (int col = threadIdx.x; col < n; col += blockDim.x) {
+    float d = 0.0f, e = 0.0f;
+    for (int q = 0; q < st.teams; ++q) {
+      d += shared[(2 * q) * n + col];
+      e += shared[(2 * q + 1) * n + col];
+    }
+    p[col] = in.gate != nullptr ? d * __ldg(in.gate + col) : d;
+    p[n + col] = post ? d * __ldg(in.post_gamma + col) : d;
+    p[2 * n + col] = e;
   }
   stream_end(s);
 }
 
-constexpr int kSumThreads = 256;
 constexpr int kSumCols = 32;
+constexpr int kSumGroups = 32;
 
-__global__ void __launch_bounds__(kSumThreads) column_sums_kernel(
+// Adds the blocks' shares in a fixed order: a warp of columns, 32 blocks at a time.
+__global__ void __launch_bounds__(kSumCols* kSumGroups) column_sums_kernel(
     const float* __restrict__ partial, int blocks, int output, float* d_post, float* d_gate,
     float* d_pre) {
-  __shared__ float parts[kSumThreads / kSumCols][kSumCols];
+  __shared__ float parts[kSumGroups][kSumCols];
   float* out = blockIdx.y == 0 ? d_post : (blockIdx.y == 1 ? d_gate : d_pre);
   if (out == nullptr) return;
   const int lane = threadIdx.x % kSumCols, group = threadIdx.x / kSumCols;
   const int col = blockIdx.x * kSumCols + lane;
   float sum = 0.0f;
   if (col < output) {
-    for (int b = group; b < blocks; b += kSumThreads / kSumCols) {
+#pragma unroll 8
+    for (int b = group; b < blocks; b += kSumGroups) {
       sum += __ldg(partial + (3LL * b + blockIdx.y) * output + col);
     }
   }
@@ -1247,7 +1106,7 @@ __global__ void __launch_bounds__(kSumThreads) column_sums_kernel(
   __syncthreads();
   if (group == 0 && col < output) {
 #pragma unroll
-    for (int i = 1; i < kSumThreads / kSumCols; ++i) sum += parts[i][lane];
+    for (int i = 1; i < kSumGroups; ++i) sum += parts[i][lane];
     out[col] = sum;
   }
 }
@@ -1260,39 +1119,45 @@ int row_threads(int output, int per) {
 }
 
 // The streamed form's layout, or blocks = 0 where the plain one runs: few
-// tokens (the ring has to fill before it pays: two stages per SM), more routes
-// than a stage keeps track of, or rows of which two stages do not fit.
+// tokens (the rings have to fill before they pay: two tokens per team), more
+// routes than a ring keeps track of, or rows of which two stages do not fit.
 Stream stream_plan(int tokens, int top_k, int output, int extra_rows, bool gradient, int elems,
                    std::size_t size) {
   Stream st;
-  if (top_k > kStreamTopK || output > kWorkers * elems) return st;
+  if (top_k > kStreamTopK || output > kStreamThreads * elems) return st;
   st.team = row_threads(output, elems);
-  st.teams = kWorkers / st.team;
+  st.teams = kStreamThreads / st.team;
   st.sources = top_k + extra_rows;
-  if (st.teams * st.sources > 32 * kRounds) return st;
   // A row's granules: up to 15 bytes before and after it.
   st.stride = static_cast<int>((output * size + 15) / 16 * 16 + 16);
-  if (gradient) st.padded = (output + 3) / 4 * 4;
-  for (;; st.teams /= 2) {  // two stages have to fit: halve the teams until they do
+  if (gradient) {
+    st.padded = (output + 3) / 4 * 4;
+    st.factors = 2;
+  }
+  // Two stages have to fit: with pre left in its own buffer, or with half the
+  // teams, if need be.
+  for (;;) {
     const std::size_t stage = static_cast<std::size_t>(st.teams) * st.sources * st.stride;
-    st.stages = static_cast<int>((kRingBytes - 8 * st.padded) / stage);
-    if (st.stages >= 2 || st.teams == 1) break;
+    st.stages = static_cast<int>((kRingBytes - 4 * st.factors * st.padded) / stage);
+    if (st.stages >= 2) break;
+    if (st.teams > 1) st.teams /= 2;
+    else if (st.factors == 2) st.factors = 1;
+    else return st;
   }
   if (st.stages > kMaxStages) st.stages = kMaxStages;
-  const int fill = 2 * kNumSms * st.teams;
-  if (st.stages >= 2 && tokens >= fill) st.blocks = kNumSms;
+  if (tokens >= 2 * kNumSms * st.teams) st.blocks = kNumSms;
   return st;
 }
 
 std::size_t ring_bytes(const Stream& st) {
-  return static_cast<std::size_t>(st.stages) * st.teams * st.sources * st.stride + 8 * st.padded;
+  return static_cast<std::size_t>(st.stages) * st.teams * st.sources * st.stride +
+         4 * st.factors * st.padded;
 }
 
-// Columns per thread of the streamed gradient: one or two routes per token have
-// a kernel of their own, up to the width its teams cover.
-int gradient_elems(int top_k, int output) {
-  return top_k <= 2 && output <= kWorkers * kPairElems ? kPairElems : kElems;
-}
+// Columns per thread of the streamed gradient: eight, so that a token's c, a, rn
+// and the thread's column sums stay in registers with sixteen warps per SM;
+// rows wider than that covers take sixteen.
+int gradient_elems(int output) { return output <= kStreamThreads * 8 ? 8 : 16; }
 
 // One resident wave of the plain gradient kernel (about 128 registers per
 // thread).
@@ -1358,7 +1223,7 @@ cudaError_t forward(const UnpermuteNorm& in, void* residual_out, void* normed, f
 cudaError_t column_sums(const float* workspace, int parts, int output,
                         const UnpermuteNormGrads& g, cudaStream_t stream) {
   if (g.d_post_gamma != nullptr || g.d_gate != nullptr || g.d_pre_gamma != nullptr) {
-    column_sums_kernel<<<dim3(ceil_div(output, kSumCols), 3), kSumThreads, 0, stream>>>(
+    column_sums_kernel<<<dim3(ceil_div(output, kSumCols), 3), kSumCols * kSumGroups, 0, stream>>>(
         workspace, parts, output, g.d_post_gamma, g.d_gate, g.d_pre_gamma);
     note_launch();
   }
@@ -1384,7 +1249,7 @@ cudaError_t forward_stream(const UnpermuteNorm& in, const Stream& st, void* resi
                            void* normed, float* inv_rms, cudaStream_t stream) {
   constexpr auto kernel = unpermute_norm_stream_kernel<T, kPer>;
   if (!allow_ring<kernel>()) return cudaErrorNotSupported;
-  kernel<<<st.blocks, st.team * st.teams + 32, ring_bytes(st), stream>>>(
+  kernel<<<st.blocks, st.team * st.teams, ring_bytes(st), stream>>>(
       in, st, static_cast<T*>(residual_out), static_cast<T*>(normed), inv_rms,
       device_error_word());
   note_launch();
@@ -1394,16 +1259,20 @@ cudaError_t forward_stream(const UnpermuteNorm& in, const Stream& st, void* resi
 template <typename T, int kPer>
 cudaError_t backward_stream(const UnpermuteNorm& in, const Stream& st, const UnpermuteNormGrads& g,
                             float* workspace, cudaStream_t stream) {
-  constexpr auto any = unpermute_norm_backward_stream_kernel<T, kPer>;
-  constexpr auto pair = unpermute_norm_backward_pair_kernel<T, kPer>;
-  const bool two = gradient_elems(in.top_k, in.output) == kPairElems;
-  if (!(two ? allow_ring<pair>() : allow_ring<any>())) return cudaErrorNotSupported;
-  (two ? pair : any)<<<st.blocks, st.team * st.teams + 32, ring_bytes(st), stream>>>(
-      in, st, g, workspace, device_error_word());
+  constexpr auto narrow2 = unpermute_norm_backward_stream_kernel<T, kPer, 8, true>;
+  constexpr auto narrow = unpermute_norm_backward_stream_kernel<T, kPer, 8, false>;
+  constexpr auto wide = unpermute_norm_backward_stream_kernel<T, kPer, 16, false>;
+  const bool eight = gradient_elems(in.output) == 8, two = in.top_k <= 2;
+  if (!(eight ? (two ? allow_ring<narrow2>() : allow_ring<narrow>()) : allow_ring<wide>())) {
+    return cudaErrorNotSupported;
+  }
+  auto* kernel = eight ? (two ? narrow2 : narrow) : wide;
+  kernel<<<st.blocks, st.team * st.teams, ring_bytes(st), stream>>>(in, st, g, workspace,
+                                                                    device_error_word());
   note_launch();
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  return column_sums(workspace, st.blocks * st.teams, in.output, g, stream);
+  return column_sums(workspace, st.blocks, in.output, g, stream);
 }
 
 }  // namespace
@@ -1413,7 +1282,11 @@ cudaError_t launch_unpermute_norm(const UnpermuteNorm& in, void* residual_out, v
   const Stream st = stream_plan(in.tokens, in.top_k, in.output, 1, false, kElems, dtype_bytes(dtype));
   const int per = stream_columns(in.output, dtype);
   const std::size_t unit = per * dtype_bytes(dtype);
-  if (st.blocks > 0 && aligned_to(in.y_permuted, 16) && aligned_to(in.residual, 16) &&
+  // Short aligned rows are a warp's work with one load per thread and row; the
+  // ring only delays them (32768 tokens, N=256: FP32 35 against 50 us streamed,
+  // N=512: 66 against 62).
+  const bool direct = in.output <= 256 && per > 2;
+  if (!direct && st.blocks > 0 && aligned_to(in.y_permuted, 16) && aligned_to(in.residual, 16) &&
       aligned_gammas(in, per) && aligned_to(residual_out, unit) && aligned_to(normed, unit)) {
     if (dtype == Dtype::kBf16) {
       auto* run = per == 8   ? forward_stream<__nv_bfloat16, 8>
@@ -1436,17 +1309,9 @@ cudaError_t launch_unpermute_norm(const UnpermuteNorm& in, void* residual_out, v
 
 std::size_t unpermute_norm_backward_workspace_bytes(int tokens, int output) {
   // Shares of the column sums: of the plain form's blocks or the streamed
-  // form's teams, whichever is more.
+  // form's, whichever are more.
   std::size_t parts = static_cast<std::size_t>(backward_blocks(tokens, output));
-  const int elems = gradient_elems(1, output);
-  if (output <= kWorkers * kElems) {
-    const std::size_t teams = static_cast<std::size_t>(kNumSms) *
-                              (kWorkers / row_threads(output, kElems));
-    const std::size_t narrow = static_cast<std::size_t>(kNumSms) *
-                               (kWorkers / row_threads(output, elems));
-    const std::size_t most = teams > narrow ? teams : narrow;
-    if (most > parts && tokens >= static_cast<long long>(narrow)) parts = most;
-  }
+  if (parts < kNumSms && tokens >= kNumSms) parts = kNumSms;
   return 12 * parts * output;
 }
 
@@ -1454,7 +1319,7 @@ cudaError_t launch_unpermute_norm_backward(const UnpermuteNorm& in, const Unperm
                                            float* workspace, Dtype dtype, cudaStream_t stream) {
   const int extra = 1 + (g.d_residual_out != nullptr) + (in.pre_gamma != nullptr);
   const Stream st = stream_plan(in.tokens, in.top_k, in.output, extra, true,
-                                gradient_elems(in.top_k, in.output), dtype_bytes(dtype));
+                                gradient_elems(in.output), dtype_bytes(dtype));
   const int per = stream_columns(in.output, dtype);
   const std::size_t unit = per * dtype_bytes(dtype);
   if (st.blocks > 0 && aligned_to(in.y_permuted, 16) && aligned_to(in.residual, 16) &&
