@@ -167,6 +167,19 @@ cudaError_t launch_gated_pointwise_backward(const float* gate_up, const void* dh
                                             int output, int ld, int parts, Activation activation,
                                             Dtype dtype, cudaStream_t stream);
 
+// The same with dg and du in FP32, [rows][output] each, for the few-row forms.
+cudaError_t launch_gated_pointwise_backward_f32(const float* gate_up, const void* dh, float* dg,
+                                                float* du, int rows, int output,
+                                                Activation activation, Dtype dtype,
+                                                cudaStream_t stream);
+cudaError_t launch_gated_few_dx(const float* dg, const float* du, const void* wg, const void* wu,
+                                const int32_t* offsets, void* dx, int rows, int experts,
+                                int hidden, int output, Dtype dtype, cudaStream_t stream);
+cudaError_t launch_gated_few_dw(const void* x, const float* dg, const float* du,
+                                const int32_t* offsets, void* dwg, void* dwu, int rows,
+                                int experts, int hidden, int output, Dtype dtype,
+                                cudaStream_t stream);
+
 // ---- int8.cu -------------------------------------------------------------------
 
 cudaError_t launch_quantize_rows_int8(const void* x, int8_t* xq, float* x_scale, int rows,

@@ -175,6 +175,21 @@ __device__ __forceinline__ void few_rows(const T* __restrict__ x, const T* __res
   }
 }
 
+// The expert whose segment holds `row` (the block's threads look at all of them),
+// or `experts`.
+__device__ __forceinline__ int expert_of(const int32_t* __restrict__ offsets, int row, int rows,
+                                         int experts) {
+  __shared__ int owner;
+  if (threadIdx.x == 0) owner = experts;
+  __syncthreads();
+  for (int e = threadIdx.x; e < experts; e += kFewThreads) {
+    const int2 s = segment(offsets, e, rows);
+    if (s.x <= row && row < s.y) atomicMin(&owner, e);
+  }
+  __syncthreads();
+  return owner;
+}
+
 // kR rows of an expert share a reading of its weights. One row at a time needs
 // half the registers, so twice the loads are in flight.
 template <typename T, int kVec, int kR>
@@ -182,17 +197,9 @@ __global__ void __launch_bounds__(kFewThreads, kR == 1 ? 4 : 2) gated_few_kernel
     const T* __restrict__ x, const T* __restrict__ wg, const T* __restrict__ wu,
     const int32_t* __restrict__ offsets, T* __restrict__ h, float* __restrict__ gate_up, int rows,
     int experts, int hidden, int output, int activation, int split) {
-  __shared__ int owner;
   __shared__ FewSmem smem;
-  if (threadIdx.x == 0) owner = experts;
-  __syncthreads();
   const int row = blockIdx.y;
-  for (int e = threadIdx.x; e < experts; e += kFewThreads) {
-    const int2 s = segment(offsets, e, rows);
-    if (s.x <= row && row < s.y) atomicMin(&owner, e);
-  }
-  __syncthreads();
-  const int e = owner;
+  const int e = expert_of(offsets, row, rows, experts);
   // Uniform over a cluster, whose blocks share the row.
   if (e == experts) return;  // a row outside every segment
   const int2 s = segment(offsets, e, rows);
@@ -244,6 +251,140 @@ cudaError_t few(const void* x, const void* wg, const void* wu, const int32_t* of
   }
   note_launch();
   return cudaSuccess;
+}
+
+// ---- gradients of few rows ------------------------------------------------------------
+//
+// From dg and du in FP32 (no rounding before the sums). The input gradient reads
+// the weights of the experts that have rows once, along their rows:
+//   dx[r, k] = sum_n dg[r, n] Wg[e][k, n] + du[r, n] Wu[e][k, n];
+// a warp takes kDxRows weight rows of up to kFewRows rows of one expert.
+
+constexpr int kDxRows = 4;
+
+template <typename T, int kVec, int kR>
+__device__ __forceinline__ void few_dx(const float* __restrict__ dg, const float* __restrict__ du,
+                                       const T* __restrict__ wg, const T* __restrict__ wu,
+                                       T* __restrict__ dx, int row, int nrows, int hidden,
+                                       int output, int k0) {
+  const int lane = threadIdx.x & 31;
+  float acc[kR][kDxRows] = {};
+  for (int n = lane * kVec; n < output; n += 32 * kVec) {  // kVec divides output
+    Raw<T, kVec> a[kDxRows], b[kDxRows];
+#pragma unroll
+    for (int j = 0; j < kDxRows; ++j) {
+      const long long at = static_cast<long long>(min(k0 + j, hidden - 1)) * output + n;
+      a[j].load(wg + at);
+      b[j].load(wu + at);
+    }
+#pragma unroll
+    for (int i = 0; i < kR; ++i) {
+      const long long at = static_cast<long long>(row + min(i, nrows - 1)) * output + n;
+      float g[kVec], u[kVec];
+#pragma unroll
+      for (int v = 0; v < kVec; ++v) {
+        g[v] = __ldg(dg + at + v);
+        u[v] = __ldg(du + at + v);
+      }
+#pragma unroll
+      for (int j = 0; j < kDxRows; ++j) {
+        float wa[kVec], wb[kVec];
+        a[j].get(wa);
+        b[j].get(wb);
+#pragma unroll
+        for (int v = 0; v < kVec; ++v) {
+          acc[i][j] = fmaf(g[v], wa[v], acc[i][j]);
+          acc[i][j] = fmaf(u[v], wb[v], acc[i][j]);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kR; ++i) {
+#pragma unroll
+    for (int j = 0; j < kDxRows; ++j) {
+      float s = acc[i][j];
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+      if (lane == i * kDxRows + j && i < nrows && k0 + j < hidden) {
+        dx[static_cast<long long>(row + i) * hidden + k0 + j] = from_f32<T>(s);
+      }
+    }
+  }
+}
+
+template <typename T, int kVec>
+__global__ void __launch_bounds__(kFewThreads) gated_few_dx_kernel(
+    const float* __restrict__ dg, const float* __restrict__ du, const T* __restrict__ wg,
+    const T* __restrict__ wu, const int32_t* __restrict__ offsets, T* __restrict__ dx, int rows,
+    int experts, int hidden, int output) {
+  const int row = blockIdx.y;
+  const int e = expert_of(offsets, row, rows, experts);
+  if (e == experts) return;
+  const int2 s = segment(offsets, e, rows);
+  if ((row - s.x) % kFewRows != 0) return;
+  const int k0 = (blockIdx.x * kFewWarps + (threadIdx.x >> 5)) * kDxRows;
+  if (k0 >= hidden) return;
+  const long long at = static_cast<long long>(e) * hidden * output;
+  const int nrows = min(kFewRows, s.y - row);
+  if (nrows == 1) {
+    few_dx<T, kVec, 1>(dg, du, wg + at, wu + at, dx, row, nrows, hidden, output, k0);
+  } else {
+    few_dx<T, kVec, kFewRows>(dg, du, wg + at, wu + at, dx, row, nrows, hidden, output, k0);
+  }
+}
+
+// The weight gradients are written once, zeros for experts without rows: bound
+// by those bytes. dW[e][k, n] = sum_r x[r, k] d[r, n]; a warp takes kDwRows
+// weight rows of 32 vectors of columns, both gradients.
+constexpr int kDwRows = 4;
+
+template <typename T, int kVec>
+__global__ void __launch_bounds__(kFewThreads) gated_few_dw_kernel(
+    const T* __restrict__ x, const float* __restrict__ dg, const float* __restrict__ du,
+    const int32_t* __restrict__ offsets, T* __restrict__ dwg, T* __restrict__ dwu, int rows,
+    int hidden, int output, int k_blocks) {
+  // Experts and blocks of k share the y axis of the grid.
+  const int e = blockIdx.y / k_blocks;
+  const int lane = threadIdx.x & 31;
+  const int n = (blockIdx.x * 32 + lane) * kVec;
+  const int k0 = ((blockIdx.y - e * k_blocks) * kFewWarps + (threadIdx.x >> 5)) * kDwRows;
+  if (k0 >= hidden || n >= output) return;
+  const int2 s = segment(offsets, e, rows);
+  float g[kDwRows][kVec] = {}, u[kDwRows][kVec] = {};
+  for (int r = s.x; r < s.y; ++r) {
+    float a[kVec], b[kVec];
+    const long long at = static_cast<long long>(r) * output + n;
+#pragma unroll
+    for (int v = 0; v < kVec; ++v) {
+      a[v] = __ldg(dg + at + v);
+      b[v] = __ldg(du + at + v);
+    }
+#pragma unroll
+    for (int j = 0; j < kDwRows; ++j) {
+      const float xv =
+          to_f32(__ldg(x + static_cast<long long>(r) * hidden + min(k0 + j, hidden - 1)));
+#pragma unroll
+      for (int v = 0; v < kVec; ++v) {
+        g[j][v] = fmaf(xv, a[v], g[j][v]);
+        u[j][v] = fmaf(xv, b[v], u[j][v]);
+      }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < kDwRows; ++j) {
+    if (k0 + j < hidden) {
+      const long long at =
+          (static_cast<long long>(e) * hidden + k0 + j) * output + n;
+      if constexpr (kVec == 1) {
+        dwg[at] = from_f32<T>(g[j][0]);
+        dwu[at] = from_f32<T>(u[j][0]);
+      } else {
+        *reinterpret_cast<uint4*>(dwg + at) = pack16<T>(g[j]);
+        *reinterpret_cast<uint4*>(dwu + at) = pack16<T>(u[j]);
+      }
+    }
+  }
 }
 
 // ---- operand parts -----------------------------------------------------------------
@@ -396,6 +537,23 @@ __global__ void __launch_bounds__(kPackThreads) gated_pointwise_backward_kernel(
   }
 }
 
+// The same for the few-row forms, in FP32.
+template <typename T>
+__global__ void __launch_bounds__(kPackThreads) gated_pointwise_backward_f32_kernel(
+    const float* __restrict__ gate_up, const T* __restrict__ dh, float* __restrict__ dg,
+    float* __restrict__ du, long long total, int output, int activation) {
+  for (long long i = static_cast<long long>(blockIdx.x) * kPackThreads + threadIdx.x; i < total;
+       i += static_cast<long long>(gridDim.x) * kPackThreads) {
+    const long long r = total <= INT_MAX ? static_cast<int>(i) / output : i / output;
+    const long long at = i + r * output;  // gate_up rows are 2 * output long
+    float slope;
+    const float a = activate<T>(activation, __ldg(gate_up + at), &slope);
+    const float d = to_f32(__ldg(dh + i));
+    dg[i] = d * __ldg(gate_up + at + output) * slope;
+    du[i] = d * a;
+  }
+}
+
 int pack_blocks(long long total) {
   const long long want = (total + kPackThreads - 1) / kPackThreads;
   const long long cap = 16LL * sm_count();
@@ -453,6 +611,88 @@ cudaError_t launch_gated_pointwise_backward(const float* gate_up, const void* dh
   }
   note_launch();
   return cudaGetLastError();
+}
+
+cudaError_t launch_gated_pointwise_backward_f32(const float* gate_up, const void* dh, float* dg,
+                                                float* du, int rows, int output,
+                                                Activation activation, Dtype dtype,
+                                                cudaStream_t stream) {
+  const long long total = static_cast<long long>(rows) * output;
+  const int blocks = pack_blocks(total);
+  const int act = static_cast<int>(activation);
+  if (dtype == Dtype::kBf16) {
+    gated_pointwise_backward_f32_kernel<<<blocks, kPackThreads, 0, stream>>>(
+        gate_up, static_cast<const __nv_bfloat16*>(dh), dg, du, total, output, act);
+  } else {
+    gated_pointwise_backward_f32_kernel<<<blocks, kPackThreads, 0, stream>>>(
+        gate_up, static_cast<const float*>(dh), dg, du, total, output, act);
+  }
+  note_launch();
+  return cudaGetLastError();
+}
+
+namespace {
+
+template <typename T>
+cudaError_t few_dx_launch(const float* dg, const float* du, const void* wg, const void* wu,
+                          const int32_t* offsets, void* dx, int rows, int experts, int hidden,
+                          int output, cudaStream_t stream) {
+  constexpr int kVec = 16 / sizeof(T);
+  const bool vec = output % kVec == 0 && aligned_to(wg, 16) && aligned_to(wu, 16);
+  auto* kernel = vec ? gated_few_dx_kernel<T, kVec> : gated_few_dx_kernel<T, 1>;
+  kernel<<<dim3(ceil_div(hidden, kFewWarps * kDxRows), rows), kFewThreads, 0, stream>>>(
+      dg, du, static_cast<const T*>(wg), static_cast<const T*>(wu), offsets, static_cast<T*>(dx),
+      rows, experts, hidden, output);
+  note_launch();
+  return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t few_dw_launch(const void* x, const float* dg, const float* du, const int32_t* offsets,
+                          void* dwg, void* dwu, int rows, int experts, int hidden, int output,
+                          cudaStream_t stream) {
+  constexpr int kVec = 16 / sizeof(T);
+  const bool vec = output % kVec == 0 && aligned_to(dwg, 16) && aligned_to(dwu, 16);
+  const int k_blocks = ceil_div(hidden, kFewWarps * kDwRows);
+  auto* kernel = vec ? gated_few_dw_kernel<T, kVec> : gated_few_dw_kernel<T, 1>;
+  // The y axis holds 65535 blocks: experts in slices that fit.
+  const int slice = k_blocks < 65535 ? 65535 / k_blocks : 0;
+  if (slice == 0) return cudaErrorInvalidConfiguration;
+  for (int e = 0; e < experts; e += slice) {
+    const int count = experts - e < slice ? experts - e : slice;
+    const long long at = static_cast<long long>(e) * hidden * output;
+    kernel<<<dim3(ceil_div(output, 32 * (vec ? kVec : 1)), count * k_blocks), kFewThreads, 0,
+             stream>>>(static_cast<const T*>(x), dg, du, offsets + e,
+                       static_cast<T*>(dwg) + at, static_cast<T*>(dwu) + at, rows, hidden, output,
+                       k_blocks);
+    note_launch();
+    const cudaError_t err = cudaGetLastError();
+    if (err != cudaSuccess) return err;
+  }
+  return cudaSuccess;
+}
+
+}  // namespace
+
+cudaError_t launch_gated_few_dx(const float* dg, const float* du, const void* wg, const void* wu,
+                                const int32_t* offsets, void* dx, int rows, int experts,
+                                int hidden, int output, Dtype dtype, cudaStream_t stream) {
+  return dtype == Dtype::kBf16
+             ? few_dx_launch<__nv_bfloat16>(dg, du, wg, wu, offsets, dx, rows, experts, hidden,
+                                            output, stream)
+             : few_dx_launch<float>(dg, du, wg, wu, offsets, dx, rows, experts, hidden, output,
+                                    stream);
+}
+
+cudaError_t launch_gated_few_dw(const void* x, const float* dg, const float* du,
+                                const int32_t* offsets, void* dwg, void* dwu, int rows,
+                                int experts, int hidden, int output, Dtype dtype,
+                                cudaStream_t stream) {
+  return dtype == Dtype::kBf16
+             ? few_dw_launch<__nv_bfloat16>(x, dg, du, offsets, dwg, dwu, rows, experts, hidden,
+                                            output, stream)
+             : few_dw_launch<float>(x, dg, du, offsets, dwg, dwu, rows, experts, hidden, output,
+                                    stream);
 }
 
 }  // namespace rrb

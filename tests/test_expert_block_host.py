@@ -81,6 +81,10 @@ def test_gated_workspace(rrlib):
     assert size(4096, 8, 64, 64, 0) == 6 * (4096 * 64 + 2 * 8 * 64 * 64)
     assert back(4096, 8, 64, 64, 2) == 2 * 4096 * 64 * 2
     assert back(4096, 8, 64, 64, 0) == 6 * (3 * 4096 * 64 + 2 * 8 * 64 * 64)
+    assert back(4, 8, 64, 64, 2) == 2 * 4 * 64 * 4   # few rows: dg and du in FP32
+    assert back(64, 8, 64, 64, 0) == 2 * 64 * 64 * 4
+    # Rows scarce among the experts keep a second part of dg and du.
+    assert back(256, 8, 64, 64, 2) == 2 * 2 * 256 * 64 * 2
     # Past 32 bits: 131072 rows of the 128-expert layer in FP32.
     assert size(131072, 128, 4096, 1408, 0) == 6 * (131072 * 4096 + 2 * 128 * 4096 * 1408)
     for bad in ((-1, 8, 64, 64, 0), (1, 0, 64, 64, 0), (1, 8, 0, 64, 0), (1, 8, 64, 64, 1)):

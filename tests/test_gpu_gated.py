@@ -353,6 +353,22 @@ def test_one_form_meets_the_other(cuda, rows):
     assert normwise(h, gated(x, wg, wu, off)[2]) < 2.0 ** -8 / math.sqrt(3)
 
 
+@pytest.mark.parametrize("dtype,k,n,experts,rows", [
+    (BF16, 64, 48, 40, 10), (BF16, 64, 48, 40, 11), (BF16, 63, 48, 6, 24), (BF16, 63, 48, 6, 25),
+    (FP32, 64, 48, 6, 48), (FP32, 64, 48, 6, 49)])
+def test_backward_forms_meet(cuda, dtype, k, n, experts, rows):
+    """Both sides of each boundary between the backward pass's two forms."""
+    counts = np.random.default_rng(rows).multinomial(rows, [1 / experts] * experts)
+    x, wg, wu, off, dh = make(counts, 2, k, n, dtype, cuda, seed=81)
+    _, gu = forward(x, wg, wu, off)
+    dx, dwg, dwu = backward(x, wg, wu, off, gu, dh)
+    want = gated_backward(x[:rows], wg, wu, off, dh[:rows])
+    bound = math.sqrt(2) * 2.0 ** -8 / math.sqrt(3) if dtype == BF16 else 2.0 ** -19
+    for got, ref in zip((dx[:rows], dwg, dwu), want):
+        assert normwise(got, ref) < bound
+    assert bool((dx[rows:] == 777.0).all())
+
+
 def test_many_experts(cuda):
     counts = np.random.default_rng(1).integers(0, 4, 1024)
     x, wg, wu, off, dh = make(counts, 0, 16, 16, FP32, cuda, seed=90)
