@@ -5,6 +5,9 @@ GEMM, combine with norms; in FP32 forward and backward, and in 8-bit integers.
 from __future__ import annotations
 
 import math
+import os
+import subprocess
+import sys
 
 import torch
 import pytest
@@ -140,3 +143,45 @@ def test_bf16_and_int8_block(cuda):
     # 0.5 * 6 / 127 / sqrt(3) of a deviation per operand, two operands.
     assert normwise(out, want) < math.sqrt(2) * 3 / 127 / math.sqrt(3) + 2.0 ** -7
     assert normwise(normed, want_n) < math.sqrt(2) * 3 / 127 / math.sqrt(3) + 2.0 ** -7
+
+
+def test_first_calls_inside_a_capture(cuda):
+    """A process whose first calls are captured: nothing needs a plain call before."""
+    worker = os.path.join(os.path.dirname(os.path.abspath(__file__)), "first_call_worker.py")
+    run = subprocess.run([sys.executable, worker], capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0, run.stdout + run.stderr
+    assert "first calls in a capture: ok" in run.stdout
+
+
+def test_streams_side_by_side(cuda):
+    """Calls on two streams at once, each with buffers and a workspace of its own."""
+    results, streams = [], [torch.cuda.Stream(), torch.cuda.Stream()]
+    bf = torch.bfloat16
+    sets = []
+    for i in range(2):
+        x = random((3000, 264), 20 + i, cuda, bf)
+        wg, wu = random((9, 264, 200), 30 + i, cuda, bf, 0.06), random((9, 264, 200), 40 + i, cuda,
+                                                                     bf, 0.06)
+        off = torch.tensor([0, 5, 5, 900, 1300, 1301, 1500, 2600, 2999, 3000],
+                           dtype=torch.int32, device=cuda)
+        size = rr.grouped_gated_gemm_workspace_size(3000, 9, 264, 200, bf, True)
+        sets.append((x, wg, wu, off, random((3000, 200), 50 + i, cuda, bf),
+                     torch.empty(size, dtype=torch.uint8, device=cuda)))
+
+    def step(i):
+        x, wg, wu, off, dh, ws = sets[i]
+        h, gu = torch.empty_like(dh), torch.empty(3000, 400, device=cuda)
+        dx, dwg, dwu = torch.empty_like(x), torch.empty_like(wg), torch.empty_like(wu)
+        rr.grouped_gated_gemm(x, wg, wu, off, h, gate_up=gu, workspace=ws)
+        rr.grouped_gated_gemm_backward(x, wg, wu, off, gu, dh, dx, dwg, dwu, workspace=ws)
+        return h, gu, dx, dwg, dwu
+
+    want = [step(0), step(1)]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                results.append((i, step(i)))
+    torch.cuda.synchronize()
+    for i, got in results:
+        assert all(torch.equal(a, b) for a, b in zip(got, want[i]))
