@@ -781,7 +781,9 @@ __device__ __forceinline__ float sum2(F2 a) {
   return lo + hi;
 }
 
-// This thread's columns of a staged row in pairs, zero past the row's end.
+// This thread's columns of a staged row in pairs. Columns past the row's end take
+// the row's first ones: the caller's factors are zero there, which costs less
+// than a test around every load.
 template <typename T, int kPer, int kPairs>
 __device__ __forceinline__ void staged_row(const char* row, int output, int team, int tid,
                                            F2 (&v)[kPairs]) {
@@ -789,30 +791,21 @@ __device__ __forceinline__ void staged_row(const char* row, int output, int team
 #pragma unroll
   for (int q = 0; q < 2 * kPairs / kPer; ++q) {
     const int col = (q * team + tid) * kPer;
-    if (col < output) {
-      staged_cols<T, kPer>(row + col * sizeof(T), f + q * kPer);
-    } else {
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) f[q * kPer + i] = 0.0f;
-    }
+    staged_cols<T, kPer>(row + (col < output ? col : 0) * sizeof(T), f + q * kPer);
   }
 #pragma unroll
   for (int i = 0; i < kPairs; ++i) v[i] = f2(f[2 * i], f[2 * i + 1]);
 }
 
+// The same of a row of factors, whose column `past` stands for those past the end.
 template <int kPer, int kPairs>
-__device__ __forceinline__ void shared_row(const float* row, int output, int team, int tid,
-                                           F2 (&v)[kPairs]) {
+__device__ __forceinline__ void factor_row(const float* row, int output, int past, int team,
+                                           int tid, F2 (&v)[kPairs]) {
   float f[2 * kPairs];
 #pragma unroll
   for (int q = 0; q < 2 * kPairs / kPer; ++q) {
     const int col = (q * team + tid) * kPer;
-    if (col < output) {
-      shared_cols<kPer>(row + col, f + q * kPer);
-    } else {
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) f[q * kPer + i] = 0.0f;
-    }
+    shared_cols<kPer>(row + (col < output ? col : past), f + q * kPer);
   }
 #pragma unroll
   for (int i = 0; i < kPairs; ++i) v[i] = f2(f[2 * i], f[2 * i + 1]);
@@ -872,12 +865,13 @@ __global__ void __launch_bounds__(kStreamThreads, 1) unpermute_norm_backward_str
   float* pg = reinterpret_cast<float*>(rings + st.teams * ring_size);
   float* shared_pre = pg + st.padded;
   for (int c = threadIdx.x; c < st.padded; c += blockDim.x) {
-    float f, p;
+    float f, p;  // zero from column n on; column padded - 8 is past the end
     column_factors<1>(in, c, &f, &p);
     pg[c] = f;
     if (st.factors > 1) shared_pre[c] = p;
   }
   const float* pr = st.factors > 1 ? shared_pre : in.pre_gamma;
+  const int past = st.padded - 8;
   stream_setup(st, in.top_k, s);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int team = threadIdx.x / st.team, tid = threadIdx.x % st.team;
@@ -900,7 +894,16 @@ __global__ void __launch_bounds__(kStreamThreads, 1) unpermute_norm_backward_str
     const float* weight = s.weight[team][loop.stage];
     const float i1 = post ? __ldg(g.inv_rms + 2 * t) : 1.0f;
     const float i2 = pre ? __ldg(g.inv_rms + 2 * t + 1) : 0.0f;
-    const F2 i12 = f2(i1), i22 = f2(i2), scale = f2(in.residual_scale);
+    // Zero for columns past the end, whose c and rn then are zero as well.
+    F2 i12[kPairs], i22[kPairs];
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) {
+      const bool in0 = ((2 * i / kPer) * st.team + tid) * kPer < n;
+      const bool in1 = (((2 * i + 1) / kPer) * st.team + tid) * kPer < n;
+      i12[i] = f2(in0 ? i1 : 0.0f, in1 ? i1 : 0.0f);
+      i22[i] = f2(in0 ? i2 : 0.0f, in1 ? i2 : 0.0f);
+    }
+    const F2 scale = f2(in.residual_scale);
     F2 c[kPairs], a[kPairs], rn[kPairs];
     F2 y0[kTwo ? kPairs : 1], y1[kTwo ? kPairs : 1];  // the routes' rows, if there are two at most
     F2 f[kPairs];                                     // post * gate
@@ -930,12 +933,12 @@ __global__ void __launch_bounds__(kStreamThreads, 1) unpermute_norm_backward_str
           for (int i = 0; i < kPairs; ++i) c[i] = fma2(w, x[i], c[i]);
         }
       }
-      shared_row<kPer>(pg, n, st.team, tid, f);
+      factor_row<kPer>(pg, n, past, st.team, tid, f);
       staged_row<T, kPer>(ring + start[at_res], n, st.team, tid, x);
 #pragma unroll
       for (int i = 0; i < kPairs; ++i) {
-        c[i] = mul2(i12, c[i]);
-        rn[i] = mul2(i22, fma2(scale, x[i], mul2(c[i], f[i])));
+        c[i] = mul2(i12[i], c[i]);
+        rn[i] = mul2(i22[i], fma2(scale, x[i], mul2(c[i], f[i])));
       }
       if (has_dro) {
         staged_row<T, kPer>(ring + start[at_dro], n, st.team, tid, a);
@@ -946,13 +949,13 @@ __global__ void __launch_bounds__(kStreamThreads, 1) unpermute_norm_backward_str
       if (pre) {
         F2 p[kPairs];
         staged_row<T, kPer>(ring + start[at_dn], n, st.team, tid, x);
-        shared_row<kPer>(pr, n, st.team, tid, p);
+        factor_row<kPer>(pr, n, 0, st.team, tid, p);
 #pragma unroll
         for (int i = 0; i < kPairs; ++i) {
           s_pre[i] = fma2(x[i], rn[i], s_pre[i]);
           const F2 v = mul2(x[i], p[i]);
           dot = fma2(v, rn[i], dot);
-          a[i] = fma2(i22, v, a[i]);
+          a[i] = fma2(i22[i], v, a[i]);
         }
       }
     }
@@ -1041,16 +1044,22 @@ __global__ void __launch_bounds__(kStreamThreads, 1) unpermute_norm_backward_str
     put_row<T, kPer>(static_cast<T*>(g.d_residual) + t * n, n, st.team, tid, x);
 #pragma unroll
     for (int i = 0; i < kPairs; ++i) {
-      a[i] = mul2(i12, fma2(nm1, c[i], mul2(f[i], a[i])));  // dc
+      a[i] = mul2(i12[i], fma2(nm1, c[i], mul2(f[i], a[i])));  // dc
     }
-    for (int k = 0; k < in.top_k; ++k) {
-      if (start[k] < 0) continue;
+    auto put_route = [&](int k) {
+      if (start[k] < 0) return;
       const F2 w = f2(weight[k]);
 #pragma unroll
       for (int i = 0; i < kPairs; ++i) x[i] = mul2(w, a[i]);
       put_row<T, kPer>(static_cast<T*>(g.d_y_permuted) +
                            static_cast<long long>(s.pos[team][loop.stage][k]) * n,
                        n, st.team, tid, x);
+    };
+    if constexpr (kTwo) {
+      put_route(0);
+      if (in.top_k > 1) put_route(1);
+    } else {
+      for (int k = 0; k < in.top_k; ++k) put_route(k);
     }
   }
   // The block's shares of the column sums, [block][3][output]: its teams' add up
@@ -1131,7 +1140,7 @@ Stream stream_plan(int tokens, int top_k, int output, int extra_rows, bool gradi
   // A row's granules: up to 15 bytes before and after it.
   st.stride = static_cast<int>((output * size + 15) / 16 * 16 + 16);
   if (gradient) {
-    st.padded = (output + 3) / 4 * 4;
+    st.padded = (output + 7) / 8 * 8 + 8;  // and eight zeros
     st.factors = 2;
   }
   // Two stages have to fit: with pre left in its own buffer, or with half the
