@@ -386,9 +386,9 @@ struct StreamSmem {
   uint64_t full[kMaxTeams][kMaxStages];
   int failed;
   // Of each token in a ring: where its rows start (-1: a skipped route), and
-  // the routes' weights and positions.
+  // the routes' weights (behind them the gradient's two 1/rms) and positions.
   int start[kMaxTeams][kMaxStages][kStreamTopK + 3];
-  float weight[kMaxTeams][kMaxStages][kStreamTopK];
+  float weight[kMaxTeams][kMaxStages][kStreamTopK + 2];
   int pos[kMaxTeams][kMaxStages][kStreamTopK];
 };
 
@@ -399,7 +399,8 @@ __device__ __forceinline__ void team_sync(int team, int threads) {
 }
 
 struct Sources {
-  const void* row[3] = {};  // residual, d_residual_out, d_normed; null ones left out
+  const void* row[3] = {};         // residual, d_residual_out, d_normed; null ones left out
+  const float* inv_rms = nullptr;  // [tokens][2], for the gradient
 };
 
 // Fills a team's ring; called by its first warp, a lane per row (sources <= 32).
@@ -413,12 +414,13 @@ struct Filler {
   int team;
   const char* base;  // of this lane's rows
   long long rows;    // how many there are
-  int pos;           // of the next token's row, fetched ahead
+  const float* inv_rms;
+  int pos;  // of the next token's row, fetched ahead
   float weight;
 
   __device__ __forceinline__ Filler(const UnpermuteNorm& in, const Stream& st, StreamSmem& s,
                                     const Sources& src, uint32_t ring, int team)
-      : in(in), st(st), s(s), ring(ring), team(team) {
+      : in(in), st(st), s(s), ring(ring), team(team), inv_rms(src.inv_rms) {
     const int lane = threadIdx.x & 31;
     const bool route = lane < in.top_k;
     base = route ? static_cast<const char*>(in.y_permuted)
@@ -434,6 +436,8 @@ struct Filler {
     if (lane < in.top_k && t < in.tokens) {
       pos = __ldg(in.route_pos + t * in.top_k + lane);
       weight = __ldg(in.route_weights + t * in.top_k + lane);
+    } else if (inv_rms != nullptr && lane < in.top_k + 2 && t < in.tokens) {
+      weight = __ldg(inv_rms + 2 * t + lane - in.top_k);
     }
   }
   // Starts token t's rows (position and weight fetched) into `stage`, and fetches
@@ -463,10 +467,8 @@ struct Filler {
     if (lane < st.sources) {
       s.start[team][stage][lane] = there ? static_cast<int>(place + (at - a0)) : -1;
     }
-    if (route) {
-      s.weight[team][stage][lane] = weight;
-      s.pos[team][stage][lane] = pos;
-    }
+    if (lane < in.top_k + 2) s.weight[team][stage][lane] = weight;
+    if (route) s.pos[team][stage][lane] = pos;
     uint32_t total;
     if constexpr (kAligned) {
       total = __popc(__ballot_sync(0xffffffffu, there)) * static_cast<uint32_t>(bytes);
@@ -886,14 +888,15 @@ __global__ void __launch_bounds__(kStreamThreads, 1) unpermute_norm_backward_str
   src.row[0] = in.residual;
   src.row[1] = has_dro ? g.d_residual_out : g.d_normed;
   src.row[2] = g.d_normed;
+  src.inv_rms = post || pre ? g.inv_rms : nullptr;
   int parity = 0;
   TokenLoop<T, kPer * sizeof(T) == 16> loop(in, st, s, src, smem_u32(ring), team, err);
   while (loop.step()) {
     const long long t = loop.t;
     const int* start = s.start[team][loop.stage];
     const float* weight = s.weight[team][loop.stage];
-    const float i1 = post ? __ldg(g.inv_rms + 2 * t) : 1.0f;
-    const float i2 = pre ? __ldg(g.inv_rms + 2 * t + 1) : 0.0f;
+    const float i1 = post ? weight[in.top_k] : 1.0f;
+    const float i2 = pre ? weight[in.top_k + 1] : 0.0f;
     // Zero for columns past the end, whose c and rn then are zero as well.
     F2 i12[kPairs], i22[kPairs];
 #pragma unroll
@@ -1004,8 +1007,10 @@ __global__ void __launch_bounds__(kStreamThreads, 1) unpermute_norm_backward_str
     auto team_sums = [&](int k) {
       if (kTwo && team_warps == 1) return mine;
       float v = 0.0f;
-      for (int w = lane & 3; w < team_warps; w += 4) {
-        v += sums[parity][warp0 + w][k >> 1][lane >> 2];
+#pragma unroll
+      for (int i = 0; i < kMaxTeams; i += 4) {
+        const int w = (lane & 3) + i;
+        if (w < team_warps) v += sums[parity][warp0 + w][k >> 1][lane >> 2];
       }
       v += __shfl_xor_sync(0xffffffffu, v, 1);
       return v + __shfl_xor_sync(0xffffffffu, v, 2);
@@ -1022,12 +1027,13 @@ __global__ void __launch_bounds__(kStreamThreads, 1) unpermute_norm_backward_str
       if (k + 1 < in.top_k && start[k + 1] >= 0) m1 = fmaf(weight[k + 1], p1, m1);
     }
     m1 = post ? i1 * m1 * per_col : 0.0f;
-    for (int k = 0; k < (kTwo ? 1 : in.top_k); k += 2) {
+    // The last warp's lane 0 writes the routes' gradients (the first one fills the ring).
+    for (int k = 0; warp - warp0 == team_warps - 1 && k < (kTwo ? 1 : in.top_k); k += 2) {
       const float v = k == 0 ? sums01 : team_sums(k);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const float d = i1 * (p_of(v, h) - m1 * sum_of(v, 3 * h + 2));
-        if (tid == 0 && k + h < in.top_k) {
+        if (lane == 0 && k + h < in.top_k) {
           g.d_route_weights[t * in.top_k + k + h] = start[k + h] >= 0 ? d : 0.0f;
         }
       }
