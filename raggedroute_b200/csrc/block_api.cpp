@@ -81,7 +81,7 @@ bool overlap(const Range& a, const Range& b) {
   return a0 < b0 + b.bytes && b0 < a0 + a.bytes;
 }
 
-// No output may touch an input or another output.
+// No output (the workspace counts as one) may touch an input or another output.
 bool outputs_clash(std::initializer_list<Range> outputs, std::initializer_list<Range> inputs) {
   for (auto o = outputs.begin(); o != outputs.end(); ++o) {
     for (const Range& i : inputs) {
@@ -255,14 +255,16 @@ rr_status rr_grouped_gated_gemm(const void* x_permuted, const void* gate_weights
     return invalid("grouped_gated_gemm: rows of a multiple of 16 bytes need 16-byte aligned buffers");
   }
   const std::size_t rows = route_pairs, weights = size * experts * hidden * output;
-  if (outputs_clash({{h, rows * output * size}, {gate_up, rows * output * 8}},
+  const GatedPlan plan = gated_plan(route_pairs, experts, hidden, output, t, false);
+  if (outputs_clash({{h, rows * output * size},
+                     {gate_up, rows * output * 8},
+                     {ctx->workspace, plan.total}},
                     {{x_permuted, rows * hidden * size},
                      {gate_weights, weights},
                      {up_weights, weights},
                      {offsets, 4ull * (experts + 1)}})) {
     return invalid("grouped_gated_gemm: an output overlaps another buffer");
   }
-  const GatedPlan plan = gated_plan(route_pairs, experts, hidden, output, t, false);
   s = check_workspace(ctx, plan.total);
   if (s.code != RR_SUCCESS) return s;
   s = check_device(ctx);
@@ -326,7 +328,11 @@ rr_status rr_grouped_gated_gemm_backward(const void* x_permuted, const void* gat
         "grouped_gated_gemm_backward: rows of a multiple of 16 bytes need 16-byte aligned buffers");
   }
   const std::size_t rows = route_pairs;
-  if (outputs_clash({{dx, rows * hidden * size}, {d_gate_weights, weights}, {d_up_weights, weights}},
+  const GatedPlan plan = gated_plan(route_pairs, experts, hidden, output, t, true);
+  if (outputs_clash({{dx, rows * hidden * size},
+                     {d_gate_weights, weights},
+                     {d_up_weights, weights},
+                     {ctx->workspace, plan.total}},
                     {{x_permuted, rows * hidden * size},
                      {gate_weights, weights},
                      {up_weights, weights},
@@ -335,7 +341,6 @@ rr_status rr_grouped_gated_gemm_backward(const void* x_permuted, const void* gat
                      {offsets, 4ull * (experts + 1)}})) {
     return invalid("grouped_gated_gemm_backward: an output overlaps another buffer");
   }
-  const GatedPlan plan = gated_plan(route_pairs, experts, hidden, output, t, true);
   s = check_workspace(ctx, plan.total);
   if (s.code != RR_SUCCESS) return s;
   s = check_device(ctx);
@@ -623,8 +628,10 @@ rr_status rr_unpermute_norm_backward(
     return invalid("unpermute_norm_backward received a misaligned buffer");
   }
   const std::size_t grid = rows * cols * size, wide = routes * cols * size;
+  const Range work{ctx->workspace, rrb::unpermute_norm_backward_workspace_bytes(tokens, output)};
   const Range dro{d_residual_out, grid}, dres{d_residual, grid};
   if (outputs_clash({dres,
+                     work,
                      {d_y_permuted, wide},
                      {d_route_weights, 4 * routes},
                      {d_post_gamma, 4 * cols},
@@ -640,7 +647,8 @@ rr_status rr_unpermute_norm_backward(
                      {inv_rms, 8 * rows},
                      {d_normed, grid}}) ||
       (d_residual != d_residual_out && overlap(dres, dro)) ||
-      outputs_clash({{d_y_permuted, wide},
+      outputs_clash({work,
+                     {d_y_permuted, wide},
                      {d_route_weights, 4 * routes},
                      {d_post_gamma, 4 * cols},
                      {d_gate, 4 * cols},
@@ -648,7 +656,7 @@ rr_status rr_unpermute_norm_backward(
                     {dro})) {
     return invalid("unpermute_norm_backward: an output overlaps another buffer");
   }
-  s = check_workspace(ctx, rrb::unpermute_norm_backward_workspace_bytes(tokens, output));
+  s = check_workspace(ctx, work.bytes);
   if (s.code != RR_SUCCESS) return s;
   s = check_device(ctx);
   if (s.code != RR_SUCCESS) return s;

@@ -17,6 +17,7 @@ import torch
 from raggedroute_b200._lib import Context, RRContext, check, lib
 from raggedroute_b200.ops import _need
 
+_MAX_SIZE = 2**31 - 1  # the entry points take sizes as int
 _DTYPES = {torch.float32: 0, torch.bfloat16: 2}
 ACTIVATIONS = {"silu": 0, "gelu_tanh": 1, "relu": 2}
 
@@ -55,6 +56,8 @@ def _expect(t: torch.Tensor | None, shape: tuple, dtype: torch.dtype, device: to
 def _rank(t: torch.Tensor, dims: int, name: str) -> None:
     if t.dim() != dims:
         raise ValueError(f"{name} must have {dims} dimensions, got {t.dim()}")
+    if t.numel() > _MAX_SIZE and max(t.shape) > _MAX_SIZE:
+        raise ValueError(f"{name}: no dimension may be longer than {_MAX_SIZE}")
     if not t.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor, got {t.device}")
 

@@ -199,3 +199,28 @@ def test_error_names_the_operator(rrlib):
                                                    0, 2, ctypes.pointer(RRContext()))
         from raggedroute_b200._lib import check
         check(status, "grouped_gated_gemm")
+
+
+def test_workspace_that_touches_a_buffer(rrlib):
+    lib = rrlib.lib()
+    bad = StatusCode.INVALID_ARGUMENT
+    size = lib.rr_grouped_gated_gemm_workspace_size(4096, 4, 64, 64, 0)
+    for buf in (BUF[0], BUF[1], BUF[4] + 256):  # x, gate weights, h
+        assert gated(lib, dtype=0, rows=4096, c=ctx(buf, size)) == bad, hex(buf)
+    size = lib.rr_grouped_gated_gemm_backward_workspace_size(64, 4, 64, 64, 2)
+    for buf in (BUF[0], BUF[5], BUF[7], BUF[6] - size + 256):  # x, gate_up, dWg, in front of dx
+        assert gated_back(lib, c=ctx(buf, size)) == bad, hex(buf)
+    size = lib.rr_unpermute_norm_backward_workspace_size(8, 64)
+    for buf in (BUF[0], BUF[3], BUF[8], BUF[11], BUF[15]):
+        assert code(lib.rr_unpermute_norm_backward(
+            *BUF[:16], 1.0, 8, 2, 64, 2, ctx(buf, size))) == bad, hex(buf)
+
+
+def test_dimensions_past_an_int(rrlib):
+    """A long dimension is refused, not cut to 32 bits."""
+    x = torch.empty(2 ** 31, 1, device="meta", dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="longer than"):
+        block.quantize_rows_int8(x, x, x)
+    w = torch.empty(2, 1, 2 ** 31, device="meta")
+    with pytest.raises(ValueError, match="longer than"):
+        block.quantize_expert_weights_int8(w, w, w)
