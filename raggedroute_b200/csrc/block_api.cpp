@@ -65,6 +65,9 @@ rr_status check_workspace(const rr_context* ctx, std::size_t bytes) {
   return ok();
 }
 
+// Column counts: an index and a few strides past it stay an int.
+constexpr int kMaxDim = 1 << 30;
+
 std::size_t up256(std::size_t n) { return (n + 255) / 256 * 256; }
 long long up8(long long n) { return (n + 7) / 8 * 8; }
 int up16(int n) { return (n + 15) / 16 * 16; }
@@ -180,8 +183,8 @@ GatedPlan gated_plan(int rows, int experts, int hidden, int output, Dtype dtype,
 
 rr_status check_gated(int route_pairs, int experts, int hidden, int output, int activation) {
   if (experts <= 0 || experts > RR_MAX_EXPERTS || route_pairs < 0 || hidden <= 0 || output <= 0 ||
-      hidden > INT_MAX - 256 || output > INT_MAX / 2 - 256 || route_pairs > INT_MAX - 512) {
-    return invalid("grouped_gated_gemm requires 1<=E<=1024, R>=0, K>=1 and N>=1");
+      hidden > kMaxDim || output > kMaxDim / 2 || route_pairs > INT_MAX - 512) {
+    return invalid("grouped_gated_gemm requires 1<=E<=1024, R>=0, 1<=K<=2^30 and 1<=N<=2^29");
   }
   if (activation < RR_ACTIVATION_SILU || activation > RR_ACTIVATION_RELU) {
     return invalid("grouped_gated_gemm received an unknown activation");
@@ -423,8 +426,9 @@ rr_status rr_quantize_expert_weights_int8(const void* expert_weights, int8_t* wq
   rr_status s = check_call(ctx, dtype);
   if (s.code != RR_SUCCESS) return s;
   if (experts <= 0 || experts > RR_MAX_EXPERTS || hidden <= 0 || hidden > RR_MAX_INT8_HIDDEN ||
-      output <= 0 || output > INT_MAX - 256) {
-    return invalid("quantize_expert_weights_int8 requires 1<=E<=1024, 1<=K<=131072 and N>=1");
+      output <= 0 || output > kMaxDim) {
+    return invalid(
+        "quantize_expert_weights_int8 requires 1<=E<=1024, 1<=K<=131072 and 1<=N<=2^30");
   }
   const std::size_t size = dtype == RR_DTYPE_BF16 ? 2 : 4;
   if (expert_weights == nullptr || wq == nullptr || w_scale == nullptr ||
@@ -456,8 +460,8 @@ rr_status rr_grouped_gemm_int8(const int8_t* xq, const float* x_scale, const int
   if (s.code != RR_SUCCESS) return s;
   if (experts <= 0 || experts > RR_MAX_EXPERTS || route_pairs < 0 ||
       route_pairs > INT_MAX - 512 || hidden <= 0 || hidden > RR_MAX_INT8_HIDDEN || output <= 0 ||
-      output > INT_MAX - 512) {
-    return invalid("grouped_gemm_int8 requires 1<=E<=1024, R>=0, 1<=K<=131072 and N>=1");
+      output > kMaxDim) {
+    return invalid("grouped_gemm_int8 requires 1<=E<=1024, R>=0, 1<=K<=131072 and 1<=N<=2^30");
   }
   if (route_pairs == 0) return ok();
   const Dtype t = static_cast<Dtype>(dtype);

@@ -224,3 +224,13 @@ def test_dimensions_past_an_int(rrlib):
     w = torch.empty(2, 1, 2 ** 31, device="meta")
     with pytest.raises(ValueError, match="longer than"):
         block.quantize_expert_weights_int8(w, w, w)
+
+
+def test_sizes_past_the_index_range(rrlib):
+    lib = rrlib.lib()
+    bad = StatusCode.INVALID_ARGUMENT
+    assert gated(lib, k=2 ** 30 + 8) == bad and gated(lib, n=2 ** 29 + 8) == bad
+    assert gated_back(lib, k=2 ** 30 + 8) == bad and gated_back(lib, n=2 ** 29 + 8) == bad
+    assert lib.rr_grouped_gated_gemm_workspace_size(64, 4, 2 ** 30 + 8, 64, 0) == 0
+    assert code(lib.rr_grouped_gemm_int8(*BUF[:6], 64, 4, 64, 2 ** 30 + 16, 2, ctx())) == bad
+    assert code(lib.rr_quantize_expert_weights_int8(*BUF[:3], 4, 64, 2 ** 30 + 16, 2, ctx())) == bad
