@@ -7,7 +7,9 @@ travels with the working tree to the GPU host. The CUDA runtime and NCCL
 (expert-parallel runtime) are linked dynamically: the library shares the
 calling application's CUDA runtime, so kernels it launches into the caller's
 streams and captured graphs are the caller's runtime objects (a caller can
-inspect or update their graph nodes).
+inspect or update their graph nodes). The Python binding of the expert-block
+operators (csrc/python, raggedroute_b200/_block_calls.so) is compiled against the
+installed torch and linked to the library beside it; other hosts do not need it.
 
 Usage: ``python -m raggedroute_b200.build [--force] [-j N]``.
 """
@@ -19,6 +21,7 @@ import glob
 import os
 import subprocess
 import sys
+import sysconfig
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
@@ -29,6 +32,7 @@ NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 COMMON = ["-std=c++17", "-O3", "-lineinfo", "-Xcompiler", "-fPIC",
           "-I" + os.path.join(ROOT, "include"), "-I" + CSRC]
+CALLS = os.path.join(PKG, "_block_calls.so")
 EXPORTS = os.path.join(CSRC, "exports.map")
 
 
@@ -61,6 +65,29 @@ def _compile(src: str, verbose_ptxas: bool) -> str:
     return out
 
 
+def build_calls(force: bool = False) -> str:
+    """The Python binding of the expert-block operators."""
+    import torch
+    src = os.path.join(CSRC, "python", "block_calls.cpp")
+    header = os.path.join(ROOT, "include", "raggedroute_b200.h")
+    newest = max(os.path.getmtime(p) for p in (src, header, torch.__file__))
+    if force or not os.path.exists(CALLS) or os.path.getmtime(CALLS) < newest:
+        torch_dir = os.path.dirname(torch.__file__)
+        cuda = os.path.dirname(os.path.dirname(NVCC))
+        cmd = [os.environ.get("CXX", "g++"), "-std=c++17", "-O2", "-fPIC", "-shared", src, "-o",
+               CALLS, "-I" + sysconfig.get_paths()["include"],
+               "-I" + os.path.join(cuda, "include"),
+               "-isystem", os.path.join(torch_dir, "include"),
+               "-isystem", os.path.join(torch_dir, "include", "torch", "csrc", "api", "include"),
+               "-L" + PKG, "-lraggedroute_b200", "-Wl,-rpath,$ORIGIN",
+               "-L" + os.path.join(torch_dir, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10",
+               "-lc10_cuda", "-L" + os.path.join(cuda, "lib64"), "-lcudart"]
+        res = subprocess.run(cmd, capture_output=True, text=True)
+        if res.returncode != 0:
+            raise RuntimeError(f"g++ failed for {src}:\n{res.stdout}\n{res.stderr}")
+    return CALLS
+
+
 def build(force: bool = False, jobs: int = 8, verbose_ptxas: bool = False) -> str:
     os.makedirs(BUILD, exist_ok=True)
     srcs = sources()
@@ -81,6 +108,7 @@ def build(force: bool = False, jobs: int = 8, verbose_ptxas: bool = False) -> st
         res = subprocess.run(cmd, capture_output=True, text=True)
         if res.returncode != 0:
             raise RuntimeError(f"link failed:\n{res.stdout}\n{res.stderr}")
+    build_calls(force)
     return LIB
 
 

@@ -7,6 +7,11 @@ caller-owned outputs, check types and shapes on the host and call the matching
 ``rr_*`` entry point on the current torch stream (or ``ctx.stream``). float32
 and bfloat16 are accepted; sizes are read from the tensors. A call runs on the
 device of its tensors. No reference counterpart.
+
+The operators of a forward or backward pass go through the compiled binding
+(csrc/python/block_calls.cpp), which makes the same checks; where one fails, or
+``ctx`` is given, or the tensors are on another device than the current one, the
+Python below makes the call and names what is wrong.
 """
 from __future__ import annotations
 
@@ -14,12 +19,29 @@ import ctypes
 
 import torch
 
-from raggedroute_b200._lib import Context, RRContext, check, lib
+from raggedroute_b200._lib import (Context, RaggedRouteError, RRContext, StatusCode, check, lib)
 from raggedroute_b200.ops import _need
 
 _MAX_SIZE = 2**31 - 1  # the entry points take sizes as int
 _DTYPES = {torch.float32: 0, torch.bfloat16: 2}
 ACTIVATIONS = {"silu": 0, "gelu_tanh": 1, "relu": 2}
+
+
+_calls = None
+
+
+def _load():
+    """The compiled binding (raises if it is missing)."""
+    global _calls
+    lib()
+    try:
+        from raggedroute_b200 import _block_calls
+    except ImportError as e:
+        raise RaggedRouteError(int(StatusCode.CUDA_ERROR), 0, f"{e}; run "
+                               "`python -m raggedroute_b200.build`", "load") from e
+    _block_calls.set_error(RaggedRouteError)
+    _calls = _block_calls
+    return _calls
 
 
 def _dtype(dtype: torch.dtype, name: str) -> int:
@@ -125,6 +147,10 @@ def grouped_gated_gemm(x_permuted: torch.Tensor, gate_weights: torch.Tensor,
     up_weights [E, K, N], h [R, N]; gate_up (float32 [R, 2N]) receives both
     products for the backward pass. activation: silu, gelu_tanh or relu.
     workspace from grouped_gated_gemm_workspace_size."""
+    if ctx is None and activation in ACTIVATIONS and (_calls or _load()).grouped_gated_gemm(
+            x_permuted, gate_weights, up_weights, offsets, h, gate_up, ACTIVATIONS[activation],
+            workspace):
+        return h
     dtype, act = _dtype(x_permuted.dtype, "x_permuted"), _activation(activation)
     sizes, inputs = _gated_inputs(x_permuted, gate_weights, up_weights, offsets)
     rows, _, _, output = sizes
@@ -147,6 +173,11 @@ def grouped_gated_gemm_backward(x_permuted: torch.Tensor, gate_weights: torch.Te
     (rr_grouped_gated_gemm_backward). dx [R, K] may be None, or both weight
     gradients [E, K, N]. workspace from
     grouped_gated_gemm_workspace_size(..., backward=True)."""
+    if ctx is None and activation in ACTIVATIONS and (
+            _calls or _load()).grouped_gated_gemm_backward(
+                x_permuted, gate_weights, up_weights, offsets, gate_up, dh, dx, d_gate_weights,
+                d_up_weights, ACTIVATIONS[activation], workspace):
+        return
     dtype, act = _dtype(x_permuted.dtype, "x_permuted"), _activation(activation)
     sizes, inputs = _gated_inputs(x_permuted, gate_weights, up_weights, offsets)
     rows, experts, hidden, output = sizes
@@ -175,6 +206,8 @@ def quantize_rows_int8(x: torch.Tensor, xq: torch.Tensor, x_scale: torch.Tensor,
     """Rows of x [R, K] in 8-bit integers with one scale each
     (rr_quantize_rows_int8): xq int8 [R, int8_row_stride(K)], x_scale float32
     [R]; x is close to xq * x_scale."""
+    if ctx is None and (_calls or _load()).quantize_rows_int8(x, xq, x_scale):
+        return
     dtype = _dtype(x.dtype, "x")
     _rank(x, 2, "x")
     rows, hidden = x.shape
@@ -208,6 +241,9 @@ def grouped_gemm_int8(xq: torch.Tensor, x_scale: torch.Tensor, wq: torch.Tensor,
     """y[r] = (xq[r] . wq[e]^T) * x_scale[r] * w_scale[e] for the rows of each
     expert's segment (rr_grouped_gemm_int8), from quantize_rows_int8 and
     quantize_expert_weights_int8; y_permuted [R, N] float32 or bfloat16."""
+    if ctx is None and (_calls or _load()).grouped_gemm_int8(xq, x_scale, wq, w_scale, offsets,
+                                                             y_permuted):
+        return y_permuted
     dtype = _dtype(y_permuted.dtype, "y_permuted")
     _rank(xq, 2, "xq")
     _rank(wq, 3, "wq")
@@ -264,6 +300,10 @@ def unpermute_norm(y_permuted: torch.Tensor, route_pos: torch.Tensor,
     gate, pre_gamma float32 [N]. Without post_gamma c is not normalised, without
     gate it is not scaled, and normed goes with pre_gamma. inv_rms (float32
     [T, 2]) receives what the backward pass needs."""
+    if ctx is None and (_calls or _load()).unpermute_norm(
+            y_permuted, route_pos, route_weights, residual, post_gamma, gate, pre_gamma,
+            residual_out, normed, inv_rms, eps, residual_scale):
+        return residual_out
     dtype = _dtype(residual.dtype, "residual")
     sizes, inputs = _norm_inputs(y_permuted, route_pos, route_weights, residual, post_gamma, gate,
                                  pre_gamma)
@@ -299,6 +339,11 @@ def unpermute_norm_backward(y_permuted: torch.Tensor, route_pos: torch.Tensor,
     d_residual [T, N] (may be d_residual_out), d_y_permuted [T * top_k, N],
     d_route_weights float32 [T, top_k] and the float32 [N] gradients of the
     parameters that are asked for."""
+    if ctx is None and (_calls or _load()).unpermute_norm_backward(
+            y_permuted, route_pos, route_weights, residual, post_gamma, gate, pre_gamma, inv_rms,
+            d_residual_out, d_normed, d_residual, d_y_permuted, d_route_weights, d_post_gamma,
+            d_gate, d_pre_gamma, residual_scale, workspace):
+        return
     dtype = _dtype(residual.dtype, "residual")
     sizes, inputs = _norm_inputs(y_permuted, route_pos, route_weights, residual, post_gamma, gate,
                                  pre_gamma)

@@ -185,3 +185,102 @@ def test_streams_side_by_side(cuda):
     torch.cuda.synchronize()
     for i, got in results:
         assert all(torch.equal(a, b) for a, b in zip(got, want[i]))
+
+
+def _calls(device, dtype):
+    """Each operator as (function, its tensors by name, other arguments, outputs)."""
+    t, k, n, e = 6, 32, 24, 3
+    f32 = torch.float32
+
+    def new(*shape, dtype=dtype):
+        return torch.zeros(*shape, dtype=dtype, device=device)
+
+    x, w = random((2 * t, k), 1, device, dtype=dtype), random((e, k, n), 2, device, dtype=dtype)
+    off = torch.tensor([0, 5, 5, 2 * t], dtype=torch.int32, device=device)
+    gated = dict(x_permuted=x, gate_weights=w, up_weights=w.clone(), offsets=off)
+    gu = random((2 * t, 2 * n), 3, device)
+    ws = new(rr.grouped_gated_gemm_workspace_size(2 * t, e, k, n, dtype, True), dtype=torch.uint8)
+    yield (rr.grouped_gated_gemm, dict(gated, h=new(2 * t, n), gate_up=new(2 * t, 2 * n, dtype=f32),
+                                       workspace=ws), dict(activation="gelu_tanh"), ["h", "gate_up"])
+    yield (rr.grouped_gated_gemm_backward,
+           dict(gated, gate_up=gu, dh=random((2 * t, n), 4, device, dtype=dtype), dx=new(2 * t, k),
+                d_gate_weights=new(e, k, n), d_up_weights=new(e, k, n), workspace=ws),
+           dict(activation="relu"), ["dx", "d_gate_weights", "d_up_weights"])
+    xq, xs = new(2 * t, k, dtype=torch.int8), new(2 * t, dtype=f32)
+    yield rr.quantize_rows_int8, dict(x=x, xq=xq, x_scale=xs), {}, ["xq", "x_scale"]
+    wq, sc = new(e, n, k, dtype=torch.int8), new(e, n, dtype=f32)
+    rr.quantize_expert_weights_int8(w, wq, sc)
+    yield (rr.grouped_gemm_int8, dict(xq=xq, x_scale=xs, wq=wq, w_scale=sc, offsets=off,
+                                      y_permuted=new(2 * t, n)), {}, ["y_permuted"])
+    norm = dict(y_permuted=random((2 * t, n), 5, device, dtype=dtype),
+                route_pos=torch.arange(2 * t, device=device).flip(0).int().view(t, 2),
+                route_weights=random((t, 2), 6, device), residual=random((t, n), 7, device, dtype=dtype),
+                post_gamma=random((n,), 8, device), gate=random((n,), 9, device),
+                pre_gamma=random((n,), 10, device))
+    inv = new(t, 2, dtype=f32)
+    yield (rr.unpermute_norm, dict(norm, residual_out=new(t, n), normed=new(t, n), inv_rms=inv),
+           dict(eps=1e-3, residual_scale=0.5), ["residual_out", "normed", "inv_rms"])
+    grads = dict(d_residual=new(t, n), d_y_permuted=new(2 * t, n),
+                 d_route_weights=new(t, 2, dtype=f32), d_post_gamma=new(n, dtype=f32),
+                 d_gate=new(n, dtype=f32), d_pre_gamma=new(n, dtype=f32))
+    yield (rr.unpermute_norm_backward,
+           dict(norm, inv_rms=inv, d_residual_out=random((t, n), 11, device, dtype=dtype),
+                d_normed=random((t, n), 12, device, dtype=dtype), **grads,
+                workspace=new(rr.unpermute_norm_backward_workspace_size(t, n), dtype=torch.uint8)),
+           dict(residual_scale=0.5), list(grads))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+def test_compiled_and_plain_calls(cuda, dtype, monkeypatch):
+    """A call through the compiled binding does what the Python one does, and
+    what the binding declines is named by the Python one."""
+    from raggedroute_b200 import expert_block
+
+    def unused(*_):
+        raise AssertionError("the Python path ran")
+
+    plain_call = expert_block._call
+    for fn, tensors, rest, outputs in _calls(cuda, dtype):
+        with monkeypatch.context() as m:
+            m.setattr(expert_block, "_call", unused)
+            fn(**tensors, **rest)
+        got = {k: tensors[k].clone() for k in outputs}
+        assert all(v.any() for v in got.values()), fn.__name__
+        for k in outputs:
+            tensors[k].zero_()
+        fn(**tensors, **rest, ctx=rr.Context())
+        for k in outputs:
+            assert torch.equal(got[k], tensors[k]), (fn.__name__, k)
+        assert expert_block._call is plain_call
+        for k, v in tensors.items():
+            if k == "workspace":
+                continue
+            wrong = [torch.cat([v, v]), v.cpu(), v.double(),
+                     torch.cat([v, v], -1).as_strided(v.shape, [2 * s for s in v.stride()])]
+            for i, bad in enumerate(wrong):
+                with pytest.raises((TypeError, ValueError)):
+                    fn(**{**tensors, k: bad}, **rest)
+        last = outputs[0]
+        source = next(k for k, v in tensors.items() if k not in outputs and k != "workspace"
+                      and v.dtype == tensors[last].dtype and v.numel() == tensors[last].numel()) \
+            if fn is rr.unpermute_norm_backward else None
+        if source is not None:  # an output that is an input: refused by the entry point
+            with pytest.raises(rr.RaggedRouteError, match="unpermute_norm_backward: INVALID"):
+                fn(**{**tensors, last: tensors[source]}, **rest)
+    torch.cuda.synchronize()
+
+
+def test_compiled_call_uses_the_current_stream(cuda):
+    fn, tensors, rest, outputs = next(_calls(cuda, torch.float32))
+    fn(**tensors, **rest)
+    want = tensors["h"].clone()
+    tensors["h"].zero_()
+    stream = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        fn(**tensors, **rest)
+    assert not tensors["h"].any()  # captured, not run
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(tensors["h"], want)
