@@ -337,6 +337,7 @@ __global__ void __launch_bounds__(kThreads, 1) expert_gemm_kernel(
     tmem_alloc_pair(&s.tmem_base, kTmemCols);
     tmem_relinquish_pair();
   }
+  follow_previous();
   int total;
   if constexpr (kMode == kDw) {
     total = p.experts * ((p.hidden + kTileM - 1) / kTileM) * n_tiles;
@@ -761,27 +762,8 @@ cudaError_t launch_engine(const CUtensorMap (&maps)[4], EngineArgs args, long lo
   if (tiles < units) units = static_cast<int>(tiles);
   if (units <= 0) return cudaSuccess;
   args.err = device_error_word();
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 2;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(2 * units, 1, 1);
-  cfg.blockDim = dim3(kThreads, 1, 1);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(
-      &cfg, expert_gemm_kernel<kMode, kPa, kPb, T>, maps[0], maps[1], maps[2], maps[3],
-      args);
-  if (e != cudaSuccess) {
-    cudaGetLastError();
-    return e;
-  }
-  note_launch();
-  return cudaSuccess;
+  return launch_following(expert_gemm_kernel<kMode, kPa, kPb, T>, dim3(2 * units), kThreads, smem, 2,
+                          stream, maps[0], maps[1], maps[2], maps[3], args);
 }
 
 // Output tiles of the row modes, at most: every expert with rows may end in a

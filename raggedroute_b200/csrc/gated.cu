@@ -198,6 +198,7 @@ __global__ void __launch_bounds__(kFewThreads, kR == 1 ? 4 : 2) gated_few_kernel
     const int32_t* __restrict__ offsets, T* __restrict__ h, float* __restrict__ gate_up, int rows,
     int experts, int hidden, int output, int activation, int split) {
   __shared__ FewSmem smem;
+  follow_previous();
   const int row = blockIdx.y;
   const int e = expert_of(offsets, row, rows, experts);
   // Uniform over a cluster, whose blocks share the row.
@@ -227,30 +228,12 @@ cudaError_t few(const void* x, const void* wg, const void* wu, const int32_t* of
          steps >= 8 * split) {
     split *= 2;
   }
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = split;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(groups * split, rows);
-  cfg.blockDim = dim3(kFewThreads);
-  cfg.stream = stream;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(
-      &cfg,
-      vec ? (single ? gated_few_kernel<T, kVec, 1> : gated_few_kernel<T, kVec, kFewRows>)
-          : (single ? gated_few_kernel<T, 1, 1> : gated_few_kernel<T, 1, kFewRows>),
-      static_cast<const T*>(x),
-      static_cast<const T*>(wg), static_cast<const T*>(wu), offsets, static_cast<T*>(h), gate_up,
-      rows, experts, hidden, output, activation, split);
-  if (e != cudaSuccess) {
-    cudaGetLastError();
-    return e;
-  }
-  note_launch();
-  return cudaSuccess;
+  auto* kernel = vec ? (single ? gated_few_kernel<T, kVec, 1> : gated_few_kernel<T, kVec, kFewRows>)
+                     : (single ? gated_few_kernel<T, 1, 1> : gated_few_kernel<T, 1, kFewRows>);
+  return launch_following(kernel, dim3(groups * split, rows), kFewThreads, 0, split, stream,
+                          static_cast<const T*>(x), static_cast<const T*>(wg),
+                          static_cast<const T*>(wu), offsets, static_cast<T*>(h), gate_up, rows,
+                          experts, hidden, output, activation, split);
 }
 
 // ---- gradients of few rows ------------------------------------------------------------
@@ -318,6 +301,7 @@ __global__ void __launch_bounds__(kFewThreads) gated_few_dx_kernel(
     const float* __restrict__ dg, const float* __restrict__ du, const T* __restrict__ wg,
     const T* __restrict__ wu, const int32_t* __restrict__ offsets, T* __restrict__ dx, int rows,
     int experts, int hidden, int output) {
+  follow_previous();
   const int row = blockIdx.y;
   const int e = expert_of(offsets, row, rows, experts);
   if (e == experts) return;
@@ -344,6 +328,7 @@ __global__ void __launch_bounds__(kFewThreads) gated_few_dw_kernel(
     const T* __restrict__ x, const float* __restrict__ dg, const float* __restrict__ du,
     const int32_t* __restrict__ offsets, T* __restrict__ dwg, T* __restrict__ dwu, int rows,
     int hidden, int output, int k_blocks) {
+  follow_previous();
   // Experts and blocks of k share the y axis of the grid.
   const int e = blockIdx.y / k_blocks;
   const int lane = threadIdx.x & 31;
@@ -451,6 +436,7 @@ constexpr int kPackThreads = 256;
 // The operands of a call are packed by one launch.
 template <typename T, int kTerms>
 __global__ void __launch_bounds__(kPackThreads) pack_terms_kernel(const PackJobs jobs) {
+  follow_previous();
   long long first = static_cast<long long>(blockIdx.x) * kPackThreads + threadIdx.x;
   const long long step = static_cast<long long>(gridDim.x) * kPackThreads;
   for (int q = 0; q < jobs.count; ++q) {
@@ -494,6 +480,7 @@ template <typename T, int kTerms, bool kVec>
 __global__ void __launch_bounds__(kPackThreads) gated_pointwise_backward_kernel(
     const float* __restrict__ gate_up, const T* __restrict__ dh, __nv_bfloat16* __restrict__ dg,
     __nv_bfloat16* __restrict__ du, int rows, int output, int ld, int activation) {
+  follow_previous();
   const int groups = ld >> 3;
   const long long total = static_cast<long long>(rows) * groups;
   const long long plane = static_cast<long long>(rows) * ld;
@@ -542,6 +529,7 @@ template <typename T>
 __global__ void __launch_bounds__(kPackThreads) gated_pointwise_backward_f32_kernel(
     const float* __restrict__ gate_up, const T* __restrict__ dh, float* __restrict__ dg,
     float* __restrict__ du, long long total, int output, int activation) {
+  follow_previous();
   for (long long i = static_cast<long long>(blockIdx.x) * kPackThreads + threadIdx.x; i < total;
        i += static_cast<long long>(gridDim.x) * kPackThreads) {
     const long long r = total <= INT_MAX ? static_cast<int>(i) / output : i / output;
@@ -578,13 +566,9 @@ cudaError_t launch_pack_terms(const PackJobs& jobs, Dtype dtype, cudaStream_t st
   for (int q = 0; q < jobs.count; ++q) total += jobs.job[q].rows * (jobs.job[q].ld >> 3);
   const int blocks = pack_blocks(total);
   if (blocks == 0) return cudaSuccess;
-  if (dtype == Dtype::kBf16) {
-    pack_terms_kernel<__nv_bfloat16, 1><<<blocks, kPackThreads, 0, stream>>>(jobs);
-  } else {
-    pack_terms_kernel<float, 3><<<blocks, kPackThreads, 0, stream>>>(jobs);
-  }
-  note_launch();
-  return cudaGetLastError();
+  auto* kernel = dtype == Dtype::kBf16 ? pack_terms_kernel<__nv_bfloat16, 1>
+                                       : pack_terms_kernel<float, 3>;
+  return launch_following(kernel, dim3(blocks), kPackThreads, 0, 0, stream, jobs);
 }
 
 cudaError_t launch_gated_pointwise_backward(const float* gate_up, const void* dh,
@@ -601,16 +585,13 @@ cudaError_t launch_gated_pointwise_backward(const float* gate_up, const void* dh
                               : gated_pointwise_backward_kernel<__nv_bfloat16, 2, false>)
                        : (vec ? gated_pointwise_backward_kernel<__nv_bfloat16, 1, true>
                               : gated_pointwise_backward_kernel<__nv_bfloat16, 1, false>);
-    kernel<<<blocks, kPackThreads, 0, stream>>>(gate_up, static_cast<const __nv_bfloat16*>(dh), dg,
-                                                du, rows, output, ld, act);
-  } else {
-    auto* kernel = vec ? gated_pointwise_backward_kernel<float, 3, true>
-                       : gated_pointwise_backward_kernel<float, 3, false>;
-    kernel<<<blocks, kPackThreads, 0, stream>>>(gate_up, static_cast<const float*>(dh), dg, du,
-                                                rows, output, ld, act);
+    return launch_following(kernel, dim3(blocks), kPackThreads, 0, 0, stream, gate_up,
+                            static_cast<const __nv_bfloat16*>(dh), dg, du, rows, output, ld, act);
   }
-  note_launch();
-  return cudaGetLastError();
+  auto* kernel = vec ? gated_pointwise_backward_kernel<float, 3, true>
+                     : gated_pointwise_backward_kernel<float, 3, false>;
+  return launch_following(kernel, dim3(blocks), kPackThreads, 0, 0, stream, gate_up,
+                          static_cast<const float*>(dh), dg, du, rows, output, ld, act);
 }
 
 cudaError_t launch_gated_pointwise_backward_f32(const float* gate_up, const void* dh, float* dg,
@@ -621,14 +602,13 @@ cudaError_t launch_gated_pointwise_backward_f32(const float* gate_up, const void
   const int blocks = pack_blocks(total);
   const int act = static_cast<int>(activation);
   if (dtype == Dtype::kBf16) {
-    gated_pointwise_backward_f32_kernel<<<blocks, kPackThreads, 0, stream>>>(
-        gate_up, static_cast<const __nv_bfloat16*>(dh), dg, du, total, output, act);
-  } else {
-    gated_pointwise_backward_f32_kernel<<<blocks, kPackThreads, 0, stream>>>(
-        gate_up, static_cast<const float*>(dh), dg, du, total, output, act);
+    return launch_following(gated_pointwise_backward_f32_kernel<__nv_bfloat16>, dim3(blocks),
+                            kPackThreads, 0, 0, stream, gate_up,
+                            static_cast<const __nv_bfloat16*>(dh), dg, du, total, output, act);
   }
-  note_launch();
-  return cudaGetLastError();
+  return launch_following(gated_pointwise_backward_f32_kernel<float>, dim3(blocks), kPackThreads, 0,
+                          0, stream, gate_up, static_cast<const float*>(dh), dg, du, total, output,
+                          act);
 }
 
 namespace {
@@ -640,11 +620,9 @@ cudaError_t few_dx_launch(const float* dg, const float* du, const void* wg, cons
   constexpr int kVec = 16 / sizeof(T);
   const bool vec = output % kVec == 0 && aligned_to(wg, 16) && aligned_to(wu, 16);
   auto* kernel = vec ? gated_few_dx_kernel<T, kVec> : gated_few_dx_kernel<T, 1>;
-  kernel<<<dim3(ceil_div(hidden, kFewWarps * kDxRows), rows), kFewThreads, 0, stream>>>(
-      dg, du, static_cast<const T*>(wg), static_cast<const T*>(wu), offsets, static_cast<T*>(dx),
-      rows, experts, hidden, output);
-  note_launch();
-  return cudaGetLastError();
+  return launch_following(kernel, dim3(ceil_div(hidden, kFewWarps * kDxRows), rows), kFewThreads, 0,
+                          0, stream, dg, du, static_cast<const T*>(wg), static_cast<const T*>(wu),
+                          offsets, static_cast<T*>(dx), rows, experts, hidden, output);
 }
 
 template <typename T>
@@ -661,12 +639,10 @@ cudaError_t few_dw_launch(const void* x, const float* dg, const float* du, const
   for (int e = 0; e < experts; e += slice) {
     const int count = experts - e < slice ? experts - e : slice;
     const long long at = static_cast<long long>(e) * hidden * output;
-    kernel<<<dim3(ceil_div(output, 32 * (vec ? kVec : 1)), count * k_blocks), kFewThreads, 0,
-             stream>>>(static_cast<const T*>(x), dg, du, offsets + e,
-                       static_cast<T*>(dwg) + at, static_cast<T*>(dwu) + at, rows, hidden, output,
-                       k_blocks);
-    note_launch();
-    const cudaError_t err = cudaGetLastError();
+    const cudaError_t err = launch_following(
+        kernel, dim3(ceil_div(output, 32 * (vec ? kVec : 1)), count * k_blocks), kFewThreads, 0, 0,
+        stream, static_cast<const T*>(x), dg, du, offsets + e, static_cast<T*>(dwg) + at,
+        static_cast<T*>(dwu) + at, rows, hidden, output, k_blocks);
     if (err != cudaSuccess) return err;
   }
   return cudaSuccess;

@@ -53,6 +53,7 @@ __global__ void __launch_bounds__(kRowThreads) quantize_rows_kernel(
     int ld) {
   constexpr int kPer = kVec ? 16 / sizeof(T) : 4;  // values per thread and step
   __shared__ uint32_t tops[kRowThreads / 32];
+  follow_previous();
   const long long row = blockIdx.x;
   const T* src = x + row * cols;
   int8_t* dst = xq + row * ld;
@@ -142,6 +143,7 @@ __global__ void __launch_bounds__(32 * kRowWarps) quantize_rows_warp_kernel(
     const T* __restrict__ x, int8_t* __restrict__ xq, float* __restrict__ x_scale, int rows,
     int cols, int ld) {
   constexpr int kPer = 16 / sizeof(T);
+  follow_previous();
   const int lane = threadIdx.x & 31;
   const long long row = static_cast<long long>(blockIdx.x) * kRowWarps + (threadIdx.x >> 5);
   if (row >= rows) return;
@@ -197,14 +199,11 @@ cudaError_t quantize_rows(const T* x, int8_t* xq, float* x_scale, int rows, int 
   if (vec && places <= 32 * 16) {
     auto* kernel = places <= 32 * 4 ? quantize_rows_warp_kernel<T, 4>
                                     : quantize_rows_warp_kernel<T, 16>;
-    kernel<<<ceil_div(rows, kRowWarps), 32 * kRowWarps, 0, stream>>>(x, xq, x_scale, rows, cols,
-                                                                     ld);
-  } else {
-    auto* kernel = vec ? quantize_rows_kernel<T, true> : quantize_rows_kernel<T, false>;
-    kernel<<<rows, kRowThreads, 0, stream>>>(x, xq, x_scale, cols, ld);
+    return launch_following(kernel, dim3(ceil_div(rows, kRowWarps)), 32 * kRowWarps, 0, 0, stream,
+                            x, xq, x_scale, rows, cols, ld);
   }
-  note_launch();
-  return cudaGetLastError();
+  auto* kernel = vec ? quantize_rows_kernel<T, true> : quantize_rows_kernel<T, false>;
+  return launch_following(kernel, dim3(rows), kRowThreads, 0, 0, stream, x, xq, x_scale, cols, ld);
 }
 
 // ---- weights -----------------------------------------------------------------------
@@ -336,6 +335,7 @@ __global__ void __launch_bounds__(kFewThreads) int8_few_kernel(
     const int32_t* __restrict__ offsets, T* __restrict__ y, int rows, int experts, int ld,
     int output) {
   __shared__ int owner;
+  follow_previous();
   if (threadIdx.x == 0) owner = experts;
   __syncthreads();
   const int row = blockIdx.y;
@@ -390,16 +390,12 @@ cudaError_t launch_int8_few(const int8_t* xq, const float* x_scale, const int8_t
                             int experts, int ld, int output, Dtype dtype, cudaStream_t stream) {
   const dim3 grid(ceil_div(output, kCols * (kFewThreads / 32)), rows);
   if (dtype == Dtype::kBf16) {
-    int8_few_kernel<<<grid, kFewThreads, 0, stream>>>(xq, x_scale, wq, w_scale, offsets,
-                                                      static_cast<__nv_bfloat16*>(y), rows,
-                                                      experts, ld, output);
-  } else {
-    int8_few_kernel<<<grid, kFewThreads, 0, stream>>>(xq, x_scale, wq, w_scale, offsets,
-                                                      static_cast<float*>(y), rows, experts, ld,
-                                                      output);
+    return launch_following(int8_few_kernel<__nv_bfloat16>, grid, kFewThreads, 0, 0, stream, xq,
+                            x_scale, wq, w_scale, offsets, static_cast<__nv_bfloat16*>(y), rows,
+                            experts, ld, output);
   }
-  note_launch();
-  return cudaGetLastError();
+  return launch_following(int8_few_kernel<float>, grid, kFewThreads, 0, 0, stream, xq, x_scale, wq,
+                          w_scale, offsets, static_cast<float*>(y), rows, experts, ld, output);
 }
 
 }  // namespace rrb

@@ -122,6 +122,7 @@ __global__ void __launch_bounds__(kMaxThreads) unpermute_norm_kernel(const Unper
                                                                      T* residual_out, T* normed,
                                                                      float* inv_rms) {
   __shared__ float parts[2][32];
+  follow_previous();
   const long long t = blockIdx.x;
   const long long row = t * in.output;
   const float per_col = 1.0f / static_cast<float>(in.output);
@@ -201,6 +202,7 @@ __global__ void __launch_bounds__(kMaxThreads) unpermute_norm_backward_kernel(
     const UnpermuteNorm in, const UnpermuteNormGrads g, float* partial) {
   __shared__ float parts[2][32];
   __shared__ float dots[kMaxTopK][32];
+  follow_previous();
   const long long routes = static_cast<long long>(in.tokens) * in.top_k;
   const float per_col = 1.0f / static_cast<float>(in.output);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -662,6 +664,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1) unpermute_norm_stream_kerne
   __shared__ StreamSmem s;
   __shared__ float parts[2][kMaxTeams];  // sums of each warp
   stream_setup(st, in.top_k, s);
+  follow_previous();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int team = threadIdx.x / st.team, tid = threadIdx.x % st.team;
   const int team_warps = st.team >> 5, warp0 = team * team_warps;
@@ -866,6 +869,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1) unpermute_norm_backward_str
   const int ring_size = st.stages * st.sources * st.stride;
   float* pg = reinterpret_cast<float*>(rings + st.teams * ring_size);
   float* shared_pre = pg + st.padded;
+  follow_previous();
   for (int c = threadIdx.x; c < st.padded; c += blockDim.x) {
     float f, p;  // zero from column n on; column padded - 8 is past the end
     column_factors<1>(in, c, &f, &p);
@@ -1106,6 +1110,7 @@ __global__ void __launch_bounds__(kSumCols* kSumGroups) column_sums_kernel(
     const float* __restrict__ partial, int blocks, int output, float* d_post, float* d_gate,
     float* d_pre) {
   __shared__ float parts[kSumGroups][kSumCols];
+  follow_previous();
   float* out = blockIdx.y == 0 ? d_post : (blockIdx.y == 1 ? d_gate : d_pre);
   if (out == nullptr) return;
   const int lane = threadIdx.x % kSumCols, group = threadIdx.x / kSumCols;
@@ -1229,20 +1234,18 @@ cudaError_t forward(const UnpermuteNorm& in, void* residual_out, void* normed, f
   if (threads > 512) threads = row_threads(in.output, kElems);
   auto* kernel = threads <= 512 ? unpermute_norm_kernel<T, kPer, 512>
                                 : unpermute_norm_kernel<T, kPer, 1024>;
-  kernel<<<in.tokens, threads, 0, stream>>>(in, static_cast<T*>(residual_out),
-                                            static_cast<T*>(normed), inv_rms);
-  note_launch();
-  return cudaGetLastError();
+  return launch_following(kernel, dim3(in.tokens), threads, 0, 0, stream, in,
+                          static_cast<T*>(residual_out), static_cast<T*>(normed), inv_rms);
 }
 
 cudaError_t column_sums(const float* workspace, int parts, int output,
                         const UnpermuteNormGrads& g, cudaStream_t stream) {
-  if (g.d_post_gamma != nullptr || g.d_gate != nullptr || g.d_pre_gamma != nullptr) {
-    column_sums_kernel<<<dim3(ceil_div(output, kSumCols), 3), kSumCols * kSumGroups, 0, stream>>>(
-        workspace, parts, output, g.d_post_gamma, g.d_gate, g.d_pre_gamma);
-    note_launch();
+  if (g.d_post_gamma == nullptr && g.d_gate == nullptr && g.d_pre_gamma == nullptr) {
+    return cudaSuccess;
   }
-  return cudaGetLastError();
+  return launch_following(column_sums_kernel, dim3(ceil_div(output, kSumCols), 3),
+                          kSumCols * kSumGroups, 0, 0, stream, workspace, parts, output,
+                          g.d_post_gamma, g.d_gate, g.d_pre_gamma);
 }
 
 template <typename T, int kPer>
@@ -1252,9 +1255,8 @@ cudaError_t backward(const UnpermuteNorm& in, const UnpermuteNormGrads& g, float
   const int blocks = backward_blocks(in.tokens, in.output);
   auto* kernel = threads <= 512 ? unpermute_norm_backward_kernel<T, kPer, 512>
                                 : unpermute_norm_backward_kernel<T, kPer, 1024>;
-  kernel<<<blocks, threads, 0, stream>>>(in, g, workspace);
-  note_launch();
-  const cudaError_t e = cudaGetLastError();
+  const cudaError_t e =
+      launch_following(kernel, dim3(blocks), threads, 0, 0, stream, in, g, workspace);
   if (e != cudaSuccess) return e;
   return column_sums(workspace, blocks, in.output, g, stream);
 }
@@ -1264,11 +1266,9 @@ cudaError_t forward_stream(const UnpermuteNorm& in, const Stream& st, void* resi
                            void* normed, float* inv_rms, cudaStream_t stream) {
   constexpr auto kernel = unpermute_norm_stream_kernel<T, kPer>;
   if (!allow_ring<kernel>()) return cudaErrorNotSupported;
-  kernel<<<st.blocks, st.team * st.teams, ring_bytes(st), stream>>>(
-      in, st, static_cast<T*>(residual_out), static_cast<T*>(normed), inv_rms,
-      device_error_word());
-  note_launch();
-  return cudaGetLastError();
+  return launch_following(kernel, dim3(st.blocks), st.team * st.teams, ring_bytes(st), 0, stream,
+                          in, st, static_cast<T*>(residual_out), static_cast<T*>(normed), inv_rms,
+                          device_error_word());
 }
 
 template <typename T, int kPer>
@@ -1282,10 +1282,9 @@ cudaError_t backward_stream(const UnpermuteNorm& in, const Stream& st, const Unp
     return cudaErrorNotSupported;
   }
   auto* kernel = eight ? (two ? narrow2 : narrow) : wide;
-  kernel<<<st.blocks, st.team * st.teams, ring_bytes(st), stream>>>(in, st, g, workspace,
-                                                                    device_error_word());
-  note_launch();
-  const cudaError_t e = cudaGetLastError();
+  const cudaError_t e = launch_following(kernel, dim3(st.blocks), st.team * st.teams,
+                                         ring_bytes(st), 0, stream, in, st, g, workspace,
+                                         device_error_word());
   if (e != cudaSuccess) return e;
   return column_sums(workspace, st.blocks, in.output, g, stream);
 }

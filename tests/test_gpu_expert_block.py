@@ -284,3 +284,89 @@ def test_compiled_call_uses_the_current_stream(cuda):
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(tensors["h"], want)
+
+
+def test_captured_over_two_streams(cuda):
+    """Kernels that start behind a fork, a copy, a memset and a join of streams,
+    as captured and replayed with new inputs."""
+    t, n = 700, 512
+    yp, res = random((2 * t, n), 1, cuda), random((t, n), 2, cuda)
+    pos = torch.randperm(2 * t, device=cuda).int().view(t, 2)
+    w, ones = random((t, 2), 3, cuda), torch.ones(n, device=cuda)
+    q, sc = torch.empty(t, n, dtype=torch.int8, device=cuda), torch.empty(t, device=cuda)
+    bufs = [torch.empty(t, n, device=cuda) for _ in range(5)]
+    q2, sc2 = torch.empty_like(q), torch.empty_like(sc)
+
+    def run(side):
+        main = torch.cuda.current_stream()
+        a, an, b, bn, c = bufs
+        rr.unpermute_norm(yp, pos, w, res, a, an, post_gamma=ones, pre_gamma=ones)
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            rr.quantize_rows_int8(an, q, sc)           # behind the fork
+            c.copy_(an)
+            rr.unpermute_norm(yp, pos, w, c, c)        # behind a copy, in place
+        rr.unpermute_norm(yp, pos, w, a, b, bn, gate=ones, pre_gamma=ones)
+        main.wait_stream(side)
+        rr.unpermute_norm(yp, pos, w, c, bn, residual_scale=0.5)  # behind the join
+        c.zero_()
+        rr.quantize_rows_int8(bn, q2, sc2)             # behind a memset
+
+    side = torch.cuda.Stream()
+    run(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run(side)
+    for seed in range(3):
+        yp.copy_(random((2 * t, n), 10 + seed, cuda))
+        res.copy_(random((t, n), 20 + seed, cuda))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [x.clone() for x in (*bufs, q, sc, q2, sc2)]
+        run(side)
+        torch.cuda.synchronize()
+        assert all(torch.equal(g, x) for g, x in zip(got, (*bufs, q, sc, q2, sc2)))
+        # The eager pass, kernel by kernel.
+        a = torch.empty_like(res)
+        an = torch.empty_like(res)
+        rr.unpermute_norm(yp, pos, w, res, a, an, post_gamma=ones, pre_gamma=ones)
+        torch.cuda.synchronize()
+        c = an.clone()
+        torch.cuda.synchronize()
+        rr.unpermute_norm(yp, pos, w, c, c)
+        torch.cuda.synchronize()
+        last = torch.empty_like(c)
+        rr.unpermute_norm(yp, pos, w, c, last, residual_scale=0.5)
+        torch.cuda.synchronize()
+        assert torch.equal(bufs[3], last) and torch.equal(bufs[0], a)
+
+
+def test_chain_of_calls_with_no_pause(cuda):
+    """Kernels of a long run of dependent calls start behind one another; each
+    reads what the one before it wrote (and overwrites what it read)."""
+    t, n = 3, 4096
+    yp = random((2 * t, n), 1, cuda, std=0.1)
+    pos = torch.arange(2 * t, device=cuda).int().view(t, 2)
+    w, ones = random((t, 2), 2, cuda), torch.ones(n, device=cuda)
+    start = random((t, n), 3, cuda)
+
+    def run(pause):
+        x = start.clone()
+        q, sc = torch.empty(t, n, dtype=torch.int8, device=cuda), torch.empty(t, device=cuda)
+        normed = torch.empty_like(x)
+        out = []
+        for i in range(200):
+            rr.unpermute_norm(yp, pos, w, x, x, normed, post_gamma=ones, pre_gamma=ones)
+            if pause:
+                torch.cuda.synchronize()
+            rr.quantize_rows_int8(normed, q, sc)
+            if pause:
+                torch.cuda.synchronize()
+            rr.unpermute_norm(yp, pos, w, normed, x, residual_scale=0.9)
+            if i % 50 == 49:
+                out += [x.clone(), q.clone(), sc.clone()]
+        return out
+
+    want, got = run(True), run(False)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
