@@ -92,6 +92,69 @@ __device__ __forceinline__ void unpack16(const uint4 v, float* f) {
   }
 }
 
+// Bytes skip to skip + 15 of two 16-byte granules (skip < 16, a multiple of
+// sizeof(T)); values from the `count`th on become zero.
+template <typename T>
+__device__ __forceinline__ uint4 shift16(const uint4 a, const uint4 b, uint32_t skip, int count) {
+  constexpr int kPer = 4 / sizeof(T);  // values in a word
+  uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+  const bool two = skip & 8u, one = skip & 4u;
+#pragma unroll
+  for (int i = 0; i < 6; ++i) w[i] = two ? w[i + 2] : w[i];
+#pragma unroll
+  for (int i = 0; i < 5; ++i) w[i] = one ? w[i + 1] : w[i];
+  if constexpr (sizeof(T) == 2) {
+    const uint32_t bits = (skip & 3u) * 8;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], bits);
+  }
+  if (count < 4 * kPer) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int left = count - kPer * i;
+      w[i] = left >= kPer ? w[i] : (left > 0 ? w[i] & 0xFFFFu : 0u);
+    }
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// A granule at `at` of which only the values in [begin, end) exist; the others
+// read as zero.
+template <typename T>
+__device__ __forceinline__ uint4 part16(uintptr_t at, const T* begin, const T* end) {
+  uint32_t w[4];
+  auto value = [&](int byte) -> uint32_t {
+    const T* p = reinterpret_cast<const T*>(at + byte);
+    if (p < begin || p >= end) return 0u;
+    if constexpr (sizeof(T) == 2) return __ldg(reinterpret_cast<const unsigned short*>(p));
+    else return __ldg(reinterpret_cast<const unsigned*>(p));
+  };
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    w[i] = value(4 * i);
+    if constexpr (sizeof(T) == 2) w[i] |= value(4 * i + 2) << 16;
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// The 16 bytes from p on, wherever p lies: the two granules around them are loaded
+// whole (neighbouring threads share them in L1), or, where one reaches past the
+// buffer [begin, end), the `count` values that exist.
+template <typename T>
+__device__ __forceinline__ uint4 load16(const T* p, const T* begin, const T* end, int count) {
+  const auto at = reinterpret_cast<uintptr_t>(p) & ~static_cast<uintptr_t>(15);
+  const auto skip = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)) & 15u;
+  uint4 a, b;
+  if (at >= reinterpret_cast<uintptr_t>(begin) && at + 32 <= reinterpret_cast<uintptr_t>(end)) {
+    a = __ldg(reinterpret_cast<const uint4*>(at));
+    b = __ldg(reinterpret_cast<const uint4*>(at) + 1);
+  } else {
+    a = part16<T>(at, begin, end);
+    b = part16<T>(at + 16, begin, end);
+  }
+  return shift16<T>(a, b, skip, count);
+}
+
 template <typename T>
 __device__ __forceinline__ uint4 pack16(const float* f) {
   if constexpr (sizeof(T) == 2) {
@@ -195,12 +258,13 @@ struct PackJob {
   long long rows = 0;
   int cols = 0;
   int ld = 0;
+  int shift = 0, step_rows = 0, step_groups = 0;  // filled in by the launch
 };
 struct PackJobs {
   PackJob job[3];
   int count = 0;
 };
-cudaError_t launch_pack_terms(const PackJobs& jobs, Dtype dtype, cudaStream_t stream);
+cudaError_t launch_pack_terms(PackJobs jobs, Dtype dtype, cudaStream_t stream);
 // dg = dh u act'(g), du = dh act(g) from gate_up [rows][2 output], written as
 // [parts][rows][ld] bfloat16 parts.
 cudaError_t launch_gated_pointwise_backward(const float* gate_up, const void* dh,

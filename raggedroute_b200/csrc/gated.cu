@@ -430,6 +430,25 @@ __device__ __forceinline__ void store_parts(__nv_bfloat16* dst, long long plane,
 
 constexpr int kPackThreads = 256;
 
+// Eight values as they lie in memory.
+template <typename T>
+struct Raw8 {
+  static constexpr int kPer = 16 / sizeof(T), kPieces = 8 / kPer;
+  uint4 w[kPieces];
+  __device__ __forceinline__ void load_aligned(const T* p) {
+#pragma unroll
+    for (int j = 0; j < kPieces; ++j) w[j] = __ldg(reinterpret_cast<const uint4*>(p) + j);
+  }
+  __device__ __forceinline__ void load(const T* p, const T* begin, const T* end, int count) {
+#pragma unroll
+    for (int j = 0; j < kPieces; ++j) w[j] = load16<T>(p + kPer * j, begin, end, count - kPer * j);
+  }
+  __device__ __forceinline__ void get(float (&v)[8]) const {
+#pragma unroll
+    for (int j = 0; j < kPieces; ++j) unpack16<T>(w[j], v + kPer * j);
+  }
+};
+
 // One thread packs eight columns: bound by the bytes (FP32: 4 read, 6 written
 // per element; 6.2 TB/s at 64 x 1024 x 1024). Runs only for FP32 operands and
 // for row strides that are no multiple of 16 bytes, which TMA cannot read.
@@ -437,35 +456,42 @@ constexpr int kPackThreads = 256;
 template <typename T, int kTerms>
 __global__ void __launch_bounds__(kPackThreads) pack_terms_kernel(const PackJobs jobs) {
   follow_previous();
-  long long first = static_cast<long long>(blockIdx.x) * kPackThreads + threadIdx.x;
-  const long long step = static_cast<long long>(gridDim.x) * kPackThreads;
+  const int index = static_cast<int>(blockIdx.x) * kPackThreads + static_cast<int>(threadIdx.x);
+  const int step = static_cast<int>(gridDim.x) * kPackThreads;
   for (int q = 0; q < jobs.count; ++q) {
     const PackJob& job = jobs.job[q];
     const int groups = job.ld >> 3;
     const long long total = job.rows * groups;
     const long long plane = job.rows * job.ld;
+    const T* src = static_cast<const T*>(job.src);
+    const T* end = src + job.rows * job.cols;
     const bool vec = (job.cols * sizeof(T)) % 16 == 0;  // such rows are 16-byte aligned
+    // A job goes on where the one before it left the grid. Row and group of an
+    // item are carried along: a division for each costs more than its bytes.
+    const int first = index < job.shift ? index - job.shift + step : index - job.shift;
+    int c = first % groups;
+    long long r = first / groups;
     for (long long i = first; i < total; i += step) {
-      const long long r =
-          total <= INT_MAX ? static_cast<int>(i) / groups : i / groups;  // 32 bits where they do
-      const int c = static_cast<int>(i - r * groups) << 3;
-      const T* p = static_cast<const T*>(job.src) + r * job.cols + c;
-      float v[8];
-      if (vec && c + 8 <= job.cols) {
-        constexpr int kPer = 16 / sizeof(T);
-#pragma unroll
-        for (int j = 0; j < 8 / kPer; ++j) {
-          unpack16<T>(__ldg(reinterpret_cast<const uint4*>(p) + j), v + j * kPer);
-        }
+      const T* p = src + r * job.cols + 8 * c;
+      const int count = job.cols - 8 * c;
+      Raw8<T> raw;
+      if (vec && count >= 8) raw.load_aligned(p);
+      else raw.load(p, src, end, count);
+      __nv_bfloat16* dst = job.dst + 8 * i;  // ld is 8 * groups
+      if constexpr (sizeof(T) == 2 && kTerms == 1) {
+        *reinterpret_cast<uint4*>(dst) = raw.w[0];
       } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = c + j < job.cols ? to_f32(__ldg(p + j)) : 0.0f;
+        float v[8];
+        raw.get(v);
+        store_parts<kTerms>(dst, plane, v);
       }
-      store_parts<kTerms>(job.dst + r * job.ld + c, plane, v);
+      r += job.step_rows;
+      c += job.step_groups;
+      if (c >= groups) {
+        c -= groups;
+        ++r;
+      }
     }
-    // The next job goes on where this one left the grid.
-    first = (first - total) % step;
-    if (first < 0) first += step;
   }
 }
 
@@ -492,26 +518,21 @@ __global__ void __launch_bounds__(kPackThreads) gated_pointwise_backward_kernel(
     const float* pu = pg + output;
     const T* pd = dh + r * output + c;
     float g[8], u[8], d[8];
+    Raw8<float> rg, ru;
+    Raw8<T> rd;
     if (kVec && c + 8 <= output) {
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        unpack16<float>(__ldg(reinterpret_cast<const uint4*>(pg) + j), g + 4 * j);
-        unpack16<float>(__ldg(reinterpret_cast<const uint4*>(pu) + j), u + 4 * j);
-      }
-      constexpr int kPer = 16 / sizeof(T);
-#pragma unroll
-      for (int j = 0; j < 8 / kPer; ++j) {
-        unpack16<T>(__ldg(reinterpret_cast<const uint4*>(pd) + j), d + j * kPer);
-      }
+      rg.load_aligned(pg);
+      ru.load_aligned(pu);
+      rd.load_aligned(pd);
     } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const bool in = c + j < output;
-        g[j] = in ? __ldg(pg + j) : 0.0f;
-        u[j] = in ? __ldg(pu + j) : 0.0f;
-        d[j] = in ? to_f32(__ldg(pd + j)) : 0.0f;
-      }
+      const float* end = gate_up + 2LL * rows * output;
+      rg.load(pg, gate_up, end, output - c);
+      ru.load(pu, gate_up, end, output - c);
+      rd.load(pd, dh, dh + static_cast<long long>(rows) * output, output - c);
     }
+    rg.get(g);
+    ru.get(u);
+    rd.get(d);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       float slope;
@@ -544,7 +565,7 @@ __global__ void __launch_bounds__(kPackThreads) gated_pointwise_backward_f32_ker
 
 int pack_blocks(long long total) {
   const long long want = (total + kPackThreads - 1) / kPackThreads;
-  const long long cap = 16LL * sm_count();
+  const long long cap = 8LL * sm_count();
   return static_cast<int>(want < cap ? want : cap);
 }
 
@@ -561,11 +582,21 @@ cudaError_t launch_gated_few(const void* x, const void* wg, const void* wu,
                                             output, act, stream);
 }
 
-cudaError_t launch_pack_terms(const PackJobs& jobs, Dtype dtype, cudaStream_t stream) {
+cudaError_t launch_pack_terms(PackJobs jobs, Dtype dtype, cudaStream_t stream) {
   long long total = 0;
   for (int q = 0; q < jobs.count; ++q) total += jobs.job[q].rows * (jobs.job[q].ld >> 3);
   const int blocks = pack_blocks(total);
   if (blocks == 0) return cudaSuccess;
+  const int step = blocks * kPackThreads;
+  long long before = 0;
+  for (int q = 0; q < jobs.count; ++q) {
+    PackJob& job = jobs.job[q];
+    const int groups = job.ld >> 3;
+    job.shift = static_cast<int>(before % step);
+    job.step_rows = step / groups;
+    job.step_groups = step % groups;
+    before += job.rows * groups;
+  }
   auto* kernel = dtype == Dtype::kBf16 ? pack_terms_kernel<__nv_bfloat16, 1>
                                        : pack_terms_kernel<float, 3>;
   return launch_following(kernel, dim3(blocks), kPackThreads, 0, 0, stream, jobs);

@@ -385,3 +385,35 @@ def test_no_rows(cuda):
     h, gu = forward(x, wg, wu, off)
     dx, dwg, dwu = backward(x, wg, wu, off, gu, dh)
     assert h.numel() == 0 and dx.numel() == 0 and not dwg.any() and not dwu.any()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("shift", range(1, 8))
+def test_buffers_that_start_anywhere(cuda, dtype, shift):
+    """Rows of no multiple of 16 bytes from buffers that start at any element,
+    between values that are not theirs: the same bits as from aligned copies."""
+    e, r, k, n = 3, 300, 131, 53
+
+    def moved(t):
+        buf = torch.full((t.numel() + 16,), float("nan"), dtype=t.dtype, device=cuda)
+        view = buf[shift:shift + t.numel()].view(t.shape)
+        view.copy_(t)
+        return view
+
+    x, dh = random((r, k), 1, cuda, dtype=dtype), random((r, n), 2, cuda, dtype=dtype)
+    wg, wu = random((e, k, n), 3, cuda, dtype=dtype), random((e, k, n), 4, cuda, dtype=dtype)
+    gu = random((r, 2 * n), 5, cuda)
+    off = torch.tensor([0, 100, 100, r], dtype=torch.int32, device=cuda)
+    size = rr.grouped_gated_gemm_workspace_size(r, e, k, n, dtype, backward=True)
+    assert size > 0  # operands are packed
+    results = []
+    for place in (lambda t: t, moved):
+        ws = torch.empty(size, dtype=torch.uint8, device=cuda)
+        h, dx = torch.empty(r, n, dtype=dtype, device=cuda), torch.empty_like(x)
+        dwg, dwu = torch.empty_like(wg), torch.empty_like(wu)
+        rr.grouped_gated_gemm(place(x), place(wg), place(wu), off, h, workspace=ws)
+        rr.grouped_gated_gemm_backward(place(x), place(wg), place(wu), off, place(gu), place(dh),
+                                       dx, dwg, dwu, workspace=ws)
+        results.append((h, dx, dwg, dwu))
+    for a, b in zip(*results):
+        assert torch.equal(a, b) and torch.isfinite(a.float()).all()
