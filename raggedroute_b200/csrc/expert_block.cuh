@@ -33,7 +33,7 @@ __device__ __forceinline__ void follow_previous() {
 }
 
 template <typename... P, typename... A>
-cudaError_t launch_following(void (*kernel)(P...), dim3 grid, int threads, std::size_t smem,
+cudaError_t launch_following(void (*kernel)(P...), dim3 grid, dim3 block, std::size_t smem,
                              int cluster, cudaStream_t stream, const A&... args) {
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -44,7 +44,7 @@ cudaError_t launch_following(void (*kernel)(P...), dim3 grid, int threads, std::
   attr[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads);
+  cfg.blockDim = block;
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cfg.attrs = attr;

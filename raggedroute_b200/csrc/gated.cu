@@ -321,22 +321,51 @@ __global__ void __launch_bounds__(kFewThreads) gated_few_dx_kernel(
 // The weight gradients are written once, zeros for experts without rows: bound
 // by those bytes. dW[e][k, n] = sum_r x[r, k] d[r, n]; a warp takes kDwRows
 // weight rows of 32 vectors of columns, both gradients.
-constexpr int kDwRows = 4;
+template <int kVec>
+constexpr int kDwRows = kVec == 1 ? 16 : 4;  // 32 and 64 sums per thread
+
+template <typename T>
+__device__ __forceinline__ void zero_range(T* p, T* end) {  // by the whole block
+  if (p >= end) return;
+  const auto up = [](T* q, uintptr_t d) {
+    return reinterpret_cast<T*>((reinterpret_cast<uintptr_t>(q) + d) & ~static_cast<uintptr_t>(15));
+  };
+  T* mid = up(p, 15) < end ? up(p, 15) : end;
+  T* last = up(end, 0) > mid ? up(end, 0) : mid;
+  for (T* q = p + threadIdx.x; q < mid; q += kFewThreads) *q = from_f32<T>(0.0f);
+  for (auto* q = reinterpret_cast<uint4*>(mid) + threadIdx.x; q < reinterpret_cast<uint4*>(last);
+       q += kFewThreads) {
+    *q = make_uint4(0u, 0u, 0u, 0u);
+  }
+  for (T* q = last + threadIdx.x; q < end; q += kFewThreads) *q = from_f32<T>(0.0f);
+}
 
 template <typename T, int kVec>
 __global__ void __launch_bounds__(kFewThreads) gated_few_dw_kernel(
     const T* __restrict__ x, const float* __restrict__ dg, const float* __restrict__ du,
     const int32_t* __restrict__ offsets, T* __restrict__ dwg, T* __restrict__ dwu, int rows,
-    int hidden, int output, int k_blocks) {
+    int hidden, int output, int k_blocks, long long part) {
   follow_previous();
-  // Experts and blocks of k share the y axis of the grid.
+  // Experts and blocks of k share the y axis of the grid; part: a block's share of
+  // an expert's elements.
   const int e = blockIdx.y / k_blocks;
   const int lane = threadIdx.x & 31;
   const int n = (blockIdx.x * 32 + lane) * kVec;
-  const int k0 = ((blockIdx.y - e * k_blocks) * kFewWarps + (threadIdx.x >> 5)) * kDwRows;
-  if (k0 >= hidden || n >= output) return;
+  const int kb = blockIdx.y - e * k_blocks;
+  const int k0 = (kb * kFewWarps + (threadIdx.x >> 5)) * kDwRows<kVec>;
   const int2 s = segment(offsets, e, rows);
-  float g[kDwRows][kVec] = {}, u[kDwRows][kVec] = {};
+  if (kVec == 1 && s.x >= s.y) {
+    // An idle expert's gradients are one run of zeros each: whole granules, also
+    // where rows start anywhere.
+    const long long size = static_cast<long long>(hidden) * output;
+    const long long from = part * (kb * gridDim.x + blockIdx.x);
+    const long long to = from + part < size ? from + part : size;
+    zero_range(dwg + e * size + from, dwg + e * size + to);
+    zero_range(dwu + e * size + from, dwu + e * size + to);
+    return;
+  }
+  if (k0 >= hidden || n >= output) return;
+  float g[kDwRows<kVec>][kVec] = {}, u[kDwRows<kVec>][kVec] = {};
   for (int r = s.x; r < s.y; ++r) {
     float a[kVec], b[kVec];
     const long long at = static_cast<long long>(r) * output + n;
@@ -346,7 +375,7 @@ __global__ void __launch_bounds__(kFewThreads) gated_few_dw_kernel(
       b[v] = __ldg(du + at + v);
     }
 #pragma unroll
-    for (int j = 0; j < kDwRows; ++j) {
+    for (int j = 0; j < kDwRows<kVec>; ++j) {
       const float xv =
           to_f32(__ldg(x + static_cast<long long>(r) * hidden + min(k0 + j, hidden - 1)));
 #pragma unroll
@@ -357,7 +386,7 @@ __global__ void __launch_bounds__(kFewThreads) gated_few_dw_kernel(
     }
   }
 #pragma unroll
-  for (int j = 0; j < kDwRows; ++j) {
+  for (int j = 0; j < kDwRows<kVec>; ++j) {
     if (k0 + j < hidden) {
       const long long at =
           (static_cast<long long>(e) * hidden + k0 + j) * output + n;
@@ -662,8 +691,11 @@ cudaError_t few_dw_launch(const void* x, const float* dg, const float* du, const
                           cudaStream_t stream) {
   constexpr int kVec = 16 / sizeof(T);
   const bool vec = output % kVec == 0 && aligned_to(dwg, 16) && aligned_to(dwu, 16);
-  const int k_blocks = ceil_div(hidden, kFewWarps * kDwRows);
+  const int k_blocks = ceil_div(hidden, kFewWarps * (vec ? kDwRows<kVec> : kDwRows<1>));
   auto* kernel = vec ? gated_few_dw_kernel<T, kVec> : gated_few_dw_kernel<T, 1>;
+  const int columns = ceil_div(output, 32 * (vec ? kVec : 1));
+  const long long blocks = static_cast<long long>(columns) * k_blocks;
+  const long long part = (static_cast<long long>(hidden) * output + blocks - 1) / blocks;
   // The y axis holds 65535 blocks: experts in slices that fit.
   const int slice = k_blocks < 65535 ? 65535 / k_blocks : 0;
   if (slice == 0) return cudaErrorInvalidConfiguration;
@@ -671,9 +703,9 @@ cudaError_t few_dw_launch(const void* x, const float* dg, const float* du, const
     const int count = experts - e < slice ? experts - e : slice;
     const long long at = static_cast<long long>(e) * hidden * output;
     const cudaError_t err = launch_following(
-        kernel, dim3(ceil_div(output, 32 * (vec ? kVec : 1)), count * k_blocks), kFewThreads, 0, 0,
-        stream, static_cast<const T*>(x), dg, du, offsets + e, static_cast<T*>(dwg) + at,
-        static_cast<T*>(dwu) + at, rows, hidden, output, k_blocks);
+        kernel, dim3(columns, count * k_blocks), kFewThreads, 0, 0, stream,
+        static_cast<const T*>(x), dg, du, offsets + e, static_cast<T*>(dwg) + at,
+        static_cast<T*>(dwu) + at, rows, hidden, output, k_blocks, part);
     if (err != cudaSuccess) return err;
   }
   return cudaSuccess;

@@ -41,7 +41,7 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
-// Sum over the block in every thread; `parts` holds 32 floats and is free
+// Sum over a token's threads (the block's x axis) in each of them; `parts` holds 32 floats and is free
 // again after the next barrier.
 __device__ __forceinline__ float block_sum(float v, float* parts) {
   v = warp_sum(v);
@@ -123,7 +123,8 @@ __global__ void __launch_bounds__(kMaxThreads) unpermute_norm_kernel(const Unper
                                                                      float* inv_rms) {
   __shared__ float parts[2][32];
   follow_previous();
-  const long long t = blockIdx.x;
+  const long long t = static_cast<long long>(blockIdx.x) * blockDim.y + threadIdx.y;
+  if (t >= in.tokens) return;  // only where warps share a block, and then no barrier
   const long long row = t * in.output;
   const float per_col = 1.0f / static_cast<float>(in.output);
   float res[kElems];
@@ -1138,9 +1139,8 @@ int row_threads(int output, int per) {
   return threads;
 }
 
-// The streamed form's layout, or blocks = 0 where the plain one runs: few
-// tokens (the rings have to fill before they pay: two tokens per team), more
-// routes than a ring keeps track of, or rows of which two stages do not fit.
+// The streamed form's layout, or blocks = 0 where it has none: more routes than a
+// ring keeps track of, or rows of which two stages do not fit.
 Stream stream_plan(int tokens, int top_k, int output, int extra_rows, bool gradient, int elems,
                    std::size_t size) {
   Stream st;
@@ -1165,7 +1165,8 @@ Stream stream_plan(int tokens, int top_k, int output, int extra_rows, bool gradi
     else return st;
   }
   if (st.stages > kMaxStages) st.stages = kMaxStages;
-  if (tokens >= 2 * kNumSms * st.teams) st.blocks = kNumSms;
+  st.blocks = ceil_div(tokens, st.teams);
+  if (st.blocks > kNumSms) st.blocks = kNumSms;
   return st;
 }
 
@@ -1209,6 +1210,34 @@ bool allow_ring() {
   return true;
 }
 
+// Where the rings pay in the forward pass: they have to fill first, and rows that
+// still lie in L2 come as fast without them. Crossovers in bytes moved: aligned
+// rows 50 to 100 MB (top 2, plain against streamed: bf16, N=2048, 2400 tokens 14.4
+// against 16.4 us, 4800 33 against 27; FP32, N=4096, 600 tokens 9.8 against 12.5, 1200
+// 22 against 21), others, which the plain form reads in single elements, 6 to 40 MB
+// (N=1027: bf16, 600 tokens 13.2 against 12.9; FP32, 1200 tokens 14.4 against 15.4, 2400
+// 24 against 23). Short aligned rows are a warp's work with one load per thread and
+// row, and stay so (32768 tokens, N=256: FP32 35 against 50 us).
+bool forward_streams(const UnpermuteNorm& in, std::size_t unit, std::size_t size) {
+  if (in.output <= 256 && unit == 16) return false;
+  const double moved = (in.top_k + 3.0) * in.tokens * in.output * size;
+  return moved >= (unit == 16 ? 64e6 : 16e6);
+}
+
+// In the gradient the streamed form needs one reduction where the plain one needs
+// two and reads a token's rows once, so it pays from about a token per SM (N=512, 148
+// tokens: FP32 8.8 us either way, 600 tokens 12.8 against 9.6; N=4096, 148 tokens: bf16
+// 26 against 17, 37 tokens 16.6 against 15.0), for rows of single elements always
+// (N=1027, one token: bf16 12.9 against 9.0), for rows of a few elements per thread
+// later (N=64: 600 tokens 7.9 against 9.0, 1200 10.7 against 9.2), and for those that
+// take sixteen from two tokens per SM (bf16, N=6363: 148 tokens 25 against 34, 600
+// 89 against 72).
+bool backward_streams(const UnpermuteNorm& in, std::size_t unit) {
+  if (in.output <= 128) return in.tokens >= 8 * kNumSms;
+  if (in.output > kStreamThreads * 8) return in.tokens >= 2 * kNumSms;
+  return unit < 16 || in.tokens >= kNumSms;
+}
+
 // Columns handled together by the streamed form: 16 bytes where rows are a
 // multiple of that, pairs of bfloat16 in rows of even length, else one.
 int stream_columns(int output, Dtype dtype) {
@@ -1234,8 +1263,13 @@ cudaError_t forward(const UnpermuteNorm& in, void* residual_out, void* normed, f
   if (threads > 512) threads = row_threads(in.output, kElems);
   auto* kernel = threads <= 512 ? unpermute_norm_kernel<T, kPer, 512>
                                 : unpermute_norm_kernel<T, kPer, 1024>;
-  return launch_following(kernel, dim3(in.tokens), threads, 0, 0, stream, in,
-                          static_cast<T*>(residual_out), static_cast<T*>(normed), inv_rms);
+  // Tokens of one warp share blocks once there are several per SM: starting a
+  // block takes longer than such a row (bf16, 65536 tokens: N=256 56 against 71 us, N=64 36
+  // against 69).
+  const int share = threads == 32 && in.tokens > 4 * kNumSms ? 8 : 1;
+  return launch_following(kernel, dim3(ceil_div(in.tokens, share)), dim3(threads, share), 0, 0,
+                          stream, in, static_cast<T*>(residual_out), static_cast<T*>(normed),
+                          inv_rms);
 }
 
 cudaError_t column_sums(const float* workspace, int parts, int output,
@@ -1296,12 +1330,9 @@ cudaError_t launch_unpermute_norm(const UnpermuteNorm& in, void* residual_out, v
   const Stream st = stream_plan(in.tokens, in.top_k, in.output, 1, false, kElems, dtype_bytes(dtype));
   const int per = stream_columns(in.output, dtype);
   const std::size_t unit = per * dtype_bytes(dtype);
-  // Short aligned rows are a warp's work with one load per thread and row; the
-  // ring only delays them (32768 tokens, N=256: FP32 35 against 50 us streamed,
-  // N=512: 66 against 62).
-  const bool direct = in.output <= 256 && per > 2;
-  if (!direct && st.blocks > 0 && aligned_to(in.y_permuted, 16) && aligned_to(in.residual, 16) &&
-      aligned_gammas(in, per) && aligned_to(residual_out, unit) && aligned_to(normed, unit)) {
+  if (st.blocks > 0 && forward_streams(in, unit, dtype_bytes(dtype)) &&
+      aligned_to(in.y_permuted, 16) && aligned_to(in.residual, 16) && aligned_gammas(in, per) &&
+      aligned_to(residual_out, unit) && aligned_to(normed, unit)) {
     if (dtype == Dtype::kBf16) {
       auto* run = per == 8   ? forward_stream<__nv_bfloat16, 8>
                   : per == 2 ? forward_stream<__nv_bfloat16, 2>
@@ -1336,9 +1367,9 @@ cudaError_t launch_unpermute_norm_backward(const UnpermuteNorm& in, const Unperm
                                 gradient_elems(in.output), dtype_bytes(dtype));
   const int per = stream_columns(in.output, dtype);
   const std::size_t unit = per * dtype_bytes(dtype);
-  if (st.blocks > 0 && aligned_to(in.y_permuted, 16) && aligned_to(in.residual, 16) &&
-      aligned_to(g.d_residual_out, 16) && aligned_to(g.d_normed, 16) && aligned_gammas(in, per) &&
-      aligned_to(g.d_residual, unit) && aligned_to(g.d_y_permuted, unit)) {
+  if (st.blocks > 0 && backward_streams(in, unit) && aligned_to(in.y_permuted, 16) &&
+      aligned_to(in.residual, 16) && aligned_to(g.d_residual_out, 16) &&
+      aligned_to(g.d_normed, 16) && aligned_gammas(in, per) && aligned_to(g.d_residual, unit) && aligned_to(g.d_y_permuted, unit)) {
     if (dtype == Dtype::kBf16) {
       auto* run = per == 8   ? backward_stream<__nv_bfloat16, 8>
                   : per == 2 ? backward_stream<__nv_bfloat16, 2>

@@ -282,3 +282,35 @@ def test_replay_and_stream(cuda):
         torch.cuda.synchronize()
         for a, b in zip(got, (out, normed, inv, *g.values(), *p.values())):
             assert torch.equal(a, b)
+
+
+# Enough bytes for the streamed forward pass: each team size, both alignments, many
+# routes, token counts that end inside a stage.
+STREAMED = [(13201, 2, 512), (6600, 2, 1000), (3299, 2, 2048), (1701, 2, 4096), (901, 2, 8192),
+            (1001, 16, 2056), (21000, 1, 130), (8003, 3, 333), (1650, 2, 1027), (421, 2, 8191)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("shape", STREAMED, ids=str)
+def test_streamed_forward(cuda, shape, dtype):
+    i = Inputs(*shape, dtype, cuda, seed=31, skip=shape[1] > 1)
+    out, normed, inv = i.forward()
+    check_forward(i, out, normed, dtype)
+    again = i.forward()
+    assert all(torch.equal(a, b) for a, b in zip((out, normed, inv), again))
+    i.res = i.res.clone()
+    out2, normed2, inv2 = i.forward(out=i.res)  # in place
+    assert torch.equal(out, out2) and torch.equal(normed, normed2) and torch.equal(inv, inv2)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("shape", [(1, 2, 515), (2, 4, 178), (149, 2, 512), (148, 1, 4096),
+                                   (1185, 2, 120), (297, 2, 8192)], ids=str)
+def test_streamed_gradient_of_few_tokens(cuda, shape, dtype):
+    """Fewer tokens than teams: most of a block has none."""
+    i = Inputs(*shape, dtype, cuda, seed=47)
+    _, _, inv = i.forward()
+    first = i.backward(inv)
+    check_backward(i, first, dtype)
+    second = i.backward(inv)
+    assert all(torch.equal(t, second[name]) for name, t in first.items())
