@@ -107,30 +107,30 @@ bool rows_aligned(const void* p, long long cols, std::size_t size) {
 
 // Few rows run without the tensor cores, straight from the caller's weights.
 // BF16: where hardly any two rows share an expert both forms read the weights
-// once, and the plain one spreads them over all SMs (128 experts, K=4096,
-// N=1408: 2 rows 11 against 22 us, 64 rows 202 against 216; 64 experts,
-// K=N=1024: 32 rows 21 against 27); sharing experts, the engine's tiles reuse
-// them (64 rows 46 against 37). FP32: the engine first writes the weights of
-// every expert as three bfloat16 parts, 16 bytes moved per element, which pays
-// from about 16 rows per expert (8 experts, K=N=1024: 128 rows 46 against 73 us,
-// 256 rows 80 against 74).
+// once, and the plain one spreads them over all SMs (64 experts, 16 rows,
+// K=2048, N=1408 37 against 49 us; 8 experts, 4 rows, K=N=1024 5 against 10);
+// sharing experts, the engine's tiles reuse them (one row per expert: 154 against
+// 121, 14 against 13). FP32: the engine first writes the weights of every expert as
+// three bfloat16 parts, 16 bytes moved per element, which pays from about 16 rows
+// per expert (64 experts, K=N=1024: 16 rows each 312 against 467 us, 24 443 against 472;
+// 64 experts, K=256, N=128: 20 against 21, 28 against 22).
 bool gated_few(int rows, int experts, Dtype dtype) {
   return rows <= 4 || (dtype == Dtype::kBf16 ? 2LL * rows <= experts : rows <= 16LL * experts);
 }
 
 // The backward pass takes its few-row forms where they beat the engine. BF16:
-// where most experts are idle (64 experts, K=2048, N=1408, 3 rows: both
-// gradients 128 against 164 us; 32 rows 271 against 236), and, as the engine
-// then packs its operands, up to a few rows per expert for sizes that are no
-// multiple of 8 (17 experts, 1001 x 333: 68 rows 52 against 59 us, 136 rows 77
-// against 58). FP32, where it always packs: 8 rows per expert (64 experts,
-// K=N=1024: 558 against 611 us, 16 rows per expert 993 against 630). The grid of
-// the weight gradients limits K.
+// up to half a row per expert (64 experts, K=2048, N=1408: 16 rows 186 against 212 us,
+// 32 rows 266 against 267, 64 rows 397 against 381; 8 experts, K=N=1024: 4 rows 15
+// against 32), and, as the engine then packs its operands, up to two for sizes that are
+// no multiple of 8 (1001 x 333: 17 experts, 34 rows 33 against 44, 64 experts, 128 rows
+// 121 against 123; four each 44 against 42 and 149 against 123). FP32, where it always
+// packs: 8 rows per expert (64 experts, K=N=1024: 547 against 629 us, 12 each 759 against
+// 640; K=256, N=128: 32 against 33). The grid of the weight gradients limits K.
 bool gated_few_backward(int rows, int experts, int hidden, int output, Dtype dtype) {
   if (hidden > (1 << 20)) return false;
   if (rows <= 4) return true;
   if (dtype == Dtype::kFp32) return rows <= 8LL * experts;
-  return hidden % 8 != 0 || output % 8 != 0 ? rows <= 4LL * experts : 4LL * rows <= experts;
+  return hidden % 8 != 0 || output % 8 != 0 ? rows <= 2LL * experts : 2LL * rows <= experts;
 }
 
 // Parts of dg and du in a bfloat16 backward pass. One rounding to bfloat16 is
