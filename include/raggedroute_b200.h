@@ -427,7 +427,10 @@ rr_status rr_ep_plan(const int32_t* count_all, int nranks, int rank, int experts
  * where an entry says so. Grouped rows are as for rr_grouped_gemm: segment e
  * is rows [offsets[e], offsets[e+1]) of route_pairs rows (clipped to them);
  * rows outside every segment are left as they were. Results repeat bit for
- * bit: no entry accumulates with atomics. Values of RR_DTYPE_* equal
+ * bit: no entry accumulates with atomics. Kernels start behind the one before
+ * them in the stream (programmatic serialization, also when captured), and touch
+ * memory only once it has ended. Calls that may run at the same time need
+ * workspaces of their own; a workspace may not touch the call's buffers. Values of RR_DTYPE_* equal
  * raggedroute::ScalarType. */
 enum { RR_DTYPE_FP32 = 0, RR_DTYPE_BF16 = 2 };
 enum { RR_ACTIVATION_SILU = 0, RR_ACTIVATION_GELU_TANH = 1, RR_ACTIVATION_RELU = 2 };
@@ -485,8 +488,8 @@ rr_status rr_quantize_expert_weights_int8(const void* expert_weights, int8_t* wq
                                           int experts, int hidden, int output, int dtype,
                                           const rr_context* ctx);
 /* y[r, n] = (sum_k xq[r, k] * wq[e, n, k]) * x_scale[r] * w_scale[e, n] for r
- * in segment e: the sum exact in 32-bit integers, the scaling in FP32, one
- * rounding to dtype (y_permuted [R, N]). */
+ * in segment e: the sum exact in 32-bit integers (values -127 to 127, as
+ * quantised), the scaling in FP32, one rounding to dtype (y_permuted [R, N]). */
 rr_status rr_grouped_gemm_int8(const int8_t* xq, const float* x_scale, const int8_t* wq,
                                const float* w_scale, const int32_t* offsets, void* y_permuted,
                                int route_pairs, int experts, int hidden, int output, int dtype,

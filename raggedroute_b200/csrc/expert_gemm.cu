@@ -42,6 +42,15 @@
 // hands that block over; warps 4-11 epilogue. TMEM holds two 256-column accumulators, so a tile's
 // epilogue runs beside the next tile's products. Waits are bounded as in the
 // other pair engine (gemm_pair.cu), with the same exit protocol.
+//
+// Bound by the tensor pipe, busy 86% of the time at 8 experts, 16384 rows, K=4096,
+// N=1408 (kGated, bfloat16: 243 us, DRAM 334 MB read, 41 MB written). 128 experts of 1024
+// rows: 2.12 ms in a burst (1.42 PFLOP/s), 2.51 ms back to back (1.21), where the power
+// limit sets the clock. FP32 (six products): 64 experts, 32768 rows, K=N=1024: 0.73
+// ms of 1.08 with the packing. Taller tiles (512 rows, two accumulators sharing B) took
+// 844 against 912 us for one dense 8192^3 product but 2.68 against 2.41 ms over ragged
+// segments, whose tails grow and whose epilogue no longer runs beside the products;
+// FP32 blocks 32 deep took 757 against 727 us.
 #include <cuda.h>
 
 #include <mutex>

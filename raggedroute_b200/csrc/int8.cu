@@ -40,7 +40,9 @@ __device__ __forceinline__ uint32_t pack_i8x4(int a, int b, int c, int d) {
 
 // ---- rows ------------------------------------------------------------------------
 //
-// Bound by the bytes in and out. Long or unaligned rows take one block each: the
+// Bound by the bytes in and out (131072 x 4096, bfloat16: 230 us, 7.0 TB/s; rows of
+// 1181, which no vector load fits: 27040 in 31 us, 3.1 TB/s, against 34 and more with
+// a warp that shifts 16-byte granules). Long or unaligned rows take one block each: the
 // row is read once into registers (up to kHeld steps per thread; what is longer
 // is read again, from L2).
 
@@ -210,7 +212,8 @@ cudaError_t quantize_rows(const T* x, int8_t* xq, float* x_scale, int rows, int 
 //
 // W[e] is [hidden][output] and wq[e] is [output][ld]: a block takes 64
 // channels of one expert, finds their scales in one pass over K and transposes
-// 64 x 64 tiles through shared memory in a second. Done once per weight set.
+// 64 x 64 tiles through shared memory in a second. Done once per weight set (128 x 4096
+// x 1408, bfloat16: 1.2 ms; the second pass reads from DRAM again).
 
 constexpr int kChan = 64;
 constexpr int kWeightThreads = 256;
@@ -268,7 +271,8 @@ __global__ void __launch_bounds__(kWeightThreads) quantize_weights_kernel(
 //
 // Bound by reading the weights of the experts that have rows, K bytes per
 // channel, once: a warp takes kCols channels of up to kFewRows rows of one
-// expert, 16 bytes per lane and channel, four-way integer dot products.
+// expert, 16 bytes per lane and channel, four-way integer dot products. (Two rows of
+// 128 experts, K=4096, N=1408: 11.5 MB in 3.3 us, of which 2 are its start.)
 
 constexpr int kFewThreads = 256;
 constexpr int kCols = 4;
