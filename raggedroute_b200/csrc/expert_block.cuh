@@ -27,9 +27,15 @@ inline std::size_t dtype_bytes(Dtype t) { return t == Dtype::kBf16 ? 2 : 4; }
 // at most one waits. Back to back, K=4096, N=1408, one token: unpermute_norm 3.6
 // against 6.2 us, quantize_rows_int8 and grouped_gemm_int8 5.9 against 10.2.
 
-__device__ __forceinline__ void follow_previous() {
+__device__ __forceinline__ void wait_for_previous() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+__device__ __forceinline__ void let_next_start() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+__device__ __forceinline__ void follow_previous() {
+  wait_for_previous();
+  let_next_start();
 }
 
 template <typename... P, typename... A>

@@ -342,11 +342,13 @@ __global__ void __launch_bounds__(kThreads, 1) expert_gemm_kernel(
     s.failed = 0;
     fence_mbar_init();
   }
+  // Tensor memory is taken only once the kernel before has ended, and the next
+  // kernel may come only once it is taken: no block waits with what another needs.
+  wait_for_previous();
   if (warp == 1) {
     tmem_alloc_pair(&s.tmem_base, kTmemCols);
     tmem_relinquish_pair();
   }
-  follow_previous();
   int total;
   if constexpr (kMode == kDw) {
     total = p.experts * ((p.hidden + kTileM - 1) / kTileM) * n_tiles;
@@ -357,6 +359,7 @@ __global__ void __launch_bounds__(kThreads, 1) expert_gemm_kernel(
   __syncthreads();
   cluster_sync();
   tc_fence_after();
+  let_next_start();
   const uint32_t tmem = s.tmem_base;
   volatile int* failed = &s.failed;
   const uint32_t peer_failed = mapa_shared(smem_u32(&s.failed), rank ^ 1);

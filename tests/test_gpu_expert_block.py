@@ -370,3 +370,23 @@ def test_chain_of_calls_with_no_pause(cuda):
 
     want, got = run(True), run(False)
     assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+def test_graph_of_the_library(cuda, dtype):
+    """Captured and replayed through raggedroute_b200.Graph."""
+    for fn, tensors, rest, outputs in _calls(cuda, dtype):
+        fn(**tensors, **rest)
+        want = {k: tensors[k].clone() for k in outputs}
+        torch.cuda.synchronize()
+        stream = torch.cuda.Stream()
+        graph = rr.Graph.capture(lambda ctx: fn(**{k: v for k, v in tensors.items()}, **rest,
+                                                ctx=ctx), stream)
+        for k in outputs:
+            tensors[k].zero_()
+        torch.cuda.synchronize()
+        for _ in range(2):
+            graph.launch(stream)
+        torch.cuda.synchronize()
+        for k in outputs:
+            assert torch.equal(tensors[k], want[k]), (fn.__name__, k)
