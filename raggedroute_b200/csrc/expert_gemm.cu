@@ -572,6 +572,17 @@ __global__ void __launch_bounds__(kThreads, 1) expert_gemm_kernel(
           return min(g.ncols, folded ? (side + 1) * half : g.ncols) - out;
         }
       };
+      // kInt8: the scales of this lane's row and, of each group, of column `lane`,
+      // read while the products run.
+      float row_scale = 0.0f, col_scale[4] = {};
+      if constexpr (kMode == kInt8) {
+        if (lane < rows) row_scale = __ldg(p.row_scale + row0 + lane);
+        const float* scales = p.col_scale + static_cast<long long>(g.expert) * p.output + g.c0;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          if (q < groups && lane < group_left(q)) col_scale[q] = __ldg(scales + group_out(q) + lane);
+        }
+      }
       // Stores group q: v, in kGated with its up columns v2.
       auto put = [&](int q, const float* v, const float* v2) {
         const int c = group_out(q);
@@ -599,14 +610,13 @@ __global__ void __launch_bounds__(kThreads, 1) expert_gemm_kernel(
           const int ld = kMode == kDx ? p.hidden : p.output;
           T* out = static_cast<T*>(p.out0) + static_cast<long long>(row0) * ld + g.c0 + c;
           if constexpr (kMode == kInt8) {
-            const float xs = lane < rows ? __ldg(p.row_scale + row0 + lane) : 0.0f;
-            const float* ws =
-                p.col_scale + static_cast<long long>(g.expert) * p.output + g.c0 + c;
+            const float ws = q < 2 ? (q == 0 ? col_scale[0] : col_scale[1])
+                                   : (q == 2 ? col_scale[2] : col_scale[3]);
             float y[32];
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
-              y[i] = static_cast<float>(__float_as_int(v[i])) * xs *
-                     (i < cols ? __ldg(ws + i) : 0.0f);
+              y[i] = static_cast<float>(__float_as_int(v[i])) * row_scale *
+                     __shfl_sync(0xffffffffu, ws, i);
             }
             store_rows32<T>(staging, y, out, ld, rows, cols, p.vec != 0);
           } else {
