@@ -244,7 +244,8 @@ __device__ __forceinline__ Tile tile_at(const EngineArgs& p, int t, const int* p
 // 64-byte pieces of eight rows at a time (or, where rows are not 16-byte
 // aligned or the piece is cut, consecutive elements). Chunk c of row r sits at
 // c ^ (r / 2 mod 4): no bank conflicts in either direction.
-template <typename T>
+// kUnroll: of the element-wise form (whole, where registers allow).
+template <typename T, int kUnroll>
 __device__ __forceinline__ void store_rows(uint8_t* staging, const float* v, T* base, long long ld,
                                            int rows, int cols, bool vec) {
   constexpr int kPer = 16 / sizeof(T);
@@ -271,24 +272,28 @@ __device__ __forceinline__ void store_rows(uint8_t* staging, const float* v, T* 
     const int col = lane % kCols;
     const int c = col / kPer;
     if (col < cols) {
-#pragma unroll 4
-      for (int r = lane / kCols; r < rows; r += 32 / kCols) {
-        base[r * ld + col] = *reinterpret_cast<const T*>(
-            staging + r * 64 + ((c ^ ((r >> 1) & 3)) << 4) + (col % kPer) * sizeof(T));
+      T* out = base + lane / kCols * ld + col;
+#pragma unroll kUnroll
+      for (int i = 0; i < kCols; ++i, out += 32 / kCols * ld) {
+        const int r = lane / kCols + i * (32 / kCols);
+        if (r < rows) {
+          *out = *reinterpret_cast<const T*>(staging + r * 64 + ((c ^ ((r >> 1) & 3)) << 4) +
+                                             (col % kPer) * sizeof(T));
+        }
       }
     }
   }
 }
 
 // 32 columns of a warp's rows: one piece of bfloat16 or two of float.
-template <typename T>
+template <typename T, int kUnroll>
 __device__ __forceinline__ void store_rows32(uint8_t* staging, const float* v, T* base,
                                              long long ld, int rows, int cols, bool vec) {
   constexpr int kCols = 64 / sizeof(T);
 #pragma unroll
   for (int i = 0; i < 32 / kCols; ++i) {
     if (cols > i * kCols) {
-      store_rows<T>(staging, v + i * kCols, base + i * kCols, ld, rows, cols - i * kCols, vec);
+      store_rows<T, kUnroll>(staging, v + i * kCols, base + i * kCols, ld, rows, cols - i * kCols, vec);
     }
   }
 }
@@ -303,6 +308,7 @@ __global__ void __launch_bounds__(kThreads, 1) expert_gemm_kernel(
   constexpr bool kMnA = kMode == kDw;
   constexpr bool kMnB = kMode == kGated || kMode == kDw;
   constexpr bool kFp32 = kPa == 3;  // every k-block its own accumulation
+  constexpr int kUnroll = kFp32 ? 8 : 32;
   constexpr int kStages = Cfg::kStages;
   constexpr int kOffB = Cfg::kOffB;
   // Byte step of one K = 16 (bfloat16) or 32 (int8) MMA inside a box, and the
@@ -593,19 +599,19 @@ __global__ void __launch_bounds__(kThreads, 1) expert_gemm_kernel(
 #pragma unroll
           for (int i = 0; i < 32; ++i) h[i] = activate<T>(p.activation, v[i]) * v2[i];
           const long long at = static_cast<long long>(row0) * p.output + g.c0 + c;
-          store_rows32<T>(staging, h, static_cast<T*>(p.out0) + at, p.output, rows, cols,
+          store_rows32<T, kUnroll>(staging, h, static_cast<T*>(p.out0) + at, p.output, rows, cols,
                           p.vec != 0);
           if (p.gate_up != nullptr) {
             float* gu = p.gate_up + 2LL * row0 * p.output + g.c0 + c;
-            store_rows32<float>(staging, v, gu, 2LL * p.output, rows, cols,
+            store_rows32<float, kUnroll>(staging, v, gu, 2LL * p.output, rows, cols,
                                 p.vec_gate_up != 0);
-            store_rows32<float>(staging, v2, gu + p.output, 2LL * p.output, rows, cols,
+            store_rows32<float, kUnroll>(staging, v2, gu + p.output, 2LL * p.output, rows, cols,
                                 p.vec_gate_up != 0);
           }
         } else if constexpr (kMode == kDw) {
           T* out = static_cast<T*>((folded ? side : hw) == 0 ? p.out0 : p.out1) +
                    (static_cast<long long>(g.expert) * p.hidden + row0) * p.output + g.c0 + c;
-          store_rows32<T>(staging, v, out, p.output, rows, cols, p.vec != 0);
+          store_rows32<T, kUnroll>(staging, v, out, p.output, rows, cols, p.vec != 0);
         } else {
           const int ld = kMode == kDx ? p.hidden : p.output;
           T* out = static_cast<T*>(p.out0) + static_cast<long long>(row0) * ld + g.c0 + c;
@@ -618,9 +624,9 @@ __global__ void __launch_bounds__(kThreads, 1) expert_gemm_kernel(
               y[i] = static_cast<float>(__float_as_int(v[i])) * row_scale *
                      __shfl_sync(0xffffffffu, ws, i);
             }
-            store_rows32<T>(staging, y, out, ld, rows, cols, p.vec != 0);
+            store_rows32<T, kUnroll>(staging, y, out, ld, rows, cols, p.vec != 0);
           } else {
-            store_rows32<T>(staging, v, out, ld, rows, cols, p.vec != 0);
+            store_rows32<T, kUnroll>(staging, v, out, ld, rows, cols, p.vec != 0);
           }
         }
       };
