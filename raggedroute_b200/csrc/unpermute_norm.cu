@@ -1222,14 +1222,16 @@ bool allow_ring() {
 // still lie in L2 come as fast without them. Crossovers in bytes moved: aligned
 // rows 50 to 100 MB (top 2, plain against streamed: bf16, N=2048, 2400 tokens 14.4
 // against 16.4 us, 4800 33 against 27; FP32, N=4096, 600 tokens 9.8 against 12.5, 1200
-// 22 against 21), others, which the plain form reads in single elements, 6 to 40 MB
-// (N=1027: bf16, 600 tokens 13.2 against 12.9; FP32, 1200 tokens 14.4 against 15.4, 2400
-// 24 against 23). Short aligned rows are a warp's work with one load per thread and
-// row, and stay so (32768 tokens, N=256: FP32 35 against 50 us).
+// 22 against 21), others, which the plain form reads in single elements, earlier: bf16
+// at 6 MB (N=1027, 600 tokens 13.2 against 12.9; N=2051, 300 tokens 16.6 against 12.5), FP32
+// at 32 MB (N=1027, 1200 tokens 14.4 against 15.4, 2400 24 against 23); always with two
+// tokens per SM (bf16, N=4095, 148 tokens 8.4 against 11.5). Short aligned rows are a
+// warp's work with one load per thread and row, and stay so (32768 tokens, N=256: FP32
+// 35 against 50 us).
 bool forward_streams(const UnpermuteNorm& in, std::size_t unit, std::size_t size) {
   if (in.output <= 256 && unit == 16) return false;
   const double moved = (in.top_k + 3.0) * in.tokens * in.output * size;
-  return moved >= (unit == 16 ? 64e6 : 16e6);
+  return in.tokens >= 2 * kNumSms && moved >= (unit == 16 ? 64e6 : size == 4 ? 32e6 : 6e6);
 }
 
 // In the gradient the streamed form needs one reduction where the plain one needs
@@ -1266,8 +1268,11 @@ bool aligned_rows(const UnpermuteNorm& in, Dtype dtype) {
 template <typename T, int kPer>
 cudaError_t forward(const UnpermuteNorm& in, void* residual_out, void* normed, float* inv_rms,
                     cudaStream_t stream) {
-  // Eight columns per thread while the block stays at 512 threads.
-  int threads = row_threads(in.output, 8);
+  // Eight columns per thread while the block stays at 512 threads; four where short rows
+  // are read in single elements and there is a token per SM at most (one token, FP32:
+  // N=333 4.5 against 5.6 us, N=1027 4.9 against 5.3, N=2051 6.6 against 5.8).
+  const bool spread = kPer == 1 && in.output <= 1536 && in.tokens <= kNumSms;
+  int threads = row_threads(in.output, spread ? 4 : 8);
   if (threads > 512) threads = row_threads(in.output, kElems);
   auto* kernel = threads <= 512 ? unpermute_norm_kernel<T, kPer, 512>
                                 : unpermute_norm_kernel<T, kPer, 1024>;
