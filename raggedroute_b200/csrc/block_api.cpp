@@ -111,11 +111,25 @@ bool rows_aligned(const void* p, long long cols, std::size_t size) {
 // K=2048, N=1408 37 against 49 us; 8 experts, 4 rows, K=N=1024 5 against 10);
 // sharing experts, the engine's tiles reuse them (one row per expert: 154 against
 // 121, 14 against 13). FP32: the engine first writes the weights of every expert as
-// three bfloat16 parts, 16 bytes moved per element, which pays from about 16 rows
-// per expert (64 experts, K=N=1024: 16 rows each 312 against 467 us, 24 443 against 472;
-// 64 experts, K=256, N=128: 20 against 21, 28 against 22).
-bool gated_few(int rows, int experts, Dtype dtype) {
-  return rows <= 4 || (dtype == Dtype::kBf16 ? 2LL * rows <= experts : rows <= 16LL * experts);
+// three bfloat16 parts and then takes a microsecond per 64 of K and round of tiles; the
+// plain form does 18 TFLOP/s (half of it in single elements) and pays for each block.
+// The smaller estimate, in microseconds, decides; it is within a fifth of what was
+// measured (plain against engine: 64 experts, K=N=1024: 16 rows each 312 against 467; K=256,
+// N=128: 20 against 21, 24 each 28 against 22; 8 experts, 4096 x 128: 64 each 62 against
+// 95, 128 each 116 against 102; 8 experts, 1784 x 126: 48 each 50 against 57, 64 each 71
+// against 57; 32 experts, 1024 x 128: 32 each 40 against 41).
+bool gated_few(int rows, int experts, int hidden, int output, Dtype dtype) {
+  if (rows <= 4) return true;
+  if (dtype == Dtype::kBf16) return 2LL * rows <= experts;
+  if (rows > 65535) return false;  // the y axis of its grid
+  const double weights = static_cast<double>(hidden) * output;
+  const double blocks = ((rows + 3) / 4) * ((output + 31LL) / 32);
+  const double plain = 4e-6 * rows * weights / 18 + 0.0072 * blocks;
+  const long long tiles = ((rows + 256LL * experts - 1) / (256LL * experts)) * experts *
+                          ((output + 127) / 128);
+  const double engine = 9 + static_cast<double>((hidden + 63) / 64) * ((tiles + 73) / 74) +
+                        4.5e-6 * experts * weights;
+  return 3 + (output % 4 != 0 ? 2 * plain : plain) <= engine;
 }
 
 // The backward pass takes its few-row forms where they beat the engine. BF16:
@@ -157,7 +171,7 @@ GatedPlan gated_plan(int rows, int experts, int hidden, int output, Dtype dtype,
   p.terms = dtype == Dtype::kFp32 ? 3 : 1;
   p.ldk = static_cast<int>(up8(hidden));
   p.ldn = static_cast<int>(up8(output));
-  if (rows <= 0 || (!backward && gated_few(rows, experts, dtype))) return p;
+  if (rows <= 0 || (!backward && gated_few(rows, experts, hidden, output, dtype))) return p;
   if (backward && gated_few_backward(rows, experts, hidden, output, dtype)) {  // dg and du in FP32
     p.few = true;
     p.du = up256(4ull * rows * output);
@@ -274,7 +288,7 @@ rr_status rr_grouped_gated_gemm(const void* x_permuted, const void* gate_weights
   if (s.code != RR_SUCCESS) return s;
   const Activation act = static_cast<Activation>(activation);
   const char* what = "grouped_gated_gemm launch failed";
-  if (gated_few(route_pairs, experts, t)) {
+  if (gated_few(route_pairs, experts, hidden, output, t)) {
     return launched(rrb::launch_gated_few(x_permuted, gate_weights, up_weights, offsets, h,
                                           gate_up, route_pairs, experts, hidden, output, act, t,
                                           stream_of(ctx)),
