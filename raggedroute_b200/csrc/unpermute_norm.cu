@@ -671,7 +671,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1) unpermute_norm_stream_kerne
   using namespace sm100;
   extern __shared__ __align__(16) char rings[];
   __shared__ StreamSmem s;
-  __shared__ float parts[2][kMaxTeams];  // sums of each warp
+  __shared__ float parts[2][kMaxTeams];  // each warp's share of a sum
   stream_setup(st, in.top_k, s);
   follow_previous();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -684,16 +684,22 @@ __global__ void __launch_bounds__(kStreamThreads, 1) unpermute_norm_stream_kerne
   for (int q = 0; q < kElems / kPer; ++q) {
     column_factors<kPer>(in, (q * st.team + tid) * kPer, pg + q * kPer, pr + q * kPer);
   }
-  auto team_sum = [&](float v, int which) {
+  // Sums take the rows of `parts` in turn, across tokens too: between a sum's reads
+  // and the writes of the next one in its row lies the barrier of the sum between
+  // them, whatever other barriers a token has.
+  int turn = 0;
+  auto team_sum = [&](float v) {
     v = warp_sum(v);
     if (team_warps == 1) {
       __syncwarp();
       return v;
     }
-    if (lane == 0) parts[which][warp] = v;
+    float* shares = parts[turn];
+    turn ^= 1;
+    if (lane == 0) shares[warp] = v;
     team_sync(team, st.team);
     float sum = 0.0f;
-    for (int w = 0; w < team_warps; ++w) sum += parts[which][warp0 + w];
+    for (int w = 0; w < team_warps; ++w) sum += shares[warp0 + w];
     return sum;
   };
   Sources src;
@@ -709,7 +715,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1) unpermute_norm_stream_kerne
       float sq = 0.0f;
 #pragma unroll
       for (int i = 0; i < kElems; ++i) sq = fmaf(c[i], c[i], sq);
-      i1 = rsqrtf(team_sum(sq, 0) * per_col + in.eps);
+      i1 = rsqrtf(team_sum(sq) * per_col + in.eps);
     } else {
       team_sync(team, st.team);
     }
@@ -733,7 +739,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1) unpermute_norm_stream_kerne
     }
     float i2 = 1.0f;
     if (in.pre_gamma != nullptr) {
-      i2 = rsqrtf(team_sum(sq, 1) * per_col + in.eps);
+      i2 = rsqrtf(team_sum(sq) * per_col + in.eps);
 #pragma unroll
       for (int q = 0; q < kElems / kPer; ++q) {
         const int col = (q * st.team + tid) * kPer;
