@@ -960,7 +960,8 @@ __global__ void __launch_bounds__(kStreamThreads, 1) unpermute_norm_backward_str
 #pragma unroll
       for (int i = 0; i < kPairs; ++i) {
         c[i] = mul2(i12[i], c[i]);
-        rn[i] = mul2(i22[i], fma2(scale, x[i], mul2(c[i], f[i])));
+        // Without the second norm r' takes no part, whatever it holds.
+        rn[i] = pre ? mul2(i22[i], fma2(scale, x[i], mul2(c[i], f[i]))) : f2(0.0f);
       }
       if (has_dro) {
         staged_row<T, kPer>(ring + start[at_dro], n, st.team, tid, a);
@@ -1037,7 +1038,12 @@ __global__ void __launch_bounds__(kStreamThreads, 1) unpermute_norm_backward_str
     auto sum_of = [&](float v, int j) { return __shfl_sync(0xffffffffu, v, 4 * j); };
     const float sums01 = team_sums(0);
     const float im2 = i2 * (sum_of(sums01, 6) * per_col);
-    auto p_of = [&](float v, int h) { return sum_of(v, 3 * h) - im2 * sum_of(v, 3 * h + 1); };
+    // Terms of a norm that is left out are not added as zero times something: a row
+    // that is not finite would spread to the token's other results.
+    auto p_of = [&](float v, int h) {
+      const float p = sum_of(v, 3 * h), r = sum_of(v, 3 * h + 1);
+      return pre ? p - im2 * r : p;
+    };
     float m1 = 0.0f;
     for (int k = 0; k < (kTwo ? 1 : in.top_k); k += 2) {
       const float v = k == 0 ? sums01 : team_sums(k);
@@ -1051,7 +1057,8 @@ __global__ void __launch_bounds__(kStreamThreads, 1) unpermute_norm_backward_str
       const float v = k == 0 ? sums01 : team_sums(k);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const float d = i1 * (p_of(v, h) - m1 * sum_of(v, 3 * h + 2));
+        const float p = p_of(v, h), cy = sum_of(v, 3 * h + 2);
+        const float d = post ? i1 * (p - m1 * cy) : p;
         if (lane == 0 && k + h < in.top_k) {
           g.d_route_weights[t * in.top_k + k + h] = start[k + h] >= 0 ? d : 0.0f;
         }
@@ -1068,8 +1075,9 @@ __global__ void __launch_bounds__(kStreamThreads, 1) unpermute_norm_backward_str
     }
     put_row<T, kPer>(static_cast<T*>(g.d_residual) + t * n, n, st.team, tid, x);
 #pragma unroll
-    for (int i = 0; i < kPairs; ++i) {
-      a[i] = mul2(i12[i], fma2(nm1, c[i], mul2(f[i], a[i])));  // dc
+    for (int i = 0; i < kPairs; ++i) {  // dc
+      a[i] = mul2(f[i], a[i]);
+      if (post) a[i] = mul2(i12[i], fma2(nm1, c[i], a[i]));
     }
     auto put_route = [&](int k) {
       if (start[k] < 0) return;
