@@ -75,6 +75,9 @@ __device__ __forceinline__ void few_rows(const T* __restrict__ x, const T* __res
   const int sum_row = warp / kWide;
   const int part = static_cast<int>(sm100::cluster_ctarank());
   const int stride = split * kGroups;
+  // A block's shared memory may be written by its cluster only once it runs: each
+  // says so here, and the others wait for that behind the weights, for nothing.
+  if (split > 1) sm100::cluster_arrive();
   const int col = (threadIdx.x % kLanes) * kVec;
   const int kg = threadIdx.x / kLanes;
   float g[kR][kVec], u[kR][kVec];
@@ -152,6 +155,7 @@ __device__ __forceinline__ void few_rows(const T* __restrict__ x, const T* __res
     }
   }
   if (split > 1) {
+    sm100::cluster_wait();
     if (part > 0 && i < kR) {
       const uint32_t to = sm100::mapa_shared(sm100::smem_u32(&s.parts[part - 1][i][0][c]), 0u);
       sm100::st_shared_cluster_u32(to, __float_as_uint(sg));
