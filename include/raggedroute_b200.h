@@ -440,8 +440,9 @@ enum { RR_ACTIVATION_SILU = 0, RR_ACTIVATION_GELU_TANH = 1, RR_ACTIVATION_RELU =
  * dtype; sums in FP32, one rounding of h. gate_up (FP32 [R, 2N], may be NULL)
  * receives both products (gate columns, then up), which the backward pass
  * reads. FP32 operands are multiplied as three bfloat16 parts each (error of
- * an FP32 product; a row or weight that holds an infinity may give NaN where
- * FP32 arithmetic gives infinity). ctx->workspace (256-byte aligned) holds
+ * an FP32 product; where FP32 arithmetic gives infinity, by an operand or by
+ * overflow, the result may be NaN, and one within 2^-6 of the largest float may
+ * overflow). ctx->workspace (256-byte aligned) holds
  * rr_grouped_gated_gemm_workspace_size bytes: 0 for bfloat16 with K and N
  * multiples of 8 and for few rows; otherwise copies of the operands that the
  * tensor cores can read (FP32: 6 bytes per element of x and of both weights).

@@ -28,8 +28,9 @@
 // is transposed.
 //
 // FP32 (three parts per operand): each operand is the exact sum of three bfloat16 parts
-// (8 + 8 + 8 significand bits), and the product sums the six part products of
-// weight 2^-16 and above; what is left out is below 2^-23 of |a||b|. The
+// (8 + 8 + 8 significand bits, each part rounded to nearest: at most 1, 2^-8 and
+// 2^-17 of it), and the product sums the six part products of weight 2^-17 and above;
+// what is left out is at most 2^-24 of |a||b| and has either sign. The
 // tensor core truncates when it accumulates, with a bias that grows with the
 // number of steps taken at full magnitude, so every k-block is its own
 // accumulation, small products first (four full-magnitude steps), and the

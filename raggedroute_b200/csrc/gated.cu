@@ -410,28 +410,34 @@ __global__ void __launch_bounds__(kFewThreads) gated_few_dw_kernel(
 
 // ---- operand parts -----------------------------------------------------------------
 
-// v as the exact sum of three bfloat16 values: each takes the top 8
-// significand bits of what is left (truncation, so nothing overflows).
-// Infinity and NaN stay in the first part.
-__device__ __forceinline__ void split3(float v, uint16_t (&part)[3]) {
-  const uint32_t bits = __float_as_uint(v);
-  if ((bits & 0x7F800000u) == 0x7F800000u) {
-    part[0] = static_cast<uint16_t>(bits >> 16) | ((bits & 0x007FFFFFu) != 0 ? 0x40u : 0u);
-    part[1] = part[2] = 0;
-    return;
+// Two values as sums of three bfloat16 values each (a in the low halves), exact from
+// 2^-110 on, below within 2^-134: each part is what is left, rounded to nearest, so
+// that the parts have either sign and the products of them that are left out do not
+// lean one way (cut off instead, the parts have the value's sign, and what is left out
+// of a product reaches 2^-21 of it, always towards zero).
+__device__ __forceinline__ void split3(float a, float b, uint32_t (&w)[3]) {
+  w[0] = pack_bf16x2(a, b);
+  if ((((w[0] & 0x7F807F80u) + 0x00800080u) & 0x80008000u) != 0) {
+    // Not finite, or rounded up to infinity: the first part cuts off. Infinity and NaN
+    // stay in it.
+    auto first = [](float v) {
+      const uint32_t bits = __float_as_uint(v);
+      return (bits & 0xFFFF0000u) | ((bits & 0x7FFFFFFFu) > 0x7F800000u ? 0x400000u : 0u);
+    };
+    w[0] = (first(a) >> 16) | first(b);
   }
-  float rest = v;
-#pragma unroll
-  for (int i = 0; i < 3; ++i) {
-    const uint32_t b = __float_as_uint(rest) & 0xFFFF0000u;
-    part[i] = static_cast<uint16_t>(b >> 16);
-    rest -= __uint_as_float(b);
-  }
+  auto rest = [](float v, uint32_t part) {
+    return (part & 0x7F800000u) == 0x7F800000u ? 0.0f : v - __uint_as_float(part);
+  };
+  a = rest(a, w[0] << 16);
+  b = rest(b, w[0] & 0xFFFF0000u);
+  w[1] = pack_bf16x2(a, b);
+  w[2] = pack_bf16x2(a - __uint_as_float(w[1] << 16), b - __uint_as_float(w[1] & 0xFFFF0000u));
 }
 
 // Eight values as one 16-byte store per part; planes `plane` elements apart. One
 // part: rounded to nearest. Two: what the first leaves, rounded again (16
-// significand bits). Three: the exact FP32 value.
+// significand bits). Three: the FP32 value (split3).
 template <int kTerms>
 __device__ __forceinline__ void store_parts(__nv_bfloat16* dst, long long plane,
                                             const float (&v)[8]) {
@@ -448,18 +454,12 @@ __device__ __forceinline__ void store_parts(__nv_bfloat16* dst, long long plane,
     *reinterpret_cast<uint4*>(dst) = top;
     *reinterpret_cast<uint4*>(dst + plane) = pack16<__nv_bfloat16>(lo);
   } else {
-    uint32_t w[3][4];
+    uint32_t w[4][3];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      uint16_t lo[3], hi[3];
-      split3(v[2 * i], lo);
-      split3(v[2 * i + 1], hi);
-#pragma unroll
-      for (int q = 0; q < 3; ++q) w[q][i] = lo[q] | (static_cast<uint32_t>(hi[q]) << 16);
-    }
+    for (int i = 0; i < 4; ++i) split3(v[2 * i], v[2 * i + 1], w[i]);
 #pragma unroll
     for (int q = 0; q < 3; ++q) {
-      *reinterpret_cast<uint4*>(dst + q * plane) = make_uint4(w[q][0], w[q][1], w[q][2], w[q][3]);
+      *reinterpret_cast<uint4*>(dst + q * plane) = make_uint4(w[0][q], w[1][q], w[2][q], w[3][q]);
     }
   }
 }
@@ -537,7 +537,7 @@ __global__ void __launch_bounds__(kPackThreads) pack_terms_kernel(const PackJobs
 //   dg = dh * u * act'(g), du = dh * act(g).
 // Written as the engine's operand parts: for bfloat16 one rounding, which every
 // tensor-core operand takes, or two parts (see gradient_parts in block_api.cpp);
-// for FP32 three exact parts. Bound by its bytes.
+// for FP32 three parts (split3). Bound by its bytes.
 template <typename T, int kTerms, bool kVec>
 __global__ void __launch_bounds__(kPackThreads) gated_pointwise_backward_kernel(
     const float* __restrict__ gate_up, const T* __restrict__ dh, __nv_bfloat16* __restrict__ dg,
