@@ -195,8 +195,11 @@ __device__ __forceinline__ float activate(int activation, float g, float* deriva
   if (activation == static_cast<int>(Activation::kGeluTanh)) {
     const float t = tanhf(kGeluC * (g + kGeluA * g * g * g));
     if (derivative != nullptr) {
+      // t is 1 or -1 long before 32, and the second term zero; beyond, its square would
+      // overflow against that zero. NaN passes.
+      const float c = g > 32.0f ? 32.0f : (g < -32.0f ? -32.0f : g);
       *derivative = 0.5f * (1.0f + t) +
-                    0.5f * g * (1.0f - t * t) * kGeluC * (1.0f + 3.0f * kGeluA * g * g);
+                    0.5f * c * (1.0f - t * t) * kGeluC * (1.0f + 3.0f * kGeluA * c * c);
     }
     return 0.5f * g * (1.0f + t);
   }
