@@ -497,6 +497,8 @@ struct Filler {
                          : "memory");
           }
         }
+        // This lane's later copies into the same place come after these stores.
+        fence_proxy_async_smem();
       }
       total = __reduce_add_sync(0xffffffffu, size);
     }

@@ -6,7 +6,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from test_gpu_unpermute_norm import BF16, EPS, FP32, Inputs, check_forward
+from test_gpu_unpermute_norm import BF16, EPS, FP32, Inputs, check_backward, check_forward
 
 pytestmark = pytest.mark.gpu
 
@@ -81,3 +81,19 @@ def test_gradient_without_the_last_norm_of_a_residual_that_is_not_finite(cuda, s
     for name, t in clean.items():
         if t is not None:
             assert torch.equal(got[name], t), name
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("shape", [(1650, 2, 1027), (8003, 3, 333), (21000, 1, 131)], ids=str)
+def test_the_last_row_comes_first(cuda, shape, dtype):
+    """The buffer's last row, whose end is copied by element, among the first tokens:
+    later rows are copied into the same place whole."""
+    i = Inputs(*shape, dtype, cuda, 71)
+    flat = i.pos.view(-1)
+    for token in (0, 1, 5):
+        last = int((flat == flat.numel() - 1).nonzero()[0, 0])
+        to = token * shape[1]
+        flat[last], flat[to] = flat[to].item(), flat[last].item()
+        out, normed, inv = i.forward()
+        check_forward(i, out, normed, dtype)
+        check_backward(i, i.backward(inv), dtype)
