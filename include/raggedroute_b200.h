@@ -446,6 +446,8 @@ enum { RR_ACTIVATION_SILU = 0, RR_ACTIVATION_GELU_TANH = 1, RR_ACTIVATION_RELU =
  * rr_grouped_gated_gemm_workspace_size bytes: 0 for bfloat16 with K and N
  * multiples of 8 and for few rows; otherwise copies of the operands that the
  * tensor cores can read (FP32: 6 bytes per element of x and of both weights).
+ * The sizes of both workspaces never fall with route_pairs: one for the largest
+ * batch serves every smaller one.
  * x, the weights, h and gate_up: 16-byte aligned where their rows are a
  * multiple of 16 bytes. */
 rr_status rr_grouped_gated_gemm(const void* x_permuted, const void* gate_weights,

@@ -195,6 +195,31 @@ GatedPlan gated_plan(int rows, int experts, int hidden, int output, Dtype dtype,
   return p;
 }
 
+// Workspace bytes that serve any number of rows up to `rows`. A call's own need
+// (gated_plan) falls where more rows take a form that needs less: from the engine to
+// the plain form in FP32, whose estimate steps with the tiles, and from two parts of dg
+// and du to one.
+std::size_t gated_workspace(int rows, int experts, int hidden, int output, Dtype dtype,
+                            bool backward) {
+  auto need = [&](long long r) {
+    return gated_plan(static_cast<int>(r), experts, hidden, output, dtype, backward).total;
+  };
+  std::size_t most = need(rows);
+  auto also = [&](long long r) {
+    if (r < rows && need(r) > most) most = need(r);
+  };
+  if (backward) {
+    also(32LL * experts);  // the most rows with two parts
+  } else if (dtype == Dtype::kFp32) {
+    // Within a step the rows of the plain form come first, so the engine's largest need
+    // up to `rows` is at `rows` or at a step's end.
+    const long long step = 256LL * experts;
+    const long long last = rows < 65535 ? rows : 65535;
+    for (long long r = step; r <= last; r += step) also(r);
+  }
+  return most;
+}
+
 rr_status check_gated(int route_pairs, int experts, int hidden, int output, int activation) {
   if (experts <= 0 || experts > RR_MAX_EXPERTS || route_pairs < 0 || hidden <= 0 || output <= 0 ||
       hidden > kMaxDim || output > kMaxDim / 2 || route_pairs > INT_MAX - 512) {
@@ -239,7 +264,7 @@ size_t rr_grouped_gated_gemm_workspace_size(int route_pairs, int experts, int hi
       (dtype != RR_DTYPE_FP32 && dtype != RR_DTYPE_BF16)) {
     return 0;
   }
-  return gated_plan(route_pairs, experts, hidden, output, static_cast<Dtype>(dtype), false).total;
+  return gated_workspace(route_pairs, experts, hidden, output, static_cast<Dtype>(dtype), false);
 }
 
 size_t rr_grouped_gated_gemm_backward_workspace_size(int route_pairs, int experts, int hidden,
@@ -248,7 +273,7 @@ size_t rr_grouped_gated_gemm_backward_workspace_size(int route_pairs, int expert
       (dtype != RR_DTYPE_FP32 && dtype != RR_DTYPE_BF16)) {
     return 0;
   }
-  return gated_plan(route_pairs, experts, hidden, output, static_cast<Dtype>(dtype), true).total;
+  return gated_workspace(route_pairs, experts, hidden, output, static_cast<Dtype>(dtype), true);
 }
 
 rr_status rr_grouped_gated_gemm(const void* x_permuted, const void* gate_weights,
