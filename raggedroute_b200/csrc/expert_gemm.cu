@@ -78,6 +78,9 @@ constexpr int kEpiWarps = 8;
 constexpr int kThreads = (kEpiWarp0 + kEpiWarps) * 32;
 constexpr uint64_t kDrainNs = 2000000;
 constexpr int kPolls = 256;
+// What a k-block may take beyond the limit of a wait (0.4 us where the tensor pipe is
+// full), for the waits that last as long as a tile's contraction.
+constexpr uint64_t kBlockLimitNs = 4000;
 constexpr int kStagingBytes = 32 * 64;  // 64 bytes of 32 rows, per epilogue warp
 
 // A stage holds one k-block: kPa parts of A and kPb parts of B, 16 KB each.
@@ -370,13 +373,14 @@ __global__ void __launch_bounds__(kThreads, 1) expert_gemm_kernel(
   const uint32_t tmem = s.tmem_base;
   volatile int* failed = &s.failed;
   const uint32_t peer_failed = mapa_shared(smem_u32(&s.failed), rank ^ 1);
-  auto wait = [&](uint64_t* bar, uint32_t parity) {
+  auto wait = [&](uint64_t* bar, uint32_t parity, int blocks = 0) {
     // Most waits end within microseconds: poll before reading any clock.
 #pragma unroll 1
     for (int i = 0; i < kPolls; ++i) {
       if (mbar_try_wait(bar, parity)) return true;
     }
-    return mbar_wait_pair(bar, parity, p.err, failed, peer_failed);
+    return mbar_wait_pair(bar, parity, p.err, failed, peer_failed,
+                          kWaitLimitNs + static_cast<uint64_t>(blocks) * kBlockLimitNs);
   };
   auto tile = [&](int t) { return tile_at<kMode>(p, t, s.prefix, n_tiles); };
 
@@ -517,7 +521,7 @@ __global__ void __launch_bounds__(kThreads, 1) expert_gemm_kernel(
         const int valid = (g.row_end - g.row0) & 63;
         if (valid == 0) continue;
         const int stage = (at + kStages - 1) % kStages;  // of the last block
-        if (!wait(&s.tail[stage], (phases >> stage) & 1u)) break;
+        if (!wait(&s.tail[stage], (phases >> stage) & 1u, g.k_blocks)) break;
         phases ^= 1u << stage;
         // Lines past the segment's end hold other segments' rows (or
         // anything): both operands become zero there. A line is one row of a
@@ -632,7 +636,7 @@ __global__ void __launch_bounds__(kThreads, 1) expert_gemm_kernel(
         }
       };
       auto take = [&]() {  // the accumulator is finished
-        if (!wait(&s.tmem_full[buf], acc_phase)) return false;
+        if (!wait(&s.tmem_full[buf], acc_phase, g.k_blocks)) return false;
         tc_fence_after();
         return true;
       };
