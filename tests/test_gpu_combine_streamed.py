@@ -97,3 +97,84 @@ def test_the_last_row_comes_first(cuda, shape, dtype):
         out, normed, inv = i.forward()
         check_forward(i, out, normed, dtype)
         check_backward(i, i.backward(inv), dtype)
+
+
+# Teams of one warp to sixteen, a wide row, two routes or more, rows of whole granules,
+# of pairs and of single elements; tokens that end inside a stage.
+GRADIENT_PARTS = [(1201, 2, 250), (600, 2, 512), (601, 4, 264), (601, 2, 4096), (599, 2, 4095),
+                  (301, 3, 2050), (299, 2, 8192), (1201, 16, 520)]
+
+
+def inverse(i: Inputs):
+    """The forward pass's inv_rms."""
+    return i.forward()[2]
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("parts", PARTS, ids=str)
+@pytest.mark.parametrize("shape", GRADIENT_PARTS, ids=str)
+def test_gradient(cuda, shape, parts, dtype):
+    post, gate, pre = map(bool, parts)
+    i = Inputs(*shape, dtype, cuda, 81, post=post, gate=gate, pre=pre, skip=True)
+    inv = inverse(i)
+    got = i.backward(inv)
+    check_backward(i, got, dtype)
+    again = i.backward(inv)
+    i.dro = d = i.dro.clone()
+    in_place = i.backward(inv, d_residual=d)  # d_residual over d_residual_out
+    for name, t in got.items():
+        assert t is None or torch.equal(t, again[name]) and torch.equal(t, in_place[name]), name
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("post", [True, False])
+@pytest.mark.parametrize("shape", GRADIENT_PARTS, ids=str)
+def test_gradients_that_are_not_given(cuda, shape, post, dtype):
+    """No d_residual_out, no d_normed, neither: as if they were zero."""
+    i = Inputs(*shape, dtype, cuda, 82, post=post, skip=True)
+    inv = inverse(i)
+    dro, dn = i.dro, i.dn
+    for without in ("dro", "dn"):
+        i.dro, i.dn = dro, dn
+        setattr(i, without, None)
+        got = i.backward(inv)
+        setattr(i, without, torch.zeros_like(dn))
+        check_backward(i, got, dtype)
+    i.dro = i.dn = None
+    for name, t in i.backward(inv).items():
+        if name == "d_yp":
+            t = t[t != 7.0]  # rows that no route names
+        assert t is None or not t.any(), name
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("shape", [(300, 1, 200), (300, 1, 512), (300, 1, 511), (300, 1, 4100),
+                                   (5, 1, 33)], ids=str)
+def test_weight_gradient_of_a_single_route(cuda, shape, dtype):
+    """With a norm of c and one route the weight's gradient cancels but for eps:
+      d_w = i1 (<v1, y> - m1 <cn, y>),  v1 = gate post dr,  m1 = mean(v1 cn).
+    Each value is within u = (64 + top_k) 2^-24 of the magnitudes it is summed from: dr of
+    |dro| + i2 (|v| + |rn| m2), m2 of mean |v||rn|; v1, cn and the dot products three
+    more times that, so 4 u of the products' magnitudes."""
+    i = Inputs(*shape, dtype, cuda, 83)
+    inv = inverse(i)
+    got = i.backward(inv)["d_w"][:, 0].double()
+    yp, w, res, post, gate, pre = (t.detach() for t in i.leaves())
+    y = yp[i.pos[:, 0].long()]
+    c = w * y
+    i1 = 1 / torch.sqrt((c * c).mean(1, keepdim=True) + EPS)
+    cn = c * i1
+    r = i.scale * res + gate * post * cn
+    i2 = 1 / torch.sqrt((r * r).mean(1, keepdim=True) + EPS)
+    rn, v = r * i2, i.dn.double() * pre
+    dr = i.dro.double() + i2 * (v - rn * (v * rn).mean(1, keepdim=True))
+    v1 = gate * post * dr
+    m1 = (v1 * cn).mean(1, keepdim=True)
+    want = (i1 * ((v1 * y).sum(1, keepdim=True) - m1 * (cn * y).sum(1, keepdim=True)))[:, 0]
+    big = (gate * post).abs() * (i.dro.double().abs() + i2 * (
+        v.abs() + rn.abs() * (v * rn).abs().mean(1, keepdim=True)))
+    big_m1 = (big * cn.abs()).mean(1, keepdim=True)
+    size = (i1 * ((big * y.abs()).sum(1, keepdim=True)
+                  + big_m1 * (cn * y).abs().sum(1, keepdim=True)))[:, 0]
+    assert bool(((got - want).abs() <= 4 * 65 * 2.0 ** -24 * size).all())
+    assert float((4 * 65 * 2.0 ** -24 * size).max()) < 0.3
