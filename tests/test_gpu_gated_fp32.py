@@ -2,12 +2,13 @@
 runs."""
 from __future__ import annotations
 
+import numpy as np
 import pytest
 import torch
 
 import raggedroute_b200 as rr
-from expert_block_reference import offsets_of
-from test_gpu_gated import backward, forward, no_device_error
+from expert_block_reference import ACTIVATIONS, gated, gated_backward, normwise, offsets_of
+from test_gpu_gated import FP32, backward, forward, make, no_device_error, workspace
 
 pytestmark = pytest.mark.gpu
 
@@ -98,3 +99,129 @@ def test_products_of_any_magnitude(cuda):
     assert bool(((gu.double() - want).abs() <= tol)[inside].all())
     assert not torch.isfinite(gu[want.abs() > 2.0 ** 128]).any()
     assert bool((gu.double()[want.abs() < 2.0 ** -100].abs() <= 2.0 ** -99).all())
+
+
+K, N = 520, 264  # the tensor-core form from a few hundred rows on
+
+
+@pytest.mark.parametrize("activation", ACTIVATIONS)
+def test_activations(cuda, activation):
+    x, wg, wu, off, dh = make([700], 0, K, N, FP32, cuda, seed=9)
+    wg = wg * 3
+    assert takes_tensor_cores(x, wg, wu, off)
+    h, gu = forward(x, wg, wu, off, activation)
+    grads = backward(x, wg, wu, off, gu, dh, activation)
+    assert normwise(h, gated(x, wg, wu, off, activation)[2]) < 2.0 ** -19
+    for got, want in zip(grads, gated_backward(x, wg, wu, off, dh, activation)):
+        assert normwise(got, want) < 2.0 ** -19
+
+
+def test_other_segments_do_not_leak(cuda):
+    """Infinities and NaN in one expert's rows and weights stay out of the others', and
+    of the rows behind the last segment."""
+    counts = [270, 290, 265]
+    x, wg, wu, off, dh = make(counts, 9, K, N, FP32, cuda, seed=11)
+    assert takes_tensor_cores(x, wg, wu, off)
+    h, gu = forward(x, wg, wu, off)
+    clean = backward(x, wg, wu, off, gu, dh)
+    x2, dh2, wg2 = x.clone(), dh.clone(), wg.clone()
+    x2[270:560:2], x2[271:560:2], x2[825:] = float("inf"), float("nan"), float("nan")
+    dh2[270:560] = float("nan")
+    wg2[1, 3] = float("inf")
+    h2, gu2 = forward(x2, wg2, wu, off)
+    dirty = backward(x2, wg2, wu, off, gu2, dh2)
+    for rows in (slice(0, 270), slice(560, 825)):
+        assert torch.equal(h2[rows], h[rows]) and torch.equal(gu2[rows], gu[rows])
+        assert torch.equal(dirty[0][rows], clean[0][rows])
+    for e in (0, 2):
+        assert torch.equal(dirty[1][e], clean[1][e]) and torch.equal(dirty[2][e], clean[2][e])
+    assert not torch.isfinite(h2[270:560]).any() and not torch.isfinite(dirty[1][1]).any()
+    assert bool((h2[825:] == 777.0).all()) and bool((dirty[0][825:] == 777.0).all())
+
+
+def test_saturated_activation(cuda):
+    """Gates far out in both directions: exp overflows and underflows."""
+    x = torch.ones(700, K, device=cuda)
+    wg = torch.zeros(1, K, N, device=cuda)
+    wg[0, 0] = torch.linspace(-400, 400, N).to(cuda)
+    wu = torch.zeros_like(wg)
+    wu[0, :8] = 0.125
+    off = offsets_of([700], cuda)
+    assert takes_tensor_cores(x, wg, wu, off)
+    h, gu = forward(x, wg, wu, off)
+    want = gated(x, wg, wu, off)[2]
+    # The gate is exact in three parts; expf, the division and the product: 8 steps.
+    assert bool(((h.double() - want).abs() <= 2.0 ** -21 * want.abs() + 1e-30).all())
+    assert all(torch.isfinite(t).all() for t in backward(x, wg, wu, off, gu, torch.ones_like(h)))
+
+
+def test_repeats_bit_for_bit_and_replays(cuda):
+    """Equal results in a second call and in a captured graph replayed on new inputs."""
+    x, wg, wu, off, dh = make([310, 0, 500, 33], 0, K, N, FP32, cuda, seed=20)
+    assert takes_tensor_cores(x, wg, wu, off)
+    ws = workspace(x, wg)
+    h, gu = torch.zeros(843, N, device=cuda), torch.zeros(843, 2 * N, device=cuda)
+    out = [torch.zeros_like(t) for t in (x, wg, wu)]
+    bufs = [t.clone() for t in (x, off, dh)]
+
+    def train(ctx):
+        rr.grouped_gated_gemm(bufs[0], wg, wu, bufs[1], h, gate_up=gu, workspace=ws, ctx=ctx)
+        rr.grouped_gated_gemm_backward(bufs[0], wg, wu, bufs[1], gu, bufs[2], *out, workspace=ws,
+                                       ctx=ctx)
+
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    graph = rr.Graph.capture(train, s)
+    x2, _, _, off2, dh2 = make([0, 800, 43, 0], 0, K, N, FP32, cuda, seed=33)
+    for xs, offs, ds in ((x, off, dh), (x2, off2, dh2)):
+        want = forward(xs, wg, wu, offs)
+        want += backward(xs, wg, wu, offs, want[1], ds)
+        again = forward(xs, wg, wu, offs)
+        assert all(torch.equal(a, b) for a, b in zip(want, again))
+        for dst, src in zip(bufs, (xs, offs, ds)):
+            dst.copy_(src)
+        torch.cuda.synchronize()
+        for _ in range(2):
+            graph.launch(s)
+            s.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip((h, gu, *out), want))
+    no_device_error()
+
+
+@pytest.mark.parametrize("shift", range(1, 4))
+def test_buffers_that_start_anywhere(cuda, shift):
+    """Rows of no multiple of 16 bytes, packed from buffers that start at any element
+    between values that are not theirs, into buffers between canaries."""
+    k, n = K - 1, N - 1
+    x, wg, wu, off, _ = make([400, 0, 500], 0, k, n, FP32, cuda, seed=60)
+    assert takes_tensor_cores(x, wg, wu, off)
+
+    def moved(t, around):
+        buf = torch.full((t.numel() + 16,), around, device=cuda)
+        view = buf[shift:shift + t.numel()].view(t.shape)
+        return buf, view.copy_(t)
+
+    h, gu = forward(x, wg, wu, off)
+    hb, h2 = moved(torch.zeros_like(h), 9.0)
+    gb, gu2 = moved(torch.zeros_like(gu), 9.0)
+    nan = float("nan")
+    rr.grouped_gated_gemm(moved(x, nan)[1], moved(wg, nan)[1], moved(wu, nan)[1], off, h2,
+                          gate_up=gu2, workspace=workspace(x, wg))
+    assert torch.equal(h, h2) and torch.equal(gu, gu2)
+    for buf, t in ((hb, h), (gb, gu)):
+        assert bool((buf[:shift] == 9.0).all()) and bool((buf[shift + t.numel():] == 9.0).all())
+
+
+# (experts, K, N, the most rows of the plain form): N a multiple of 4 and not.
+@pytest.mark.parametrize("edge", [(3, 128, 128, 756), (6, 520, 264, 400), (5, 130, 129, 368),
+                                  (7, 333, 259, 208)], ids=str)
+def test_forms_meet(cuda, edge):
+    e, k, n, most = edge
+    for rows, engine in ((most, False), (most + 1, True)):
+        counts = np.random.default_rng(rows).multinomial(rows, [1 / e] * e)
+        x, wg, wu, off, _ = make(counts, 0, k, n, FP32, cuda, seed=81)
+        assert takes_tensor_cores(x, wg, wu, off) == engine
+        h, gu = forward(x, wg, wu, off)
+        g, u, want = gated(x, wg, wu, off)
+        assert normwise(h, want) < 2.0 ** -19
+        assert normwise(gu, torch.cat((g, u), 1)) < 2.0 ** -20
