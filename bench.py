@@ -1026,11 +1026,13 @@ def config_sweep(torch, rr, device, hbm_gbs: float, peak_3x: float, bf16_tflops:
 # reference CPU arm
 # ---------------------------------------------------------------------------
 
+NO_REFERENCE = ("oracle/_ref/librr_ref.so is missing (build it with python "
+                "oracle/build_oracle.py where the reference checkout exists)")
+
+
 def _ref_lib():
+    """The reference's CPU functions, or None where they were not built."""
     import oracle
-    if oracle.ref is None:
-        raise RuntimeError("oracle/_ref/librr_ref.so is missing (build it with "
-                           "python oracle/build_oracle.py where the reference checkout exists)")
     return oracle.ref
 
 
@@ -1066,6 +1068,8 @@ def cpu_baseline(inp, steps: int = 1, sample_tokens: int = 256) -> dict:
     passes), so equal per-token times at both sizes support extrapolating to
     the full batch."""
     ref = _ref_lib()
+    if ref is None:
+        return {"unavailable": NO_REFERENCE}
     threads = os.cpu_count() or 1
     x = inp.x[:sample_tokens].contiguous().cpu()
     wr, bias, we = inp.router_w.cpu(), inp.logit_bias.cpu(), inp.expert_w.cpu()
@@ -1104,6 +1108,8 @@ def run_reference(args, rank: int) -> dict | None:
     if rank != 0:
         return None
     ref = _ref_lib()
+    if ref is None:
+        return {"impl": "reference", "unavailable": NO_REFERENCE}
     threads = os.cpu_count() or 1
     sample = int(os.environ.get("RR_REF_SAMPLE_TOKENS", "256"))
     x, wr, bias, we = _sample_inputs(sample)
