@@ -25,8 +25,8 @@
 // take plain blocks (forward_streams and backward_streams say when).
 //
 // Top 2, both norms and the gate: bf16, 32768 tokens, N=4096 forward 253 us (5.3
-// TB/s), gradient 475 (4.5; its instructions issue 45% of the time with the 16
-// warps per SM that its registers allow); FP32, 16384 tokens, N=1024 60 and 95 (5.5 and
+// TB/s), gradient 470 (4.6; latency: the 16 warps per SM that its registers allow
+// issue 47% of the time, and DRAM is not full either); FP32, 16384 tokens, N=1024 60 and 95 (5.5 and
 // 5.7 TB/s); rows that are no multiple of 16 bytes 1.7 to 2.3 TB/s, their columns taken
 // singly or in pairs (bf16, N=1491, 2340). Tried for the gradient at N=4096 and slower:
 // two tokens per step (spills), sixteen columns per thread; a warp that only
