@@ -6,6 +6,7 @@ from __future__ import annotations
 import pytest
 import torch
 
+from expert_block_reference import half_step
 from test_gpu_unpermute_norm import BF16, EPS, FP32, Inputs, check_backward, check_forward
 
 pytestmark = pytest.mark.gpu
@@ -178,3 +179,97 @@ def test_weight_gradient_of_a_single_route(cuda, shape, dtype):
                   + big_m1 * (cn * y).abs().sum(1, keepdim=True)))[:, 0]
     assert bool(((got - want).abs() <= 4 * 65 * 2.0 ** -24 * size).all())
     assert float((4 * 65 * 2.0 ** -24 * size).max()) < 0.3
+
+
+def check_gradient_elementwise(i: Inputs, got, dtype):
+    """Every gradient within the first-order bound of FP32 arithmetic. Each value is
+    within u = (64 + top_k) 2^-24 of the magnitudes it is summed from, and carries on the
+    errors of what it is computed from (d*). Short rows need this: with N = 1 a norm's
+    1/rms reaches 1 / sqrt(eps) = 1000 and its gradient cancels all but eps of itself.
+    Twice the bound, for terms of second order and the grouping of the sums."""
+    yp, w, res, post, gate, pre = (t.detach() for t in i.leaves())
+    t, k, n = *i.pos.shape, i.res.shape[1]
+    u = (64 + k) * 2.0 ** -24
+    there = (i.pos >= 0) & (i.pos < t * k)
+    y = yp[i.pos.clamp(0, t * k - 1).long()] * there[..., None]
+    w = (w * there)[..., None]
+
+    def mean(v):
+        return v.mean(1, keepdim=True)
+
+    c, dc = (w * y).sum(1), u * (w * y).abs().sum(1)
+    i1 = 1 / torch.sqrt(mean(c * c) + EPS)
+    e1 = i1 * mean(dc * dc).sqrt() + u  # relative, of i1
+    cn, dcn = c * i1, i1 * dc + (c * i1).abs() * e1
+    f = gate * post
+    r = i.scale * res + f * cn
+    dr_ = u * (abs(i.scale) * res.abs() + (f * cn).abs()) + f.abs() * dcn
+    i2 = 1 / torch.sqrt(mean(r * r) + EPS)
+    e2 = i2 * mean(dr_ * dr_).sqrt() + u
+    rn, drn = r * i2, i2 * dr_ + (r * i2).abs() * e2
+    dro, dn = i.dro.double(), i.dn.double()
+    v = dn * pre
+    m2, dm2 = mean(v * rn), mean(v.abs() * (drn + u * rn.abs()))
+    x, big_x = v - rn * m2, v.abs() + (rn * m2).abs()
+    dr = dro + i2 * x
+    ddr = u * dro.abs() + i2 * ((u + e2) * big_x + drn * m2.abs() + rn.abs() * dm2)
+    v1, dv1 = f * dr, f.abs() * (ddr + u * (dro.abs() + i2 * big_x))
+    big_cn = i1 * (w * y).abs().sum(1)
+    m1 = mean(v1 * cn)
+    dm1 = mean(dv1 * big_cn + v1.abs() * (dcn + u * big_cn))
+    dct = i1 * (v1 - cn * m1)
+    ddct = i1 * ((u + e1) * (v1.abs() + (cn * m1).abs()) + dv1 + dcn * m1.abs() + cn.abs() * dm1)
+    half = half_step(dtype)
+    named = torch.zeros(t * k, dtype=torch.bool, device=yp.device)
+    named[i.pos[there].long()] = True
+    want_y, err_y = torch.zeros_like(yp), torch.zeros_like(yp)
+    want_y[i.pos[there].long()] = (w * dct[:, None])[there]
+    err_y[i.pos[there].long()] = (w.abs() * ddct[:, None])[there]
+    big_y = y.abs() * (i1 * (v1.abs() + (cn * m1).abs()))[:, None]
+    adds = (t / 148 + 400) * 2.0 ** -24  # of a column sum: tokens of a block, then blocks
+
+    def column(a, da, b, db):
+        return (a * b).sum(0), (da * b.abs() + a.abs() * db + adds * (a * b).abs()).sum(0)
+
+    checks = dict(
+        d_residual=(i.scale * dr, abs(i.scale) * ddr, half),
+        d_yp=(want_y, err_y, half),
+        d_w=((dct[:, None] * y).sum(2), (ddct[:, None] * y.abs() + u * big_y).sum(2), 0.0),
+        d_post=(*column(dr * gate, ddr * gate.abs(), cn, dcn), 0.0),
+        d_gate=(*column(dr, ddr, cn * post, dcn * post.abs()), 0.0),
+        d_pre=(*column(dn, u * dn.abs(), rn, drn), 0.0))
+    for name, (want, err, step) in checks.items():
+        g = got[name].double()
+        if name == "d_yp":
+            assert bool((g[~named] == 7.0).all())
+            g, want, err = g[named], want[named], err[named]
+        assert bool(((g - want).abs() <= 2 * err + step * want.abs() + 2.0 ** -100).all()), name
+
+
+# Rows of one element to a few, many of them in a granule, and some of each width.
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("shape", [(700001, 2, 1), (90001, 2, 7), (2500, 2, 1), (2501, 3, 2),
+                                   (1301, 16, 17), (601, 2, 4096), (599, 3, 4095), (300, 1, 8192),
+                                   (5, 2, 200)], ids=str)
+def test_gradient_elementwise(cuda, shape, dtype):
+    i = Inputs(*shape, dtype, cuda, 91, skip=True)
+    out, normed, inv = i.forward()
+    check_forward(i, out, normed, dtype)
+    check_gradient_elementwise(i, i.backward(inv), dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("shape", [(9, 2, 200), (1701, 2, 4096), (601, 2, 512), (1650, 2, 1027),
+                                   (700, 5, 520)], ids=str)
+def test_tokens_without_routes(cuda, shape, dtype):
+    """A padded batch: whole tokens, the first and last among them, whose routes went
+    nowhere. c is zero there, r' the scaled residual, and no weight has a gradient."""
+    i = Inputs(*shape, dtype, cuda, 92)
+    idle = torch.arange(0, shape[0], 4, device=cuda)
+    i.pos[idle], i.pos[-1] = -1, shape[0] * shape[1]
+    out, normed, inv = i.forward()
+    check_forward(i, out, normed, dtype)
+    got = i.backward(inv)
+    check_backward(i, got, dtype)
+    assert torch.equal(out[idle], (i.scale * i.res[idle].float()).to(dtype))
+    assert not got["d_w"][idle].any() and not got["d_w"][-1].any()

@@ -35,3 +35,5 @@ def test_a_contraction_of_seconds(cuda):
     g = 15 * torch.arange(1.0, n + 1, device=cuda)
     assert torch.equal(gu, torch.cat((g, torch.full_like(g, -30.0))).expand(rows, -1))
     assert torch.equal(h, (g * -30.0).to(BF16).expand(rows, -1))
+    del x, wg, wu
+    torch.cuda.empty_cache()  # 45 GB
